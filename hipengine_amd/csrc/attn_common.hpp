@@ -1,0 +1,164 @@
+// What the kernels of the attention half share: vector loads of activations, the position rotation, the geometry of
+// the 8-bit paged KV cache and the mapping of a ragged batch onto blocks of its tokens.
+//
+// KV cache. A page holds page_size tokens (a power of two, 32 or more) of every KV head; inside a (page, head) the
+// tokens lie in blocks of 32, and a block has one float32 scale for K and one for V. Values are bytes 128 + q with q in
+// -127..127 (excess-128 needs no sign extension on the way to fp16: the byte under the exponent of 1024.0 is a fp16
+// number, and one packed subtraction of 1152 gives q). Both block layouts are the operand order of
+// v_mfma_f32_32x32x16_f16, so that a wave's 16-byte loads are contiguous and nothing passes through LDS:
+//   K block  [D/16][32 tokens][16 dims]   lane (token, half) reads dims 16 (2i + half) .. + 15 as one load
+//   V block  [D][32 places]               token t at place (t & 3) | (t >> 3 & 3) << 2 | (t >> 2 & 1) << 4:
+//                                         lane (dim, half) reads the 16 tokens that the 32x32 accumulator of
+//                                         K Q^T leaves in that half of the wave, in the accumulator's register order
+#pragma once
+
+#include "gguf_common.hpp"
+
+namespace hipengine_gfx950 {
+
+constexpr int KV_BLOCK = 32;
+constexpr float KV_SCALE_FLOOR = 5.421010862427522e-20f;   // 2^-64: no block has a smaller scale
+
+struct KvCacheQ8 {
+  uint8_t* k;          // [pages, heads, page_size / 32, D * 32]
+  uint8_t* v;
+  float* k_scale;      // [pages, heads, page_size / 32]
+  float* v_scale;
+  const int32_t* table;   // [batch, table_stride] page numbers
+  int64_t table_stride;
+  int64_t pages;
+  int heads;
+  int page_log2;       // log2(page_size)
+};
+
+__device__ __forceinline__ int v_place(int t) { return (t & 3) | ((t >> 3 & 3) << 2) | ((t >> 2 & 1) << 4); }
+__device__ __forceinline__ int v_token(int p) { return (p & 3) | ((p >> 2 & 3) << 3) | ((p >> 4 & 1) << 2); }
+
+// Number of the 32-token block `blk` (of its sequence `seq`) of KV head `head` in the cache, or -1: behind the page
+// table, or on a page number outside the cache. Whatever a table holds, nothing outside the cache is addressed.
+__device__ __forceinline__ int64_t kv_block_index(const KvCacheQ8& c, int seq, int64_t blk, int head) {
+  const int per_page_log2 = c.page_log2 - 5;
+  const int64_t slot = blk >> per_page_log2;
+  if (slot >= c.table_stride) return -1;
+  const int64_t page = c.table[seq * c.table_stride + slot];
+  if (page < 0 || page >= c.pages) return -1;
+  return ((page * c.heads + head) << per_page_log2) + (blk & ((1 << per_page_log2) - 1));
+}
+
+// Rows [first, first + count) of sequence `seq` of a ragged batch, kept inside the batch whatever q_start holds.
+struct SeqRows {
+  int64_t first;
+  int64_t count;
+};
+__device__ __forceinline__ SeqRows seq_rows(const int32_t* __restrict__ q_start, int seq, int64_t tokens) {
+  const int64_t a = min(max(static_cast<int64_t>(q_start[seq]), int64_t{0}), tokens);
+  const int64_t b = min(max(static_cast<int64_t>(q_start[seq + 1]), a), tokens);
+  return {a, b - a};
+}
+
+// ---- vector loads and stores of 8 activations (element alignment is enough) ----------------------------------
+
+template <int KIND>
+__device__ __forceinline__ void load8_f32(const void* base, int64_t idx, float (&v)[8]) {
+  if constexpr (KIND == KIND_F32) {
+    __builtin_memcpy(v, __builtin_assume_aligned(static_cast<const float*>(base) + idx, 4), 32);
+  } else {
+    uint4 u;
+    __builtin_memcpy(&u, __builtin_assume_aligned(static_cast<const uint16_t*>(base) + idx, 2), 16);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (KIND == KIND_BF16) {
+        v[2 * i] = bits_to_float(w[i] << 16);
+        v[2 * i + 1] = bits_to_float(w[i] & 0xFFFF0000u);
+      } else {
+        v[2 * i] = f16_bits_to_float(w[i] & 0xFFFFu);
+        v[2 * i + 1] = f16_bits_to_float(w[i] >> 16);
+      }
+    }
+  }
+}
+
+// bf16 stores keep NaN a NaN (float_to_bf16_bits carries a NaN's low mantissa into the sign).
+__device__ __forceinline__ uint32_t bf16_bits_nan(float v) {
+  return v != v ? 0x7FC0u : static_cast<uint32_t>(float_to_bf16_bits(v));
+}
+
+template <int KIND>
+__device__ __forceinline__ uint32_t half_bits(float v) {
+  return KIND == KIND_BF16 ? bf16_bits_nan(v) : static_cast<uint32_t>(float_to_f16_bits(v));
+}
+
+template <int KIND>
+__device__ __forceinline__ void store8_f32(void* base, int64_t idx, const float (&v)[8]) {
+  if constexpr (KIND == KIND_F32) {
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<float*>(base) + idx, 4), v, 32);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = half_bits<KIND>(v[2 * i]) | (half_bits<KIND>(v[2 * i + 1]) << 16);
+    __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(base) + idx, 2), w, 16);
+  }
+}
+
+// ---- position rotation ---------------------------------------------------------------------------------------
+
+// cos and sin of position * inv_freq, times `scale`. The product and its reduction to a fraction of a turn are in 64
+// bits: at position 10^6 a 32-bit product is off by a tenth of a radian.
+__device__ __forceinline__ float2 rotation(int64_t position, float inv_freq, float scale) {
+  const double turns = static_cast<double>(position) * static_cast<double>(inv_freq) * 0.15915494309189535;
+  const float part = static_cast<float>(turns - rint(turns));   // -0.5 .. 0.5
+  float s, c;
+  sincospif(2.0f * part, &s, &c);
+  return make_float2(c * scale, s * scale);
+}
+
+// One head's RMS norm and rotation by the lanes that hold it, 8 values a lane.  `x` is the lane's own 8 values (head
+// dims 8 * slot ..), `src` the head in memory: a lane that needs the other half of its pairs reads them again (they are
+// in L1) instead of asking its neighbours.
+// `turn` holds (cos, sin) of the rotary_dim / 2 pairs.  rotary_dim is a multiple of 16, so a lane's 8 values lie on one
+// side of every border.
+template <int KIND, int D>
+__device__ __forceinline__ void norm_rotate8(float (&x)[8], const void* src, int64_t src_idx, int slot,
+                                             const float* __restrict__ weight, float eps, const float2* turn,
+                                             int rotary_dim, bool interleaved) {
+  constexpr int LANES = D / 8;
+  const int d0 = 8 * slot, pairs = rotary_dim >> 1;
+  const bool split = !interleaved && d0 < rotary_dim;
+  float y[8];
+  const int other = d0 < pairs ? d0 + pairs : d0 - pairs;
+  if (split) load8_f32<KIND>(src, src_idx + other, y);
+  if (weight) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) sum += __shfl_xor(sum, off);
+    const float r = 1.0f / sqrtf(sum * (1.0f / D) + eps);
+    float w[8];
+    load8_f32<KIND_F32>(weight, d0, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+    if (split) {
+      load8_f32<KIND_F32>(weight, other, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
+    }
+  }
+  if (split) {
+    const float sign = d0 < pairs ? -1.0f : 1.0f;
+    const float2* cs = turn + (d0 < pairs ? d0 : other);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i].x, sign * y[i] * cs[i].y);
+  } else if (interleaved && d0 < rotary_dim) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 cs = turn[(d0 >> 1) + i];
+      const float a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = fmaf(a, cs.x, -b * cs.y);
+      x[2 * i + 1] = fmaf(b, cs.x, a * cs.y);
+    }
+  }
+}
+
+}  // namespace hipengine_gfx950

@@ -1,0 +1,365 @@
+// The paged KV cache in 8 bits: appending tokens (with the keys' norm and rotation on the way) and reading them back.
+//
+// One float32 scale for each block of 32 tokens and head, K and V apart:
+//   scale' = max(scale of the tokens that stay, amax / 127, 2^-64),   byte = 128 + clamp(rint(x / scale'), -127, 127)
+// and where that is more than the old scale the tokens that stay are brought to it, q' = rint(q * scale / scale').
+// A block whose first token is among the appended ones starts anew: whatever it held, its old scale is not looked at.
+// A NaN or infinity among a block's new tokens makes its scale NaN, and with it everything that the block yields (8-bit
+// values have no place for one); it stays so until the block starts anew.  Bytes behind the appended tokens stay.
+//
+// Work is cut by (sequence, block, head, K or V), and one workgroup owns that piece: the only writer of the block's
+// scale and bytes, so there are no atomics and results do not depend on timing.  A piece reads and writes at most
+// 32 * D values; the launch is bound by HBM for prompts and by latency for single tokens.
+
+#include <hip/hip_runtime.h>
+
+#include "attn_common.hpp"
+
+#include "gguf_init.hpp"
+
+#include "../../include/hipengine_gfx950.h"
+
+namespace {
+
+using namespace hipengine_gfx950;
+
+constexpr int THREADS = 256;
+
+// Byte offset of the 16-byte item in a block, K or V: item i of K is dims 16 (i / 32) .. of token i % 32, item i of V is
+// places 16 (i % 2) .. of dim i / 2; in both layouts the items follow each other.
+__device__ __forceinline__ int item_offset(int item) { return item * 16; }
+
+// Which block of which sequence a workgroup works on.  With `per_seq` > 0 every sequence has that many blocks in the
+// grid; with 0 sequence b has floor(q_start[b] / 32) + 2b blocks in front of it, which leaves room for the most that its
+// tokens can touch (n tokens touch at most floor(n / 32) + 2 blocks) without a prefix sum over the batch.
+struct Piece {
+  int seq;
+  int64_t block;       // in its sequence
+  int first, last;     // tokens of the block that this call is about: [first, last), 0..32
+  int64_t row;         // row of the batch that token `first` is
+};
+
+__device__ __forceinline__ bool find_piece(const int32_t* __restrict__ q_start, const int32_t* __restrict__ kv_lens,
+                                           int64_t tokens, int batch, int per_seq, int64_t unit, int* found, Piece& p) {
+  int seq;
+  int64_t local;
+  if (per_seq > 0) {
+    seq = static_cast<int>(unit / per_seq);
+    local = unit - static_cast<int64_t>(seq) * per_seq;
+  } else {
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    int mine = -1;
+    for (int b = threadIdx.x; b < batch; b += THREADS)
+      if ((max(q_start[b], 0) >> 5) + 2 * static_cast<int64_t>(b) <= unit) mine = b;
+    if (mine >= 0) atomicMax(found, mine);
+    __syncthreads();
+    seq = *found;
+    if (seq < 0) return false;
+    local = unit - ((max(q_start[seq], 0) >> 5) + 2 * static_cast<int64_t>(seq));
+  }
+  const SeqRows rows = seq_rows(q_start, seq, tokens);
+  const int64_t end = kv_lens[seq];                  // place behind the last token
+  const int64_t begin = end - rows.count;            // place of the first row; rows at negative places are left out
+  const int64_t from = max(begin, int64_t{0});
+  p.seq = seq;
+  p.block = (from >> 5) + local;
+  const int64_t base = p.block << 5;
+  if (base >= end || rows.count <= 0) return false;
+  p.first = static_cast<int>(max(from - base, int64_t{0}));
+  p.last = static_cast<int>(min(end - base, int64_t{KV_BLOCK}));
+  p.row = rows.first + (base + p.first - begin);
+  return p.first < p.last;
+}
+
+struct AppendArgs {
+  KvCacheQ8 cache;
+  const void* k;
+  const void* v;
+  int64_t k_stride, v_stride;
+  const float* k_weight;
+  const int64_t* positions;
+  const float* inv_freq;
+  const int32_t* q_start;
+  const int32_t* kv_lens;
+  int64_t tokens;
+  int batch, per_seq, rotary_dim, interleaved;
+  float eps, rope_scale;
+};
+
+__device__ __forceinline__ uint32_t quantize(float x, float scale) {
+  return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(x / scale), -127.0f), 127.0f)) + 128);
+}
+__device__ __forceinline__ uint32_t requantize(uint32_t byte, float ratio) {
+  return static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(static_cast<int>(byte) - 128) * ratio)) + 128);
+}
+
+// grid (units, heads, 2): z 0 is K, z 1 is V.
+template <int KIND, int D>
+__global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendArgs a) {
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES, PAD = D + 4;
+  __shared__ float x[KV_BLOCK * PAD];
+  __shared__ float2 turn[ROWS][D / 2];
+  __shared__ float amax_of[THREADS / 64];
+  __shared__ int found;
+  const bool is_v = blockIdx.z != 0;
+  const int head = blockIdx.y;
+  Piece p;
+  if (!find_piece(a.q_start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, &found, p)) return;
+  const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
+  if (block < 0) return;
+
+  // The new tokens, normed and rotated, in float32 in LDS; their largest magnitude on the way.
+  const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  const void* src = is_v ? a.v : a.k;
+  const int64_t stride = is_v ? a.v_stride : a.k_stride;
+  float amax = 0.0f;
+  bool finite = true;
+  for (int t0 = p.first; t0 < p.last; t0 += ROWS) {
+    const int t = t0 + sub;
+    const int64_t row = p.row + (t - p.first);
+    float y[8];
+    if (t < p.last) load8_f32<KIND>(src, row * stride + static_cast<int64_t>(head) * D + 8 * slot, y);
+    if (!is_v && a.inv_freq) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < ROWS * (a.rotary_dim / 2); i += THREADS) {
+        const int r = i / (a.rotary_dim / 2), j = i - r * (a.rotary_dim / 2);
+        if (t0 + r < p.last) {
+          const int64_t at = a.positions ? a.positions[p.row + (t0 + r - p.first)] : (p.block << 5) + t0 + r;
+          turn[r][j] = rotation(at, a.inv_freq[j], a.rope_scale);
+        }
+      }
+      __syncthreads();
+    }
+    if (t < p.last) {
+      if (!is_v)
+        norm_rotate8<KIND, D>(y, src, row * stride + static_cast<int64_t>(head) * D, slot, a.k_weight, a.eps, turn[sub],
+                              a.rotary_dim, a.interleaved != 0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[t * PAD + 8 * slot + i] = y[i];
+        amax = fmaxf(amax, fabsf(y[i]));
+        finite = finite && fabsf(y[i]) <= 3.4028234663852886e+38f;
+      }
+    }
+  }
+  if (!finite) amax = __builtin_inff();
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+  if ((threadIdx.x & 63) == 0) amax_of[threadIdx.x >> 6] = amax;
+  __syncthreads();
+  amax = fmaxf(fmaxf(amax_of[0], amax_of[1]), fmaxf(amax_of[2], amax_of[3]));
+
+  float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
+  const float old = p.first > 0 ? *scale_at : 0.0f;
+  const bool poisoned = !(amax <= 3.4028234663852886e+38f) || old != old;
+  const float scale = fmaxf(fmaxf(old, amax / 127.0f), KV_SCALE_FLOOR);
+  const float ratio = old / scale;                    // 1 where the scale stays
+  uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
+  __syncthreads();                                     // every thread has read the old scale
+  if (threadIdx.x == 0) *scale_at = poisoned ? __builtin_nanf("") : scale;
+
+  for (int item = threadIdx.x; item < 2 * D; item += THREADS) {
+    // 16 bytes: of K one token's 16 dims, of V one dim's 16 tokens.
+    const int t_k = item & 31, d_k = (item >> 5) * 16;
+    const int d_v = item >> 1, place0 = (item & 1) * 16;
+    const bool grown = ratio != 1.0f && !poisoned;
+    bool keeps, takes;                                  // whether it holds tokens that stay (or lie behind), or new ones
+    if (is_v) {
+      keeps = p.first > 0 || p.last < KV_BLOCK;
+      takes = true;
+    } else {
+      keeps = t_k < p.first;
+      takes = t_k >= p.first && t_k < p.last;
+    }
+    if (!takes && !(keeps && grown)) continue;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (keeps) u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t r = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = is_v ? v_token(place0 + 4 * i + j) : t_k;
+        const int d = is_v ? d_v : d_k + 4 * i + j;
+        uint32_t b = (w[i] >> (8 * j)) & 0xFFu;
+        if (t >= p.first && t < p.last) b = poisoned ? 128u : quantize(x[t * PAD + d], scale);
+        else if (t < p.first && grown) b = requantize(b, ratio);
+        r |= b << (8 * j);
+      }
+      w[i] = r;
+    }
+    *reinterpret_cast<uint4*>(bytes + item_offset(item)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+struct ReadArgs {
+  KvCacheQ8 cache;
+  void* k;
+  void* v;
+  int64_t k_stride, v_stride;
+  const int32_t* start;
+  const int32_t* kv_lens;
+  int64_t tokens;
+  int batch, per_seq;
+};
+
+// grid (units, heads, 2).  The block passes through LDS as bytes, so that a row's values leave as whole lines.  A block
+// that is not in the cache (a bad page) yields zeros.
+template <int KIND, int D>
+__global__ void __launch_bounds__(THREADS) kv_read_kernel(ReadArgs a) {
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES, V_ROW = KV_BLOCK + 4;   // V rows padded: 8 lanes read 8 dims apart
+  __shared__ __align__(16) uint8_t lds[D * V_ROW];
+  __shared__ int found;
+  const bool is_v = blockIdx.z != 0;
+  void* dst = is_v ? a.v : a.k;
+  if (!dst) return;
+  const int head = blockIdx.y;
+  Piece p;
+  if (!find_piece(a.start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, &found, p)) return;
+  const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
+  const float scale = block < 0 ? 0.0f : (is_v ? a.cache.v_scale : a.cache.k_scale)[block];
+  if (block >= 0) {
+    const uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
+    for (int item = threadIdx.x; item < 2 * D; item += THREADS) {
+      const uint4 u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
+      uint32_t* to = reinterpret_cast<uint32_t*>(lds + (is_v ? (item >> 1) * V_ROW + (item & 1) * 16 : item_offset(item)));
+      to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
+    }
+  }
+  __syncthreads();
+  const int slot = threadIdx.x % LANES;
+  const int64_t stride = is_v ? a.v_stride : a.k_stride;
+  for (int t = p.first + static_cast<int>(threadIdx.x) / LANES; t < p.last; t += ROWS) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = 8 * slot + i;
+      const int at = is_v ? d * V_ROW + v_place(t) : ((d >> 4) * KV_BLOCK + t) * 16 + (d & 15);
+      y[i] = block < 0 ? 0.0f : static_cast<float>(static_cast<int>(lds[at]) - 128) * scale;
+    }
+    store8_f32<KIND>(dst, (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D + 8 * slot, y);
+  }
+}
+
+// The cheaper of the two ways of cutting a batch into units (see Piece): `per_seq` blocks for every sequence where all
+// are short, else 32-token steps over the whole batch.  0 per sequence means the second.
+struct Units {
+  int64_t units;
+  int per_seq;
+};
+Units units_of(int64_t tokens, int64_t batch, int64_t longest) {
+  const int64_t per_seq = longest > 0 ? (longest + 30) / 32 + 1 : 0;   // n tokens, at worst from place 31 of a block on
+  const int64_t even = longest == 1 ? batch : per_seq * batch, steps = tokens / 32 + 2 * batch;
+  if (longest > 0 && even <= steps) return {even, static_cast<int>(longest == 1 ? 1 : per_seq)};
+  return {steps, 0};
+}
+
+bool cache_ok(const void* k, const void* v, const float* ks, const float* vs, const int32_t* table, int64_t table_stride,
+              const int32_t* q_start, const int32_t* kv_lens, int64_t pages, int64_t page_size, int64_t kv_heads,
+              int64_t head_dim) {
+  return k && v && ks && vs && table && q_start && kv_lens && table_stride > 0 && pages > 0 && pages <= 0x7FFFFFFF &&
+         page_size >= KV_BLOCK && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0 && kv_heads > 0 &&
+         kv_heads <= 65535 && (head_dim == 64 || head_dim == 128 || head_dim == 256) &&
+         ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
+}
+
+KvCacheQ8 cache_of(void* k, void* v, float* ks, float* vs, const int32_t* table, int64_t table_stride, int64_t pages,
+                   int64_t page_size, int64_t kv_heads) {
+  return {static_cast<uint8_t*>(k), static_cast<uint8_t*>(v), ks, vs, table, table_stride, pages, static_cast<int>(kv_heads),
+          63 - __builtin_clzll(static_cast<unsigned long long>(page_size))};
+}
+
+constexpr int64_t MAX_UNITS = 8388607;   // a grid holds fewer than 2^32 threads a dimension
+constexpr int BAD = static_cast<int>(hipErrorInvalidValue);
+
+template <int KIND>
+int launch_append(const AppendArgs& a, int dim, dim3 grid, hipStream_t stream) {
+  switch (dim) {
+    case 64: hipLaunchKernelGGL((kv_append_kernel<KIND, 64>), grid, dim3(THREADS), 0, stream, a); break;
+    case 128: hipLaunchKernelGGL((kv_append_kernel<KIND, 128>), grid, dim3(THREADS), 0, stream, a); break;
+    default: hipLaunchKernelGGL((kv_append_kernel<KIND, 256>), grid, dim3(THREADS), 0, stream, a); break;
+  }
+  return static_cast<int>(hipGetLastError());
+}
+
+template <int KIND>
+int launch_read(const ReadArgs& a, int dim, dim3 grid, hipStream_t stream) {
+  switch (dim) {
+    case 64: hipLaunchKernelGGL((kv_read_kernel<KIND, 64>), grid, dim3(THREADS), 0, stream, a); break;
+    case 128: hipLaunchKernelGGL((kv_read_kernel<KIND, 128>), grid, dim3(THREADS), 0, stream, a); break;
+    default: hipLaunchKernelGGL((kv_read_kernel<KIND, 256>), grid, dim3(THREADS), 0, stream, a); break;
+  }
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace
+
+extern "C" int hipengine_gfx950_kv_append_q8(const void* k, const void* v, int32_t in_kind, int64_t k_stride,
+                                             int64_t v_stride, const float* k_weight, const int64_t* positions,
+                                             const float* inv_freq, int64_t rotary_dim, int32_t interleaved, float eps,
+                                             float rope_scale, uint8_t* k_cache, uint8_t* v_cache, float* k_scale,
+                                             float* v_scale, const int32_t* page_table, int64_t table_stride,
+                                             const int32_t* q_start, const int32_t* kv_lens, int64_t tokens, int64_t batch,
+                                             int64_t max_q_len, int64_t pages, int64_t page_size, int64_t kv_heads,
+                                             int64_t head_dim, hipStream_t stream) {
+  if (!cache_ok(k_cache, v_cache, k_scale, v_scale, page_table, table_stride, q_start, kv_lens, pages, page_size, kv_heads,
+                head_dim))
+    return BAD;
+  if (!k || !v || in_kind < KIND_F32 || in_kind > KIND_F16 || tokens <= 0 || tokens > 0x7FFFFFFF || batch <= 0 ||
+      batch > MAX_UNITS / 2 || max_q_len <= 0 || !(eps >= 0.0f))
+    return BAD;
+  if (inv_freq ? (rotary_dim < 16 || rotary_dim > head_dim || rotary_dim % 16 != 0) : rotary_dim != 0) return BAD;
+  const int64_t width = kv_heads * head_dim;
+  if (k_stride == 0) k_stride = width;
+  if (v_stride == 0) v_stride = width;
+  if (k_stride < width || v_stride < width) return BAD;
+  const Units u = units_of(tokens, batch, max_q_len < tokens ? max_q_len : tokens);
+  if (u.units > MAX_UNITS) return BAD;
+  const AppendArgs a{cache_of(k_cache, v_cache, k_scale, v_scale, page_table, table_stride, pages, page_size, kv_heads),
+                     k, v, k_stride, v_stride, k_weight, positions, inv_freq, q_start, kv_lens, tokens,
+                     static_cast<int>(batch), u.per_seq, static_cast<int>(rotary_dim), interleaved, eps, rope_scale};
+  const dim3 grid(static_cast<unsigned>(u.units), static_cast<unsigned>(kv_heads), 2);
+  const int dim = static_cast<int>(head_dim);
+  switch (in_kind) {
+    case KIND_F32: return launch_append<KIND_F32>(a, dim, grid, stream);
+    case KIND_BF16: return launch_append<KIND_BF16>(a, dim, grid, stream);
+    default: return launch_append<KIND_F16>(a, dim, grid, stream);
+  }
+}
+
+extern "C" int hipengine_gfx950_kv_read_q8(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale,
+                                           const float* v_scale, const int32_t* page_table, int64_t table_stride,
+                                           const int32_t* row_start, const int32_t* kv_lens, void* k_out, void* v_out,
+                                           int32_t out_kind, int64_t k_out_stride, int64_t v_out_stride, int64_t tokens,
+                                           int64_t batch, int64_t pages, int64_t page_size, int64_t kv_heads,
+                                           int64_t head_dim, hipStream_t stream) {
+  if (!cache_ok(k_cache, v_cache, k_scale, v_scale, page_table, table_stride, row_start, kv_lens, pages, page_size, kv_heads,
+                head_dim))
+    return BAD;
+  if ((!k_out && !v_out) || out_kind < KIND_F32 || out_kind > KIND_F16 || tokens <= 0 || tokens > 0x7FFFFFFF || batch <= 0 ||
+      batch > MAX_UNITS / 2)
+    return BAD;
+  const int64_t width = kv_heads * head_dim;
+  if (k_out_stride == 0) k_out_stride = width;
+  if (v_out_stride == 0) v_out_stride = width;
+  if (k_out_stride < width || v_out_stride < width) return BAD;
+  const Units u = units_of(tokens, batch, 0);
+  if (u.units > MAX_UNITS) return BAD;
+  const ReadArgs a{cache_of(const_cast<uint8_t*>(k_cache), const_cast<uint8_t*>(v_cache), const_cast<float*>(k_scale),
+                            const_cast<float*>(v_scale), page_table, table_stride, pages, page_size, kv_heads),
+                   k_out, v_out, k_out_stride, v_out_stride, row_start, kv_lens, tokens, static_cast<int>(batch), u.per_seq};
+  const dim3 grid(static_cast<unsigned>(u.units), static_cast<unsigned>(kv_heads), 2);
+  const int dim = static_cast<int>(head_dim);
+  switch (out_kind) {
+    case KIND_F32: return launch_read<KIND_F32>(a, dim, grid, stream);
+    case KIND_BF16: return launch_read<KIND_BF16>(a, dim, grid, stream);
+    default: return launch_read<KIND_F16>(a, dim, grid, stream);
+  }
+}
+
+int hipengine_gfx950::kv_cache_load() {
+  hipFuncAttributes attr;
+  return static_cast<int>(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(kv_append_kernel<KIND_BF16, 128>)));
+}

@@ -1,0 +1,135 @@
+// RMS norm of every query and key head and the position rotation, in one pass over the activations.
+//
+//   y = x / sqrt(mean(x^2) + eps) * w          (per head; skipped where the weight is null)
+//   (a, b) -> s (a cos t - b sin t, b cos t + a sin t),  t = position * inv_freq[i]
+//   over the first rotary_dim values of a head, pairs (i, i + rotary_dim / 2) or (2i, 2i + 1); the rest stays
+//
+// Statistics and rotation are in float32 and the angle in float64; the result is rounded once, on its way out.
+// A launch reads and writes every value once, so HBM (or, for a few tokens, the launch) is what bounds it.
+
+#include "attn_common.hpp"
+
+#include "gguf_init.hpp"
+
+#include "../../include/hipengine_gfx950.h"
+
+namespace {
+
+using namespace hipengine_gfx950;
+
+constexpr int64_t MAX_TOKENS = 4194303;   // a grid holds fewer than 2^32 threads, a workgroup up to 1024
+
+struct QkArgs {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const float* q_weight;
+  const float* k_weight;
+  const int64_t* positions;
+  const float* inv_freq;
+  int64_t q_stride, k_stride, q_out_stride, k_out_stride;
+  int q_heads, kv_heads, rotary_dim, interleaved;
+  float eps, rope_scale;
+};
+
+// One workgroup per token, D / 8 lanes per head; the angles of a token are computed once and shared by its heads.
+template <int IN, int OUT, int D>
+__global__ void __launch_bounds__(1024) qk_norm_rope_kernel(QkArgs a) {
+  __shared__ float2 turn[D / 2];
+  constexpr int LANES = D / 8;
+  const int64_t t = blockIdx.x;
+  const int heads = a.q_heads + a.kv_heads;
+  const int per_pass = blockDim.x / LANES;
+  const int slot = threadIdx.x % LANES;
+  int head = threadIdx.x / LANES;
+  float x[8];
+  const void* src = nullptr;
+  int64_t idx = 0;
+  auto load = [&] {
+    if (head < heads) {
+      const bool is_q = head < a.q_heads;
+      src = is_q ? a.q : a.k;
+      idx = is_q ? t * a.q_stride + static_cast<int64_t>(head) * D : t * a.k_stride + static_cast<int64_t>(head - a.q_heads) * D;
+      load8_f32<IN>(src, idx + 8 * slot, x);
+    }
+  };
+  load();
+  if (a.inv_freq) {
+    for (int i = threadIdx.x; i < a.rotary_dim / 2; i += blockDim.x)
+      turn[i] = rotation(a.positions[t], a.inv_freq[i], a.rope_scale);
+    __syncthreads();
+  }
+  while (head < heads) {
+    const bool is_q = head < a.q_heads;
+    norm_rotate8<IN, D>(x, src, idx, slot, is_q ? a.q_weight : a.k_weight, a.eps, turn, a.rotary_dim, a.interleaved != 0);
+    void* dst = is_q ? a.q_out : a.k_out;
+    const int64_t at = is_q ? t * a.q_out_stride + static_cast<int64_t>(head) * D
+                            : t * a.k_out_stride + static_cast<int64_t>(head - a.q_heads) * D;
+    store8_f32<OUT>(dst, at + 8 * slot, x);
+    head += per_pass;
+    load();
+  }
+}
+
+template <int IN, int OUT>
+int launch_dim(const QkArgs& a, int64_t tokens, int dim, hipStream_t stream) {
+  const int lanes = dim / 8;
+  const int64_t want = static_cast<int64_t>(a.q_heads + a.kv_heads) * lanes;
+  const unsigned threads = static_cast<unsigned>(want >= 1024 ? 1024 : (want + 63) / 64 * 64);
+  const dim3 grid(static_cast<unsigned>(tokens));
+  switch (dim) {
+    case 64: hipLaunchKernelGGL((qk_norm_rope_kernel<IN, OUT, 64>), grid, dim3(threads), 0, stream, a); break;
+    case 128: hipLaunchKernelGGL((qk_norm_rope_kernel<IN, OUT, 128>), grid, dim3(threads), 0, stream, a); break;
+    default: hipLaunchKernelGGL((qk_norm_rope_kernel<IN, OUT, 256>), grid, dim3(threads), 0, stream, a); break;
+  }
+  return static_cast<int>(hipGetLastError());
+}
+
+template <int IN>
+int launch_out(const QkArgs& a, int out_kind, int64_t tokens, int dim, hipStream_t stream) {
+  switch (out_kind) {
+    case KIND_F32: return launch_dim<IN, KIND_F32>(a, tokens, dim, stream);
+    case KIND_BF16: return launch_dim<IN, KIND_BF16>(a, tokens, dim, stream);
+    default: return launch_dim<IN, KIND_F16>(a, tokens, dim, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" int hipengine_gfx950_qk_norm_rope(const void* q, const void* k, const float* q_weight, const float* k_weight,
+                                             const int64_t* positions, const float* inv_freq, void* q_out, void* k_out,
+                                             int32_t in_kind, int32_t out_kind, int64_t tokens, int64_t q_heads,
+                                             int64_t kv_heads, int64_t head_dim, int64_t rotary_dim, int64_t q_stride,
+                                             int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, float eps,
+                                             float rope_scale, int32_t interleaved, hipStream_t stream) {
+  const int bad = static_cast<int>(hipErrorInvalidValue);
+  if (tokens <= 0 || tokens > MAX_TOKENS || q_heads < 0 || kv_heads < 0 || q_heads > 4096 || kv_heads > 4096 ||
+      q_heads + kv_heads == 0 || !(head_dim == 64 || head_dim == 128 || head_dim == 256) || in_kind < KIND_F32 ||
+      in_kind > KIND_F16 || out_kind < KIND_F32 || out_kind > KIND_F16 || !(eps >= 0.0f))
+    return bad;
+  if ((q_heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out))) return bad;
+  if (inv_freq ? (!positions || rotary_dim < 16 || rotary_dim > head_dim || rotary_dim % 16 != 0) : rotary_dim != 0) return bad;
+  const int64_t qw = q_heads * head_dim, kw = kv_heads * head_dim;
+  if (q_stride == 0) q_stride = qw;
+  if (k_stride == 0) k_stride = kw;
+  if (q_out_stride == 0) q_out_stride = qw;
+  if (k_out_stride == 0) k_out_stride = kw;
+  if (q_stride < qw || q_out_stride < qw || k_stride < kw || k_out_stride < kw) return bad;
+  // In place only where a value keeps its address.
+  if (q_heads > 0 && q == q_out && (in_kind != out_kind || q_stride != q_out_stride)) return bad;
+  if (kv_heads > 0 && k == k_out && (in_kind != out_kind || k_stride != k_out_stride)) return bad;
+  const QkArgs a{q, k, q_out, k_out, q_weight, k_weight, positions, inv_freq, q_stride, k_stride, q_out_stride, k_out_stride,
+                 static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(rotary_dim), interleaved, eps, rope_scale};
+  const int dim = static_cast<int>(head_dim);
+  switch (in_kind) {
+    case KIND_F32: return launch_out<KIND_F32>(a, out_kind, tokens, dim, stream);
+    case KIND_BF16: return launch_out<KIND_BF16>(a, out_kind, tokens, dim, stream);
+    default: return launch_out<KIND_F16>(a, out_kind, tokens, dim, stream);
+  }
+}
+
+int hipengine_gfx950::qk_norm_rope_load() {
+  hipFuncAttributes attr;
+  return static_cast<int>(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(qk_norm_rope_kernel<KIND_BF16, KIND_BF16, 128>)));
+}

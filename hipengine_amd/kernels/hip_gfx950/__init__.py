@@ -24,6 +24,7 @@ def register_backend_kernels(replace: bool = False) -> None:
     global _registered
     if _registered and not replace:
         return
+    from hipengine_amd.kernels.hip_gfx950.attention import kv_cache_q8, paged_attention_q8, qk_norm_rope
     from hipengine_amd.kernels.hip_gfx950.fused import paro_combine
     from hipengine_amd.kernels.hip_gfx950.linear import lm_head
     from hipengine_amd.kernels.hip_gfx950.moe import group_scatter, router
@@ -44,4 +45,7 @@ def register_backend_kernels(replace: bool = False) -> None:
     gguf_embedding.register_kernels(BACKEND, replace=True)
     lm_head.register_kernels(BACKEND, replace=True)
     paro_combine.register_kernels(BACKEND, replace=True)
+    qk_norm_rope.register_kernels(BACKEND, replace=True)
+    kv_cache_q8.register_kernels(BACKEND, replace=True)
+    paged_attention_q8.register_kernels(BACKEND, replace=True)
     _registered = True

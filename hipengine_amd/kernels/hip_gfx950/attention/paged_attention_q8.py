@@ -1,0 +1,76 @@
+"""Attention of ragged queries over the 8-bit paged KV cache of :mod:`kv_cache_q8`: single tokens, drafts of a few and
+prompts, causal, grouped query heads, optionally within a sliding window.
+
+``out = softmax(scale * q K^T) V``; the query in row i of a sequence's n is at place ``kv_lens[b] - n + i`` and sees the
+places up to its own, with ``window > 0`` the last ``window`` of them. A query that sees nothing gives zeros.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+from hipengine_amd.core.hip import HipRuntime
+from hipengine_amd.kernels.hip_gfx950 import _launch
+from hipengine_amd.kernels.hip_gfx950._launch import I32, I64, VOID, check_launch, entry, validate_pointers
+from hipengine_amd.kernels.hip_gfx950.attention._args import F32, KINDS, check_head_dim, check_positive, check_stride, kind_of
+from hipengine_amd.kernels.hip_gfx950.attention.kv_cache_q8 import KVCacheQ8
+from hipengine_amd.kernels.registry import KernelKey, register
+
+_ARGS = [VOID, VOID, I32, I64, I64] + [VOID] * 5 + [I64] + [VOID] * 2 + [I64] * 9 + [F32, I64, VOID, I64, VOID]
+_WORKSPACE_ARGS = [I64] * 7 + [ctypes.POINTER(I64)]
+
+
+def _check_shape(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int) -> None:
+    check_positive(tokens=tokens, batch=batch, max_q_len=max_q_len, q_heads=q_heads, kv_heads=kv_heads)
+    if tokens > 1 << 26 or batch > 65535:
+        raise ValueError("tokens must be at most 2^26 and batch at most 65535")
+    if max_kv_len < 0 or max_kv_len > 1 << 30:
+        raise ValueError("max_kv_len must be 0 .. 2^30")
+    if q_heads % kv_heads != 0 or q_heads > 4096:
+        raise ValueError("q_heads must be a multiple of kv_heads, at most 4096")
+    check_head_dim(head_dim)
+
+
+def paged_attention_q8_workspace_bytes(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int,
+                                       kv_heads: int, head_dim: int, *, library: ctypes.CDLL | None = None) -> int:
+    """Bytes of scratch that a call of these sizes needs, whatever its window; 0 where it needs none."""
+    _check_shape(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim)
+    out = I64(0)
+    check_launch(entry("hipengine_gfx950_paged_attention_q8_workspace_bytes", _WORKSPACE_ARGS, library)(
+        tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim, ctypes.byref(out)), None)
+    return int(out.value)
+
+
+def paged_attention_q8(cache: KVCacheQ8, q_ptr: int, out_ptr: int, page_table_ptr: int, table_stride: int,
+                       q_start_ptr: int, kv_lens_ptr: int, tokens: int, batch: int, max_q_len: int, max_kv_len: int,
+                       q_heads: int, *, workspace_ptr: int | None = None, workspace_bytes: int = 0,
+                       scale: float | None = None, window: int = 0, kind: str = "bf16", q_stride: int = 0,
+                       out_stride: int = 0, stream: int = 0, library: ctypes.CDLL | None = None,
+                       runtime: HipRuntime | None = None) -> None:
+    """q and out ``[tokens, q_heads, head_dim]`` (bf16 or fp16 bits, both of one kind). ``max_q_len`` and ``max_kv_len``
+    are at least the longest sequence's; ``scale`` defaults to ``head_dim ** -0.5``. The workspace (16-byte aligned) is
+    scratch of the size ``paged_attention_q8_workspace_bytes`` gives; calls that overlap in time need one each."""
+    if _launch.VALIDATE:
+        _check_shape(tokens, batch, max_q_len, max_kv_len, q_heads, cache.kv_heads, cache.head_dim)
+        check_positive(table_stride=table_stride)
+        kind_of(kind, "kind", ("bf16", "fp16"))
+        if scale is not None and not 0.0 < scale < math.inf:
+            raise ValueError("scale must be positive and finite")
+        if window < 0 or window > 1 << 30:
+            raise ValueError("window must be 0 (none) .. 2^30")
+        check_stride("q_stride", q_stride, q_heads * cache.head_dim)
+        check_stride("out_stride", out_stride, q_heads * cache.head_dim)
+        validate_pointers(q_ptr=q_ptr, out_ptr=out_ptr, page_table_ptr=page_table_ptr, q_start_ptr=q_start_ptr,
+                          kv_lens_ptr=kv_lens_ptr)
+        if q_ptr == out_ptr:
+            raise ValueError("out_ptr must not be q_ptr")
+    check_launch(entry("hipengine_gfx950_paged_attention_q8", _ARGS, library)(
+        q_ptr, out_ptr, KINDS[kind], q_stride, out_stride, cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr,
+        page_table_ptr, table_stride, q_start_ptr, kv_lens_ptr, tokens, batch, max_q_len, max_kv_len, q_heads,
+        cache.kv_heads, cache.head_dim, cache.pages, cache.page_size, cache.head_dim ** -0.5 if scale is None else scale,
+        window, workspace_ptr, workspace_bytes, stream), runtime)
+
+
+def register_kernels(backend: str = "hip_gfx950", *, replace: bool = False) -> None:
+    register(KernelKey(backend, "attention", "q8_block32", "paged"), paged_attention_q8, replace=replace)

@@ -881,6 +881,80 @@ int hipengine_gfx950_moe_tile_map(const int64_t* expert_start_compact, int64_t* 
                                   int64_t tile_capacity, int32_t tile_rows, hipengine_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Attention: q / k norm with rotation, the 8-bit paged KV cache, attention over it.  New here.
+ *
+ * Shared arguments:
+ *   head_dim        64, 128 or 256
+ *   *_stride        elements from one token's row to the next; 0 = packed (heads * head_dim)
+ *   positions       int64 [tokens];  inv_freq  float32 [rotary_dim / 2], radians per position
+ *   rotary_dim      a multiple of 16, at most head_dim; 0 with inv_freq null (no rotation)
+ *   interleaved     0: pairs (i, i + rotary_dim / 2); else pairs (2i, 2i + 1)
+ *   rope_scale      factor on cos and sin (1 without an attention factor)
+ *   k_cache, v_cache  uint8 [pages, kv_heads, page_size / 32, head_dim * 32], 16-byte aligned: bytes 128 + q, q in
+ *                   -127..127, in blocks of 32 tokens.  K block: [head_dim / 16][32 tokens][16]; V block:
+ *                   [head_dim][32], token t at place (t & 3) | (t >> 3 & 3) << 2 | (t >> 2 & 1) << 4.
+ *   k_scale, v_scale  float32 [pages, kv_heads, page_size / 32]: value = q * scale.  A scale under 2^-64 counts as 2^-64.
+ *   page_size       tokens of a page: a power of two, 32 .. 2^20
+ *   page_table      int32 [batch, table_stride] page numbers.  A number outside 0 .. pages - 1 is no page: tokens on it are
+ *                   not written, read as zeros and not attended to.  Entries behind a sequence's end are not looked at.
+ *   q_start         int32 [batch + 1]: sequence b's rows are q_start[b] .. q_start[b + 1] - 1
+ *   kv_lens         int32 [batch]: tokens in sequence b's cache, its rows of this call (the last ones) included.
+ *                   A sequence may have no rows, and no tokens.
+ *   max_q_len, max_kv_len  at least the longest sequence's rows / cached tokens (any larger value is right, too)
+ * ------------------------------------------------------------------------ */
+
+/* RMS norm of every head (weight float32 [head_dim]; null: none) and rotation of q [tokens, q_heads, head_dim] and
+ * k [tokens, kv_heads, head_dim], each into its output; in_kind / out_kind are HIPENGINE_GFX950_F32 / BF16 / F16.  Either
+ * of the two may be left out (0 heads).  An output may be its input (same kind and stride); other overlaps are undefined. */
+int hipengine_gfx950_qk_norm_rope(const void* q, const void* k, const float* q_weight, const float* k_weight,
+                                  const int64_t* positions, const float* inv_freq, void* q_out, void* k_out,
+                                  int32_t in_kind, int32_t out_kind, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, int64_t rotary_dim, int64_t q_stride, int64_t k_stride,
+                                  int64_t q_out_stride, int64_t k_out_stride, float eps, float rope_scale,
+                                  int32_t interleaved, hipengine_stream_t stream);
+
+/* Appends the rows of k (normed with k_weight, rotated; each only if given; positions null: a token's place in its
+ * sequence) and v to the cache, at places kv_lens[b] - rows .. kv_lens[b] - 1 of sequence b.  A block's scale grows to hold
+ * the new tokens and its earlier tokens are rescaled then; a block whose first token is appended starts anew; bytes behind
+ * the new tokens stay as they were.  Rows at negative places (more rows than kv_lens[b]) are left out.  A NaN or infinity
+ * makes its block's scale NaN until the block starts anew.  Within one call no two sequences may append to the same
+ * block: which one's tokens it then holds is not defined. */
+int hipengine_gfx950_kv_append_q8(const void* k, const void* v, int32_t in_kind, int64_t k_stride, int64_t v_stride,
+                                  const float* k_weight, const int64_t* positions, const float* inv_freq,
+                                  int64_t rotary_dim, int32_t interleaved, float eps, float rope_scale, uint8_t* k_cache,
+                                  uint8_t* v_cache, float* k_scale, float* v_scale, const int32_t* page_table,
+                                  int64_t table_stride, const int32_t* q_start, const int32_t* kv_lens, int64_t tokens,
+                                  int64_t batch, int64_t max_q_len, int64_t pages, int64_t page_size, int64_t kv_heads,
+                                  int64_t head_dim, hipengine_stream_t stream);
+
+/* Reads cached tokens back: row row_start[b] + i of the outputs [tokens, kv_heads, head_dim] is the token at place
+ * kv_lens[b] - (row_start[b + 1] - row_start[b]) + i of sequence b.  Either output may be null.  Rows of no sequence, and
+ * rows at negative places, are left as they were. */
+int hipengine_gfx950_kv_read_q8(const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale, const float* v_scale,
+                                const int32_t* page_table, int64_t table_stride, const int32_t* row_start,
+                                const int32_t* kv_lens, void* k_out, void* v_out, int32_t out_kind, int64_t k_out_stride,
+                                int64_t v_out_stride, int64_t tokens, int64_t batch, int64_t pages, int64_t page_size,
+                                int64_t kv_heads, int64_t head_dim, hipengine_stream_t stream);
+
+/* out = softmax(softmax_scale * q K^T) V for q, out [tokens, q_heads, head_dim], bf16 or fp16 (`kind`, of both).  The query
+ * in row i of n of sequence b is at place kv_lens[b] - n + i and sees the places up to its own (window > 0: the last
+ * `window` of them); q head h reads KV head h / (q_heads / kv_heads).  A query that sees nothing gives zeros; rows of no
+ * sequence are left as they were.  `workspace` (16-byte aligned, the size that the function below gives for the same
+ * sizes; null if 0) is scratch: calls that overlap in time need one each.  Results do not depend on timing. */
+int hipengine_gfx950_paged_attention_q8(const void* q, void* out, int32_t kind, int64_t q_stride, int64_t out_stride,
+                                        const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale,
+                                        const float* v_scale, const int32_t* page_table, int64_t table_stride,
+                                        const int32_t* q_start, const int32_t* kv_lens, int64_t tokens, int64_t batch,
+                                        int64_t max_q_len, int64_t max_kv_len, int64_t q_heads, int64_t kv_heads,
+                                        int64_t head_dim, int64_t pages, int64_t page_size, float softmax_scale,
+                                        int64_t window, void* workspace, int64_t workspace_bytes, hipengine_stream_t stream);
+
+/* Host only: *bytes = workspace of a call of these sizes, whatever its window. */
+int hipengine_gfx950_paged_attention_q8_workspace_bytes(int64_t tokens, int64_t batch, int64_t max_q_len,
+                                                        int64_t max_kv_len, int64_t q_heads, int64_t kv_heads,
+                                                        int64_t head_dim, int64_t* bytes);
+
+/* ------------------------------------------------------------------------
  * Verification exports: the integer unpack and the int32 sub-block dots the
  * production kernels compute, written out so that they can be compared bit for
  * bit with a CPU oracle.  New here.
