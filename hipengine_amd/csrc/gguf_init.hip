@@ -38,7 +38,8 @@ extern "C" int hipengine_gfx950_init(void) {
   if (rc != static_cast<int>(hipSuccess)) return rc;
   int (*const loads[])() = {hipengine_gfx950::quantize_load, hipengine_gfx950::mmq_load, hipengine_gfx950::moe_load,
                             hipengine_gfx950::embedding_load, hipengine_gfx950::qk_norm_rope_load,
-                            hipengine_gfx950::kv_cache_load, hipengine_gfx950::paged_attention_load};
+                            hipengine_gfx950::kv_cache_load, hipengine_gfx950::paged_attention_load,
+                            hipengine_gfx950::sample_rows_load};
   for (auto load : loads) {
     rc = load();
     if (rc != static_cast<int>(hipSuccess)) return rc;

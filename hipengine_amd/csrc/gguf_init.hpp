@@ -33,6 +33,7 @@ int embedding_load();
 int qk_norm_rope_load();
 int kv_cache_load();
 int paged_attention_load();
+int sample_rows_load();
 
 // True once hipengine_gfx950_init() has completed for the current device; runs it otherwise.
 // Launch paths that depend on the set-up call this first.

@@ -1,0 +1,639 @@
+// Sampling one token of every row of float32 logits from given uniform numbers: temperature, top-k, top-p, min-p.
+//
+// Tokens are ordered by logit, the highest first and equal ones by index.  With w = exp((l - l_max) / temperature):
+//   top-k   keeps the first k;   top-p keeps, of those, the tokens before which less than p of their total lies (the
+//   shortest prefix that holds p);   min-p drops those with w < min_p (the largest w is 1).
+// The token is the first one, by index, up to which the kept weights sum to more than u times their total.
+//
+// Sums are integers: a weight is held as w * 2^40 in 64 bits, so sums do not depend on the order in which atomics add, a
+// prefix and its border are exact, and the result is the same in every run.  (The argument is computed in float64, exp2
+// of its fraction in float32: a weight is good to 2^-23 of itself, or 2^-40 of the largest.)  Nothing is sorted.
+//
+// A row is read three times by many workgroups, each on a chunk of 4096 logits (the second and third time from the
+// caches): 1. its maximum; 2. a histogram of counts and weights over 512 bins of an eighth of an octave of w; 3. knowing
+// from it the bin B that holds the border: sums of the chunk's weights above B, and the tokens of B in a list (with top-k,
+// all tokens down to B: k needs no sums then).  4. One workgroup per row finds the exact border inside the list and the
+// token.  The three passes are bound by launch latency for a few rows and by the caches for many.
+// A list that would not fit (a row so flat that one bin holds over 16384 tokens) is replaced by the row itself.
+
+#include "gguf_common.hpp"
+
+#include "gguf_init.hpp"
+
+#include "../../include/hipengine_gfx950.h"
+
+namespace {
+
+using namespace hipengine_gfx950;
+
+constexpr int CHUNK = 4096;              // logits of a workgroup in passes 1 to 3
+constexpr int THREADS = 256;
+constexpr int LAST = 1024;               // threads of pass 4
+constexpr int BINS = 512;
+constexpr int LIST = 16384;
+constexpr int64_t MAX_VOCAB = 1 << 22;   // 1024 chunks; 2^22 weights of 2^40 stay under 2^63
+constexpr int MAX_CHUNKS = static_cast<int>(MAX_VOCAB / CHUNK);
+
+struct Args {
+  const float* logits;
+  int64_t stride;
+  const float* uniform;
+  const float* temperature;   // null: 1
+  const int32_t* top_k;       // null, 0 or less: all
+  const float* top_p;         // null, 1 or more: all
+  const float* min_p;         // null, 0 or less: all
+  int32_t* ids;
+  float* logprobs;            // or null
+  int vocab, chunks;
+  int cap;                    // tokens that a row's list holds
+  // workspace
+  uint64_t* best;             // [rows][chunks] key << 32 | ~index of the chunk's first token in the order
+  uint64_t* sums;             // [rows][chunks]
+  uint64_t* bin_weight;       // [rows][BINS]
+  uint64_t* list;             // [rows][cap] key << 32 | ~index
+  uint32_t* bin_count;        // [rows][BINS]
+  uint32_t* listed;           // [rows]
+};
+
+// The order as one number, higher is earlier: the logit's bits made to order like unsigned integers, then the index
+// downwards.  0 where the token cannot be chosen (-infinity, NaN).  -0 is made 0, infinity the largest number.
+__device__ __forceinline__ uint32_t key_of(float l) {
+  l = fminf(l + 0.0f, 3.4028234663852886e+38f);
+  if (!(l >= -3.4028234663852886e+38f)) return 0;      // (fminf gave the number for a NaN: looked at by the caller)
+  const uint32_t u = float_to_bits(l);
+  return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t order_of(float l, int index) {
+  const uint32_t key = l != l ? 0 : key_of(l);
+  return key ? (static_cast<uint64_t>(key) << 32) | static_cast<uint32_t>(~index) : 0;
+}
+__device__ __forceinline__ float logit_of(uint64_t order) {
+  const uint32_t k = static_cast<uint32_t>(order >> 32);
+  return bits_to_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ int index_of(uint64_t order) { return static_cast<int>(~static_cast<uint32_t>(order)); }
+
+struct Row {
+  float top;             // largest logit
+  double per;            // octaves of weight per unit of logit: log2(e) / temperature
+  bool greedy;
+  int k;                 // 0: all
+  double p;              // 1: all
+  double octaves;        // min-p's border; infinity: none
+};
+
+__device__ __forceinline__ Row row_of(const Args& a, int64_t row, float top) {
+  Row r;
+  r.top = top;
+  const float t = a.temperature ? a.temperature[row] : 1.0f;
+  r.greedy = !(t > 0.0f);
+  r.per = r.greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(t);
+  const int k = a.top_k ? a.top_k[row] : 0;
+  r.k = k > 0 && k < a.vocab ? k : 0;
+  const float p = a.top_p ? a.top_p[row] : 1.0f;
+  r.p = p < 1.0f ? fmax(static_cast<double>(p), 0.0) : 1.0;
+  const float m = a.min_p ? a.min_p[row] : 0.0f;
+  r.octaves = m > 0.0f ? -log2(fmin(static_cast<double>(m), 1.0)) : __builtin_inf();
+  return r;
+}
+__device__ __forceinline__ bool cuts(const Row& r) { return r.k > 0 || r.p < 1.0 || r.octaves < __builtin_inf(); }
+
+// Octaves below the largest weight.
+__device__ __forceinline__ double depth(const Row& r, float l) {
+  return fmin((static_cast<double>(r.top) - static_cast<double>(l)) * r.per, 2000.0);
+}
+__device__ __forceinline__ int bin_of(double y) { return min(static_cast<int>(y * 8.0), BINS - 1); }
+__device__ __forceinline__ uint64_t weight(double y) {   // 2^-y * 2^40
+  const double n = rint(y);
+  const uint32_t e = float_to_bits(__builtin_amdgcn_exp2f(static_cast<float>(n - y)));   // 0.7 .. 1.42
+  const int shift = 17 + static_cast<int>(e >> 23) - 127 - static_cast<int>(n);          // 40 - 23
+  const uint64_t m = (e & 0x7FFFFFu) | 0x800000u;
+  return shift >= 0 ? m << shift : shift > -32 ? m >> -shift : 0;
+}
+
+template <int N>
+__device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* lds) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(v), off);
+    v = o > v ? o : v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) v = lds[w] > v ? lds[w] : v;
+  return v;
+}
+template <int N>
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* lds) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(static_cast<unsigned long long>(v), off);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) v += lds[w];
+  return v;
+}
+
+__device__ __forceinline__ uint64_t row_best(const Args& a, int64_t row, int threads, uint64_t* lds) {
+  uint64_t v = 0;
+  for (int c = threadIdx.x; c < a.chunks; c += threads) {
+    const uint64_t o = a.best[row * a.chunks + c];
+    v = o > v ? o : v;
+  }
+  return threads == LAST ? block_max<LAST>(v, lds) : block_max<THREADS>(v, lds);
+}
+
+// A thread's 16 logits of a chunk: groups of 4 at (g * 256 + thread) * 4.  Behind the row's end: NaN.
+__device__ __forceinline__ int chunk_index(int chunk, int i) {
+  return chunk * CHUNK + ((i >> 2) * THREADS + static_cast<int>(threadIdx.x)) * 4 + (i & 3);
+}
+__device__ __forceinline__ void load_chunk(const Args& a, int64_t row, int chunk, float (&l)[16]) {
+  const float* src = a.logits + row * a.stride;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int at = chunk_index(chunk, 4 * g);
+    if (at + 4 <= a.vocab) {
+      __builtin_memcpy(&l[4 * g], __builtin_assume_aligned(src + at, 4), 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[4 * g + j] = at + j < a.vocab ? src[at + j] : __builtin_nanf("");
+    }
+  }
+}
+
+// Pass 1; also clears what pass 2 adds to.
+__global__ void __launch_bounds__(THREADS) sample_max_kernel(Args a) {
+  __shared__ uint64_t lds[THREADS / 64];
+  const int64_t row = blockIdx.y;
+  const int chunk = blockIdx.x;
+  float l[16];
+  load_chunk(a, row, chunk, l);
+  uint64_t v = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t o = order_of(l[i], chunk_index(chunk, i));
+    v = o > v ? o : v;
+  }
+  v = block_max<THREADS>(v, lds);
+  if (threadIdx.x == 0) a.best[row * a.chunks + chunk] = v;
+  for (int i = chunk * THREADS + threadIdx.x; i < BINS; i += a.chunks * THREADS) {
+    a.bin_weight[row * BINS + i] = 0;
+    a.bin_count[row * BINS + i] = 0;
+  }
+  if (chunk == 0 && threadIdx.x == 0) a.listed[row] = 0;
+}
+
+// Pass 2.
+__global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
+  __shared__ uint64_t lds[THREADS / 64];
+  __shared__ unsigned long long weights[BINS];
+  __shared__ uint32_t counts[BINS];
+  const int64_t row = blockIdx.y;
+  const int chunk = blockIdx.x;
+  float l[16];
+  load_chunk(a, row, chunk, l);
+  const uint64_t best = row_best(a, row, THREADS, lds);
+  const Row r = row_of(a, row, logit_of(best));
+  if (best == 0 || r.greedy || !cuts(r)) return;
+  for (int i = threadIdx.x; i < BINS; i += THREADS) { weights[i] = 0; counts[i] = 0; }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t o = order_of(l[i], 0);
+    if (o == 0) continue;
+    const double y = depth(r, logit_of(o));
+    const int b = bin_of(y);
+    atomicAdd(&counts[b], 1u);
+    if (b < BINS - 1) atomicAdd(&weights[b], static_cast<unsigned long long>(weight(y)));   // the last bin's are 0
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < BINS; i += THREADS) {
+    if (counts[i] == 0) continue;
+    atomicAdd(&a.bin_count[row * BINS + i], counts[i]);
+    if (weights[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.bin_weight[row * BINS + i]), weights[i]);
+  }
+}
+
+enum Mode : int { ALL, BOUND, PREFIX, FULL };
+
+// What passes 3 and 4 know from the histogram.
+struct Cut {
+  int mode;
+  int bin;              // B
+  uint64_t above;       // weight of the bins before B (BOUND)
+  uint64_t need;        // top-p: a token stays if less than this lies before it (BOUND)
+};
+
+__device__ __forceinline__ uint64_t border(double p, uint64_t total) {   // smallest whole number >= p * total
+  return static_cast<uint64_t>(ceil(p * static_cast<double>(total)));
+}
+
+// By the first 64 threads, 8 bins each, then told to all.
+__device__ __forceinline__ Cut find_cut(const Args& a, int64_t row, const Row& r, Cut* told) {
+  if (!cuts(r)) return {ALL, BINS, 0, 0};
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    uint64_t w[8], ws = 0;
+    uint32_t c[8], cs = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = a.bin_weight[row * BINS + lane * 8 + i];
+      c[i] = a.bin_count[row * BINS + lane * 8 + i];
+      ws += w[i];
+      cs += c[i];
+    }
+    uint64_t wi = ws;          // inclusive prefix over lanes
+    uint32_t ci = cs;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint64_t wo = __shfl_up(static_cast<unsigned long long>(wi), off);
+      const uint32_t co = __shfl_up(ci, off);
+      if (lane >= off) { wi += wo; ci += co; }
+    }
+    const uint64_t total = __shfl(static_cast<unsigned long long>(wi), 63);
+    const uint64_t need = r.p < 1.0 ? border(r.p, total) : ~uint64_t{0};
+    const int min_bin = r.octaves < __builtin_inf() ? bin_of(fmin(r.octaves, 2000.0)) : BINS - 1;
+    // First bin up to which k tokens, or `need`, are reached.
+    int k_bin = BINS - 1, p_bin = BINS - 1;
+    uint64_t wp = wi - ws;
+    uint32_t cp = ci - cs;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wp += w[i];
+      cp += c[i];
+      if (r.k > 0 && cp >= static_cast<uint32_t>(r.k)) k_bin = min(k_bin, lane * 8 + i);
+      if (wp >= need) p_bin = min(p_bin, lane * 8 + i);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      k_bin = min(k_bin, __shfl_xor(k_bin, off));
+      p_bin = min(p_bin, __shfl_xor(p_bin, off));
+    }
+    Cut cut;
+    cut.need = need;
+    cut.above = 0;
+    // A border in the last bin cuts nothing: its weights are 0.
+    const bool by_k = k_bin < BINS - 1;
+    cut.bin = by_k ? k_bin : min(p_bin, min_bin);
+    // Tokens and weight before and in the bin.
+    uint64_t in_w = 0;
+    uint32_t in_c = 0, to_c = 0;
+    wp = wi - ws;
+    cp = ci - cs;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (lane * 8 + i == cut.bin) { in_w = wp; in_c = c[i]; to_c = cp + c[i]; }
+      wp += w[i];
+      cp += c[i];
+    }
+    const int owner = cut.bin >> 3;
+    cut.above = __shfl(static_cast<unsigned long long>(in_w), owner);
+    const uint32_t in_bin = __shfl(in_c, owner), up_to = __shfl(to_c, owner);
+    if (by_k) cut.mode = up_to <= static_cast<uint32_t>(a.cap) ? PREFIX : FULL;
+    else if (cut.bin == BINS - 1) { cut.mode = ALL; cut.bin = BINS; }
+    else cut.mode = in_bin <= static_cast<uint32_t>(a.cap) ? BOUND : FULL;
+    if (lane == 0) *told = cut;
+  }
+  __syncthreads();
+  return *told;
+}
+
+// Pass 3.
+__global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
+  __shared__ uint64_t lds[THREADS / 64];
+  __shared__ Cut told;
+  __shared__ uint32_t here, base;
+  const int64_t row = blockIdx.y;
+  const int chunk = blockIdx.x;
+  float l[16];
+  load_chunk(a, row, chunk, l);
+  const uint64_t best = row_best(a, row, THREADS, lds);
+  const Row r = row_of(a, row, logit_of(best));
+  if (best == 0 || r.greedy) return;
+  if (threadIdx.x == 0) here = 0;
+  const Cut cut = find_cut(a, row, r, &told);
+  if (cut.mode == FULL) return;
+  __syncthreads();                                  // `here` is 0 for everyone, also where find_cut returned at once
+  uint64_t sum = 0;
+  uint32_t slot[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    slot[i] = ~0u;
+    const uint64_t o = order_of(l[i], 0);
+    if (o == 0) continue;
+    const double y = depth(r, logit_of(o));
+    const int b = bin_of(y);
+    if (cut.mode != PREFIX && b < cut.bin) sum += weight(y);
+    if (cut.mode == PREFIX ? b <= cut.bin : b == cut.bin) slot[i] = atomicAdd(&here, 1u);
+  }
+  if (cut.mode != PREFIX) {
+    sum = block_sum<THREADS>(sum, lds);
+    if (threadIdx.x == 0) a.sums[row * a.chunks + chunk] = sum;
+  }
+  __syncthreads();
+  if (here == 0) return;
+  if (threadIdx.x == 0) base = atomicAdd(&a.listed[row], here);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (slot[i] != ~0u && base + slot[i] < static_cast<uint32_t>(a.cap)) a.list[row * a.cap + base + slot[i]] = order_of(l[i], chunk_index(chunk, i));
+}
+
+// ---- pass 4 ------------------------------------------------------------------------------------------------------
+
+struct Digits {
+  unsigned long long weights[256];
+  uint32_t counts[256];
+  uint64_t before;       // found: weight (or count) of the buckets before the one
+  uint64_t in;           // found: tokens in it
+  int digit;
+};
+
+// The tokens that pass 4 looks through: a list, or the whole row.
+struct Tokens {
+  const uint64_t* list;
+  const float* logits;
+  int n;
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i = threadIdx.x; i < n; i += LAST) {
+      const uint64_t o = list ? list[i] : order_of(logits[i], i);
+      if (o) f(o);
+    }
+  }
+};
+
+// Walks down a 64-bit number digit by digit (8 bits, from `bits` on) to the token at which a running sum first exceeds
+// `before` (the sum up to and including it is more than that).  value(order): the number, larger is earlier.  add(order):
+// what the token adds (0: not among them).  Counts or weights: any whole numbers.  Returns the number; ends early where
+// one token is left in the bucket.
+template <typename V, typename A>
+__device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, int bits, uint64_t before, V value, A add) {
+  uint64_t prefix = 0;
+  for (int shift = bits - 8; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += LAST) { d.weights[i] = 0; d.counts[i] = 0; }
+    __syncthreads();
+    t.each([&](uint64_t o) {
+      const uint64_t v = value(o);
+      if (shift + 8 < 64 && (v >> (shift + 8)) != prefix) return;
+      const uint64_t w = add(o);
+      if (w == 0) return;
+      const int digit = static_cast<int>(v >> shift) & 255;
+      atomicAdd(&d.weights[digit], static_cast<unsigned long long>(w));
+      atomicAdd(&d.counts[digit], 1u);
+    });
+    __syncthreads();
+    if (threadIdx.x < 64) {      // lane 0 holds the largest digits
+      const int lane = threadIdx.x;
+      uint64_t w[4], s = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { w[i] = d.weights[255 - 4 * lane - i]; s += w[i]; }
+      uint64_t run = s;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
+        if (lane >= off) run += o;
+      }
+      const unsigned long long over = __ballot(run > before);
+      const int owner = over ? __builtin_ctzll(over) : 63;
+      if (lane == owner) {
+        run -= s;
+        int i = 0;
+        while (i < 3 && !(run + w[i] > before)) run += w[i++];
+        d.digit = 255 - 4 * lane - i;
+        d.before = run;
+        d.in = d.counts[d.digit];
+      }
+    }
+    __syncthreads();
+    prefix = (prefix << 8) | static_cast<uint64_t>(d.digit);
+    before -= d.before;
+    const uint64_t in = d.in;
+    __syncthreads();
+    if (in == 1 && shift > 0) {     // its remaining digits
+      if (threadIdx.x == 0) d.before = 0;
+      __syncthreads();
+      t.each([&](uint64_t o) {
+        const uint64_t v = value(o);
+        if ((v >> shift) == prefix && add(o)) d.before = v;
+      });
+      __syncthreads();
+      prefix = d.before;
+      __syncthreads();
+      return prefix;
+    }
+  }
+  return prefix;
+}
+
+__global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
+  __shared__ uint64_t lds[LAST / 64];
+  __shared__ Cut told;
+  __shared__ Digits digits;
+  __shared__ unsigned long long chunk_sum[MAX_CHUNKS];
+  __shared__ int chosen_chunk;
+  __shared__ uint64_t rest;
+  const int64_t row = blockIdx.x;
+  const uint64_t best = row_best(a, row, LAST, lds);
+  const Row r = row_of(a, row, logit_of(best));
+  if (best == 0 || r.greedy) {
+    if (threadIdx.x == 0) {
+      a.ids[row] = best ? index_of(best) : -1;
+      if (a.logprobs) a.logprobs[row] = best ? 0.0f : -__builtin_inff();
+    }
+    return;
+  }
+  const Cut cut = find_cut(a, row, r, &told);
+  const float* logits = a.logits + row * a.stride;
+  Tokens t;
+  t.list = cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr;
+  t.logits = logits;
+  t.n = cut.mode == FULL ? a.vocab : cut.mode == ALL ? 0 : min(a.listed[row], static_cast<uint32_t>(a.cap));
+  const uint64_t above = cut.mode == BOUND ? cut.above : 0;
+  auto self = [](uint64_t o) { return o; };
+  auto w_of = [&](uint64_t o) { return weight(depth(r, logit_of(o))); };
+
+  // Borders: a token stays if its order is `least` or more and its weight min-p's or more.
+  uint64_t least = 0;
+  if (cut.mode != ALL) {
+    uint64_t total = 0;      // of the tokens that top-k leaves
+    if (cut.mode != BOUND) {
+      if (r.k > 0) {
+        uint64_t there = 0;
+        t.each([&](uint64_t) { ++there; });
+        there = block_sum<LAST>(there, lds);
+        if (there > static_cast<uint64_t>(r.k))
+          least = walk(t, digits, 64, static_cast<uint64_t>(r.k) - 1, self, [](uint64_t) { return uint64_t{1}; });
+      }
+      t.each([&](uint64_t o) { if (o >= least) total += w_of(o); });
+      total = block_sum<LAST>(total, lds);
+    }
+    if (r.p < 1.0) {
+      const uint64_t need = cut.mode == BOUND ? cut.need : border(r.p, total);
+      if (need == 0) {
+        least = best;            // p = 0: the first token
+      } else {
+        // The token up to which the sum reaches `need`, that is exceeds need - 1.
+        uint64_t in = 0;
+        t.each([&](uint64_t o) { if (o >= least) in += w_of(o); });
+        in = block_sum<LAST>(in, lds);
+        if (above + in >= need) {
+          const uint64_t from = least;
+          least = walk(t, digits, 64, need - above - 1, self, [&](uint64_t o) { return o >= from ? w_of(o) : uint64_t{0}; });
+        }
+      }
+    }
+  }
+  auto kept = [&](uint64_t o, double y) { return o >= least && y <= r.octaves; };
+  auto kept_weight = [&](uint64_t o) {
+    const double y = depth(r, logit_of(o));
+    return kept(o, y) ? weight(y) : uint64_t{0};
+  };
+
+  uint64_t total = 0;
+  const bool by_chunk = cut.mode == ALL || cut.mode == BOUND;
+  if (by_chunk) {
+    for (int c = threadIdx.x; c < a.chunks; c += LAST) chunk_sum[c] = a.sums[row * a.chunks + c];
+    __syncthreads();
+    t.each([&](uint64_t o) {
+      const uint64_t w = kept_weight(o);
+      if (w) atomicAdd(&chunk_sum[index_of(o) / CHUNK], static_cast<unsigned long long>(w));
+    });
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.chunks; c += LAST) total += chunk_sum[c];
+  } else {
+    t.each([&](uint64_t o) { total += kept_weight(o); });
+  }
+  total = block_sum<LAST>(total, lds);
+  const float u = a.uniform[row];
+  uint64_t target = static_cast<uint64_t>((u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0) * static_cast<double>(total));
+  if (target >= total) target = total - 1;        // the largest weight is 2^40, so there is a total
+
+  int id;
+  if (by_chunk) {
+    if (threadIdx.x < 64) {
+      const int lane = threadIdx.x;
+      uint64_t passed = 0;
+      for (int c0 = 0; c0 < a.chunks; c0 += 64) {
+        const uint64_t s = c0 + lane < a.chunks ? chunk_sum[c0 + lane] : 0;
+        uint64_t run = s;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
+          if (lane >= off) run += o;
+        }
+        const unsigned long long over = __ballot(passed + run > target);
+        if (over) {
+          const int owner = __builtin_ctzll(over);
+          if (lane == owner) { chosen_chunk = c0 + lane; rest = target - (passed + run - s); }
+          break;
+        }
+        passed += __shfl(static_cast<unsigned long long>(run), 63);
+      }
+    }
+    __syncthreads();
+    // The chunk's tokens, 4 neighbours a thread, in index order.
+    const int first = chosen_chunk * CHUNK + static_cast<int>(threadIdx.x) * 4;
+    uint64_t w[4], s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = 0;
+      const uint64_t o = first + i < a.vocab ? order_of(logits[first + i], first + i) : 0;
+      if (o) {
+        const double y = depth(r, logit_of(o));
+        const int b = bin_of(y);
+        if (b < cut.bin || (b == cut.bin && kept(o, y))) w[i] = weight(y);
+      }
+      s += w[i];
+    }
+    uint64_t run = s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
+      if (lane >= off) run += o;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = run;
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) run += lds[v];
+    if (run > rest && run - s <= rest) {            // one thread
+      uint64_t at = run - s;
+      int i = 0;
+      while (i < 3 && !(at + w[i] > rest)) at += w[i++];
+      digits.digit = first + i;
+    }
+    __syncthreads();
+    id = digits.digit;
+  } else {
+    // Smaller indices first: the complement of the index orders them so, in 24 bits.
+    const uint64_t v = walk(t, digits, 24, target, [](uint64_t o) { return o & 0xFFFFFFu; }, kept_weight);
+    id = static_cast<int>(~static_cast<uint32_t>(v) & 0xFFFFFFu);
+  }
+  if (threadIdx.x == 0) {
+    a.ids[row] = id;
+    if (a.logprobs) {
+      const float l = fminf(logits[id] + 0.0f, 3.4028234663852886e+38f);
+      a.logprobs[row] = static_cast<float>(-((static_cast<double>(r.top) - static_cast<double>(l)) * r.per +
+                                             log2(static_cast<double>(total)) - 40.0) * 0.6931471805599453);
+    }
+  }
+}
+
+constexpr int BAD = static_cast<int>(hipErrorInvalidValue);
+
+bool shape_ok(int64_t rows, int64_t vocab) { return rows > 0 && rows <= 65535 && vocab > 0 && vocab <= MAX_VOCAB; }
+int64_t chunks_of(int64_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
+int64_t cap_of(int64_t vocab) { return vocab < LIST ? vocab : LIST; }
+int64_t workspace_of(int64_t rows, int64_t vocab) {
+  return rows * (16 * chunks_of(vocab) + 12 * BINS + 8 * cap_of(vocab) + 4);
+}
+
+}  // namespace
+
+extern "C" int hipengine_gfx950_sample_f32_rows_i32_workspace_bytes(int64_t rows, int64_t vocab_size, int64_t* bytes) {
+  if (!bytes || !shape_ok(rows, vocab_size)) return BAD;
+  *bytes = workspace_of(rows, vocab_size);
+  return 0;
+}
+
+extern "C" int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t logits_stride, const float* uniform,
+                                                    const float* temperature, const int32_t* top_k, const float* top_p,
+                                                    const float* min_p, int32_t* out_ids, float* out_logprobs, int64_t rows,
+                                                    int64_t vocab_size, void* workspace, int64_t workspace_bytes,
+                                                    hipStream_t stream) {
+  if (!logits || !uniform || !out_ids || !shape_ok(rows, vocab_size) || !workspace ||
+      workspace_bytes < workspace_of(rows, vocab_size) || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0)
+    return BAD;
+  if (logits_stride == 0) logits_stride = vocab_size;
+  if (logits_stride < vocab_size) return BAD;
+  const int64_t chunks = chunks_of(vocab_size);
+  uint64_t* w = static_cast<uint64_t*>(workspace);
+  Args a{logits, logits_stride, uniform, temperature, top_k, top_p, min_p, out_ids, out_logprobs, static_cast<int>(vocab_size),
+         static_cast<int>(chunks), static_cast<int>(cap_of(vocab_size)), nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  a.best = w;
+  a.sums = a.best + rows * chunks;
+  a.bin_weight = a.sums + rows * chunks;
+  a.list = a.bin_weight + rows * BINS;
+  a.bin_count = reinterpret_cast<uint32_t*>(a.list + rows * a.cap);
+  a.listed = a.bin_count + rows * BINS;
+  const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(rows)), threads(THREADS);
+  hipLaunchKernelGGL(sample_max_kernel, grid, threads, 0, stream, a);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess) return static_cast<int>(err);
+  hipLaunchKernelGGL(sample_histogram_kernel, grid, threads, 0, stream, a);
+  if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
+  hipLaunchKernelGGL(sample_collect_kernel, grid, threads, 0, stream, a);
+  if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
+  hipLaunchKernelGGL(sample_choose_kernel, dim3(static_cast<unsigned>(rows)), dim3(LAST), 0, stream, a);
+  return static_cast<int>(hipGetLastError());
+}
+
+int hipengine_gfx950::sample_rows_load() {
+  hipFuncAttributes attr;
+  return static_cast<int>(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(sample_choose_kernel)));
+}

@@ -35,6 +35,7 @@ def register_backend_kernels(replace: bool = False) -> None:
         gguf_q8_1_gemv,
         gguf_quantize,
     )
+    from hipengine_amd.kernels.hip_gfx950.sampling import sample_rows
 
     gguf_quantize.register_kernels(BACKEND, replace=True)
     gguf_q8_1_gemv.register_kernels(BACKEND, replace=True)
@@ -48,4 +49,5 @@ def register_backend_kernels(replace: bool = False) -> None:
     qk_norm_rope.register_kernels(BACKEND, replace=True)
     kv_cache_q8.register_kernels(BACKEND, replace=True)
     paged_attention_q8.register_kernels(BACKEND, replace=True)
+    sample_rows.register_kernels(BACKEND, replace=True)
     _registered = True

@@ -955,6 +955,29 @@ int hipengine_gfx950_paged_attention_q8_workspace_bytes(int64_t tokens, int64_t 
                                                         int64_t head_dim, int64_t* bytes);
 
 /* ------------------------------------------------------------------------
+ * Sampling, beside the arg-max above.  New here.
+ * ------------------------------------------------------------------------ */
+
+/* One token of every row of float32 logits [rows, vocab_size] (logits_stride elements from row to row; 0 = vocab_size),
+ * vocab_size at most 2^22, from uniform [rows] in 0 <= u < 1.  With the row's tokens in order of their logits, highest
+ * first, equal ones by index, and w = exp((l - l_max) / temperature[row]): top_k > 0 keeps the first top_k; top_p < 1
+ * keeps of those the shortest prefix whose weight is at least top_p of theirs (at least one token); min_p > 0 drops those
+ * with w < min_p (a min_p over 1 counts as 1).  out_ids is the first kept token, by index, up to which the kept weights
+ * sum to more than u times their total; out_logprobs (or null) the log of its share.  The four settings are arrays
+ * [rows], each of which may be null: 1, all, all, all.  A temperature of 0 (or less, or NaN) takes the first token of the
+ * order, with log-probability 0.  Logits of -infinity and NaN are not there; a row of nothing else gives -1 and -infinity.
+ * `workspace`: scratch, 8-byte aligned, of the size that the function below gives; calls that overlap in time need one
+ * each.  Results do not depend on timing. */
+int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t logits_stride, const float* uniform,
+                                         const float* temperature, const int32_t* top_k, const float* top_p,
+                                         const float* min_p, int32_t* out_ids, float* out_logprobs, int64_t rows,
+                                         int64_t vocab_size, void* workspace, int64_t workspace_bytes,
+                                         hipengine_stream_t stream);
+
+/* Host only: *bytes = workspace of a call of these sizes. */
+int hipengine_gfx950_sample_f32_rows_i32_workspace_bytes(int64_t rows, int64_t vocab_size, int64_t* bytes);
+
+/* ------------------------------------------------------------------------
  * Verification exports: the integer unpack and the int32 sub-block dots the
  * production kernels compute, written out so that they can be compared bit for
  * bit with a CPU oracle.  New here.

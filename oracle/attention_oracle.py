@@ -162,3 +162,38 @@ def attention(q, k_int, v_int, k_scale, v_scale, table, q_start, kv_lens, *, sca
                 dev[row + i, h] = p[i] @ np.abs(vv - o[i])
             arg[row: row + n, h] = np.where(seen, np.abs(x) @ np.abs(kk).T * scale, 0.0).max(-1, keepdims=True)
     return out, dev, mag, arg
+
+
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, accuracy=0.0):
+    """{id: (lowest, highest log-probability)} of one row: with accuracy 0 the one token of the definition. With accuracy e
+    every token that it gives if prefix sums (around top-p's border, and around the token's) are moved by up to e of
+    themselves, and min-p by 2^-20 of that: what such arithmetic may answer, nearly always one token too."""
+    l = np.minimum(np.asarray(logits, np.float64) + 0.0, np.finfo(np.float32).max)
+    there = np.flatnonzero(~np.isnan(l) & (l > -np.inf))
+    if not there.size:
+        return {-1: (-np.inf, -np.inf)}
+    order = there[np.lexsort((there, -l[there]))]
+    if not temperature > 0:
+        return {int(order[0]): (0.0, 0.0)}
+    if top_k > 0:
+        order = order[:top_k]
+    w = np.exp(np.maximum((l[order] - l[order[0]]) / np.float64(temperature), -5000))
+    u = min(float(uniform), 1.0) if uniform > 0 else 0.0
+    cum, found = np.cumsum(w), {}
+    for a in {-accuracy, 0.0, accuracy}:
+        n = 1 + int(np.sum(cum[:-1] < max(float(top_p), 0.0) * cum[-1] * (1 + a))) if top_p < 1 else len(w)
+        for b in {-accuracy, 0.0, accuracy}:
+            m = min(float(min_p), 1.0) * (1 + b * 2.0 ** -20) if min_p > 0 else 0.0   # (an argument in float64 decides)
+            keep = (np.arange(len(w)) < n) & ((w >= m) | (w == 1))
+            ids, v = order[keep], w[keep]
+            by = np.argsort(ids)
+            ids, v = ids[by], v[by]
+            run = np.cumsum(v)
+            for c in {-accuracy, 0.0, accuracy}:
+                i = min(int(np.searchsorted(run, (u + c) * run[-1], side="right")), len(v) - 1)
+                while v[i] == 0:
+                    i -= 1
+                p = float(np.log(v[i]) - np.log(run[-1]))
+                lo, hi = found.get(int(ids[i]), (p, p))
+                found[int(ids[i])] = (min(lo, p), max(hi, p))
+    return found

@@ -13,6 +13,7 @@ from hipengine_amd.core.build import load_library
 from hipengine_amd.kernels.hip_gfx950.attention import kv_cache_q8 as C
 from hipengine_amd.kernels.hip_gfx950.attention import paged_attention_q8 as A
 from hipengine_amd.kernels.hip_gfx950.attention import qk_norm_rope as R
+from hipengine_amd.kernels.hip_gfx950.sampling import sample_rows as S
 from hipengine_amd.kernels.registry import resolve
 from oracle import attention_oracle as O
 
@@ -96,6 +97,16 @@ def test_attention_refusals(over):
         A.paged_attention_q8(cache(), **(ATTEND | over), library=Never())
 
 
+SAMPLE = dict(logits_ptr=16, uniform_ptr=16, out_ids_ptr=16, rows=2, vocab_size=100, workspace_ptr=16, workspace_bytes=1 << 20)
+
+
+@pytest.mark.parametrize("over", [{"rows": 0}, {"rows": 65536}, {"vocab_size": 0}, {"vocab_size": 2**22 + 1}, {"logits_stride": 99},
+                                  {"logits_stride": -1}, {"logits_ptr": 0}, {"uniform_ptr": None}, {"out_ids_ptr": 0}, {"workspace_ptr": None}])
+def test_sample_refusals(over):
+    with pytest.raises(ValueError):
+        S.sample_f32_rows_i32(**(SAMPLE | over), library=Never())
+
+
 # ---- the C entry points refuse by themselves -------------------------------------------------------------------------
 
 
@@ -165,6 +176,28 @@ def test_c_attention_refuses(over):
     assert _attend(**over) == 1
 
 
+def _sample(**over):
+    a = dict(logits=16, ls=0, u=16, t=None, k=None, p=None, m=None, ids=16, lp=None, rows=2, vocab=100, ws=16, wsb=1 << 20, stream=None) | over
+    fn = load_library().hipengine_gfx950_sample_f32_rows_i32
+    fn.argtypes, fn.restype = S._ARGS, ctypes.c_int
+    return fn(*a.values())
+
+
+@pytest.mark.parametrize("over", [{"logits": None}, {"ls": 99}, {"u": None}, {"ids": None}, {"rows": 0}, {"rows": 65536}, {"vocab": 0},
+                                  {"vocab": 1 << 23}, {"ws": None}, {"ws": 20}, {"wsb": 100}])
+def test_c_sample_refuses(over):
+    assert _sample(**over) == 1
+
+
+def test_sample_workspace_function():
+    assert 0 < S.sample_workspace_bytes(1, 1) < S.sample_workspace_bytes(1, 1000) < S.sample_workspace_bytes(2, 1000)
+    with pytest.raises(ValueError):
+        S.sample_workspace_bytes(0, 5)
+    fn = load_library().hipengine_gfx950_sample_f32_rows_i32_workspace_bytes
+    fn.argtypes = S._WORKSPACE_ARGS
+    assert fn(1, 1, None) == 1 and fn(1, 1 << 23, ctypes.byref(ctypes.c_int64())) == 1
+
+
 def test_workspace_function():
     f = A.paged_attention_q8_workspace_bytes
     assert f(1, 1, 1, 1, 8, 8, 128) == 0
@@ -188,6 +221,7 @@ def test_registry_keys():
     assert resolve(backend="hip_gfx950", layer="kv_cache", quant="q8_block32", variant="append") is C.kv_append_q8
     assert resolve(backend="hip_gfx950", layer="kv_cache", quant="q8_block32", variant="read") is C.kv_read_q8
     assert resolve(backend="hip_gfx950", layer="attention", quant="q8_block32", variant="paged") is A.paged_attention_q8
+    assert resolve(backend="hip_gfx950", layer="sample", quant="f32", variant="rows_i32") is S.sample_f32_rows_i32
 
 
 # ---- the statements the GPU tests compare with -----------------------------------------------------------------------
@@ -234,3 +268,16 @@ def test_statement_of_append_and_attention():
     s = q[0, 1] @ values[0, 34:39].T * 0.1                 # the query at place 38 sees 34 .. 38
     p = np.exp(s) / np.exp(s).sum()
     assert np.allclose(out[0, 1], p @ vv[0, 34:39])
+
+
+def test_statement_of_sampling():
+    row = np.log(np.array([1.0, 4.0, 2.0, 4.0, 1.0]))                   # order: 1, 3, 2, 0, 4
+    one = lambda *args, **kw: next(iter(O.sample(*args, **kw)))  # noqa: E731
+    assert one(row, 0.0) == 0 and one(row, 0.99) == 4
+    assert one(row, 0.5, top_k=1) == 1 and one(row, 0.6, top_k=2) == 3
+    assert one(row, 0.99, top_p=0.4) == 3                                # 4 of 12 is not 0.4, 8 is
+    assert one(row, 0.99, top_p=0.3) == 1
+    assert one(row, 0.99, min_p=0.4) == 3 and one(row, 0.45, min_p=0.4) == 2
+    assert one(row, 0.99, temperature=0) == 1 and one(np.full(3, -np.inf), 0.5) == -1
+    assert np.isclose(O.sample(row, 0.0)[0][0], math.log(1 / 12))
+    assert set(O.sample(row, 1 / 12 + 1e-9, accuracy=1e-6)) == {0, 1}    # on the border between the first two tokens
