@@ -22,6 +22,8 @@
 // Splits.  Where rows are few, the keys of a sequence are cut into chunks for workgroups of their own, whose partial
 // maxima, sums and outputs go to a workspace and are joined by a second kernel in chunk order (no atomics).
 
+#include <type_traits>
+
 #include "attn_common.hpp"
 
 #include "gguf_init.hpp"
@@ -37,7 +39,9 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-constexpr int WAVES = 4;
+constexpr int WAVES = 4;               // of attention_keys_kernel
+constexpr int ROW_WAVES = 8;           // of attention_rows_kernel, each with 32 rows
+constexpr int ROW_TILE = 32 * ROW_WAVES;
 constexpr int MAX_KV = 1 << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEVER = -1e30f;        // a maximum before any key: finite, so that differences to it are no NaN
@@ -63,6 +67,9 @@ struct AttnArgs {
 };
 
 // Four excess-128 bytes -> four fp16 whole numbers.  0x6400 | b is 1024 + b in fp16.
+// (Half of these instructions could go: a byte under zeros is the subnormal b * 2^-24, and the excess could come off the
+// sums. But the matrix instruction drops the low bits of what it adds, in one direction, and with an excess of 128 in
+// every value that showed: O was off by 2^-19 of 128 steps of V.)
 __device__ __forceinline__ void bytes_to_half(uint32_t w, h2& lo, h2& hi) {
   const h2 bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
   lo = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, 0x07010700u)) - bias;
@@ -75,6 +82,14 @@ __device__ __forceinline__ h8 bytes8_to_half(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(h8, p);
 }
 
+// A barrier for what goes through LDS: unlike __syncthreads() it does not wait for loads from memory, which are on their
+// way across it on purpose.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // The other half of the wave's value of the same column.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
@@ -82,301 +97,399 @@ __device__ __forceinline__ float read_lane_f(float v, int lane) {
   return bits_to_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(float_to_bits(v)), lane)));
 }
 
-// KEYS: the four waves of a workgroup share its rows and take blocks of keys in turn (decode); else every wave has rows
-// of its own and walks over all keys (prompts).  NT: columns of 32 rows that a wave holds.
+// The keys that a query sees: places [lower, limit).
+struct Sight {
+  int kv_len, q_len, window;
+  __device__ __forceinline__ int limit(int query) const { return min(max(kv_len - q_len + query + 1, 0), kv_len); }
+  __device__ __forceinline__ int lower(int query) const { return window > 0 ? max(kv_len - q_len + query + 1 - window, 0) : 0; }
+};
+
+// One column: a row of queries as the matrix instruction's second operand (lane (column, half) holds dims 32 i + 16 half +
+// 8 b .. + 7 of piece 2 i + b), and what goes with it.
+template <int D>
+struct Column {
+  h8 q[D / 16];
+  float c;             // argument of the softmax, in log2, per raw product and unit of K's scale
+  int lim, lo;
+  bool valid;
+  int64_t row, member; // of the batch; of the KV head's group
+};
+
+template <int D, int KIND>
+__device__ __forceinline__ Column<D> load_column(const AttnArgs& a, const SeqRows& rows, const Sight& sight, int r, int n_rows, int head) {
+  constexpr int P = D / 16;
+  const int half = (threadIdx.x & 63) >> 5;
+  Column<D> k;
+  k.valid = r < n_rows;
+  const int query = k.valid ? r / a.group : 0;
+  k.member = k.valid ? r - query * a.group : 0;
+  k.lim = sight.limit(query);
+  k.lo = sight.lower(query);
+  k.row = rows.first + query;
+  const int64_t at = k.row * a.q_stride + (head * a.group + k.member) * static_cast<int64_t>(D);
+  float x[P][8], amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    load8_f32<KIND>(a.q, at + 32 * (i >> 1) + 16 * half + 8 * (i & 1), x[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[i][j]));
+  }
+  int e = 0;
+  if constexpr (KIND == KIND_BF16) {
+    amax = fmaxf(amax, other_half(amax));
+    e = max(static_cast<int>(float_to_bits(amax) >> 23), 1) - 127;
+  }
+  k.c = ldexpf(1.0f, e) * a.scale;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k.q[i][j] = static_cast<_Float16>(KIND == KIND_BF16 ? ldexpf(x[i][j], -e) : x[i][j]);
+    // (keeps the conversion in front of the loop: the compiler sinks it into the loop otherwise, 97 instructions a block)
+    asm volatile("" : "+v"(k.q[i]));
+  }
+  return k;
+}
+
+// Numbers and scales of 64 of a sequence's blocks, `step` apart, one a lane.  A block that is not there (a bad page, or
+// behind the end) is block 0 with a V scale of zero: it adds nothing, and nothing branches on it.
+struct Blocks {
+  int base, step;
+  int64_t number;
+  float ks, lv, iv;    // scale of K, log2 of V's, 1 / V's
+  __device__ __forceinline__ void lookup(const KvCacheQ8& c, int seq, int head, int from, int end) {
+    base = from;
+    const int mine = from + static_cast<int>(threadIdx.x & 63) * step;
+    const int64_t found = mine < end ? kv_block_index(c, seq, mine, head) : -1;
+    number = max(found, int64_t{0});
+    const float v = c.v_scale[number], k = c.k_scale[number];
+    const float v_clean = fmaxf(v, KV_SCALE_FLOOR);          // of a NaN: the floor
+    ks = found < 0 ? 0.0f : fmaxf(k, k != k ? k : KV_SCALE_FLOOR);
+    lv = found < 0 ? -__builtin_inff() : v == v ? log2f(v_clean) : v;
+    iv = found < 0 ? 0.0f : 1.0f / v_clean;
+  }
+  __device__ __forceinline__ int slot(int which) const { return (which - base) / step; }
+  __device__ __forceinline__ int64_t at(int which) const {
+    const int k = slot(which);
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(number), k));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(number >> 32), k));
+    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+  }
+};
+
+struct Scales {
+  float ks, lv, iv;
+  bool far;            // V's is less than a quarter of the largest so far
+};
+__device__ __forceinline__ Scales scales_of(const Blocks& b, int which, float& lv_top) {
+  const int slot = b.slot(which);
+  Scales r{read_lane_f(b.ks, slot), read_lane_f(b.lv, slot), read_lane_f(b.iv, slot), false};
+  lv_top = fmaxf(lv_top, r.lv);
+  r.far = r.lv < lv_top - 2.0f && r.lv > -__builtin_inff();
+  return r;
+}
+
+// One block of the softmax of a column: raw products s of its 32 keys -> P, as the operand of O += V P, with the running
+// reference m and sum l.  rescale(f) multiplies O where the reference moves.
+template <int D, typename F>
+__device__ __forceinline__ void softmax_block(f16v& s, const Column<D>& k, const Scales& b, bool masked, int key0, float one,
+                                              float& m, float& l, h8 (&p)[2], F rescale) {
+  const int half = (threadIdx.x & 63) >> 5;
+  const float c = b.ks * k.c;
+  auto sees = [&](int i) {
+    const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
+    return key < k.lim && key >= k.lo;
+  };
+  // The argument of a key is fma(s, c, lv), and c > 0 keeps the order.
+  float top = -__builtin_inff();
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, sees(i) ? s[i] : -__builtin_inff());
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
+  }
+  top = fmaxf(top, other_half(top));
+  const float high = fmaf(top, c, b.lv);       // a NaN (a poisoned block, or nothing seen at a zero c) moves nothing
+  if (__any(high > m + HEADROOM)) {
+    const float to = fmaxf(m, high);
+    const float f = __builtin_amdgcn_exp2f(m - to);
+    m = to;
+    l *= f;
+    rescale(f);
+  }
+  if (b.far) {
+    // w may be lost in fp16 although p counts in the sum, which then takes p itself, at the price of 16 more exponentials.
+    float e = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float p_i = __builtin_amdgcn_exp2f(fmaf(s[i], c, OFFSET - m));
+      e += !masked || sees(i) ? p_i : 0.0f;
+    }
+    l += e;
+  }
+  const float shift = b.lv - m + OFFSET;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift));
+  if (masked) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = sees(i) ? s[i] : 0.0f;
+  }
+  // P is summed as rounded, its subnormals too (the dot product instruction would take those as 0): v_fma_mix_f32 with a
+  // `one` that the compiler does not see through.
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    const h2 r = __builtin_convertvector((f2v{s[i], s[i + 1]}), h2);
+    p[i >> 3][i & 7] = r.x;
+    p[i >> 3][(i & 7) + 1] = r.y;
+    sum = fmaf(static_cast<float>(r.x), one, sum);
+    sum = fmaf(static_cast<float>(r.y), one, sum);
+  }
+  l = fmaf(sum, b.far ? 0.0f : b.iv, l);
+}
+
+__device__ __forceinline__ float opaque_one() {
+  float one = 1.0f;
+  asm volatile("" : "+v"(one));
+  return one;
+}
+
+// A column's result: to the output, or with splits to the workspace.
+template <int D, int KIND>
+__device__ __forceinline__ void store_column(const AttnArgs& a, const Column<D>& k, int head, int split, float m, float l,
+                                             const f16v (&acc)[D / 32]) {
+  if (!k.valid) return;
+  const int half = (threadIdx.x & 63) >> 5;
+  const int64_t q_head = head * a.group + k.member;
+  if (a.splits > 1) {
+    const int64_t at = (static_cast<int64_t>(split) * a.tokens + k.row) * a.q_heads + q_head;
+    if (half == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = l;
+    }
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(a.part_acc + at * D + 32 * t + 2 * i + 4 * half) =
+            make_float4(acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]);
+    return;
+  }
+  const float r = l == 0.0f ? 0.0f : 1.0f / l;   // a row that saw no key gives zeros
+  uint16_t* out = static_cast<uint16_t*>(a.out) + k.row * a.out_stride + q_head * D + 4 * half;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      uint32_t w[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        w[b] = half_bits<KIND>(acc[t][i + 2 * b] * r) | (half_bits<KIND>(acc[t][i + 2 * b + 1] * r) << 16);
+      __builtin_memcpy(__builtin_assume_aligned(out + 32 * t + 2 * i, 2), w, 8);
+    }
+}
+
+// ---- few rows: the four waves of a workgroup share 32 rows and take blocks of keys in turn --------------------------
+// grid (KV heads, row tiles, batch * splits).  Bound by the cache's bytes: a wave converts a block's 64 * D bytes in 1200
+// clocks, four times what HBM delivers in that time.
+template <int D, int KIND>
+__global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_kernel(AttnArgs a) {
+  constexpr int KC = D / 32;           // 16-byte loads of K a lane, and tiles of 32 dims of V
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.x;
+  const int seq = blockIdx.z / a.splits, split = blockIdx.z - seq * a.splits;
+  const SeqRows rows = seq_rows(a.q_start, seq, a.tokens);
+  const int n_rows = static_cast<int>(rows.count) * a.group, row0 = blockIdx.y * 32;
+  if (row0 >= n_rows) return;
+  const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
+  const int first_q = row0 / a.group, last_q = (min(row0 + 32, n_rows) - 1) / a.group;
+  const int lim_first = sight.limit(first_q), lo_last = sight.lower(last_q);
+  int blk = sight.lower(first_q) >> 5, blk_end = (sight.limit(last_q) + 31) >> 5;
+  if (a.splits > 1) {
+    blk += split * a.chunk;
+    if (split + 1 < a.splits) blk_end = min(blk_end, blk + a.chunk);   // the last chunk takes what a longer cache than announced holds
+  }
+  const Column<D> k = load_column<D, KIND>(a, rows, sight, row0 + (lane & 31), n_rows, head);
+  f16v acc[KC];
+#pragma unroll
+  for (int t = 0; t < KC; ++t) acc[t] = f16v{0};
+  float m = NEVER, l = 0.0f, lv_top = -__builtin_inff();
+  const float one = opaque_one();
+  int j = blk + wave;
+  Blocks blocks;
+  blocks.step = WAVES;
+  const int k_off = lane * 16, v_off = (lane & 31) * 32 + (lane >> 5) * 16;
+  auto load = [&](const uint8_t* from, int which, int off, uint4 (&r)[KC]) {
+    const uint8_t* p = from + blocks.at(which) * (D * KV_BLOCK);
+#pragma unroll
+    for (int i = 0; i < KC; ++i) r[i] = *reinterpret_cast<const uint4*>(p + i * 1024 + off);
+  };
+  if (j < blk_end) {
+    // K's registers are loaded with the next block as soon as the products with them are issued, V's likewise: each load
+    // has the other half of a step to arrive in.
+    uint4 kr[KC], vr[KC];
+    blocks.lookup(a.cache, seq, head, j, blk_end);
+    load(a.cache.k, j, k_off, kr);
+    load(a.cache.v, j, v_off, vr);
+    for (; j < blk_end; j += WAVES) {
+      const Scales b = scales_of(blocks, j, lv_top);
+      f16v s = f16v{0};
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bytes8_to_half(kr[i].x, kr[i].y), k.q[2 * i], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(bytes8_to_half(kr[i].z, kr[i].w), k.q[2 * i + 1], s, 0, 0, 0);
+      }
+      const int next = j + WAVES, key0 = j * KV_BLOCK;
+      if (blocks.slot(next) >= 64) blocks.lookup(a.cache, seq, head, next, blk_end);
+      load(a.cache.k, next, k_off, kr);
+      h8 p[2];
+      softmax_block<D>(s, k, b, key0 + KV_BLOCK > lim_first || key0 < lo_last, key0, one, m, l, p, [&](float f) {
+#pragma unroll
+        for (int t = 0; t < KC; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][i] *= f;
+      });
+#pragma unroll
+      for (int t = 0; t < KC; ++t) {
+        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bytes8_to_half(vr[t].x, vr[t].y), p[0], acc[t], 0, 0, 0);
+        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bytes8_to_half(vr[t].z, vr[t].w), p[1], acc[t], 0, 0, 0);
+      }
+      load(a.cache.v, next, v_off, vr);
+    }
+  }
+  l += other_half(l);
+
+  // Join the four waves: 2 and 3 into 0 and 1, then 1 into 0; through at most 32 KB of LDS.
+  constexpr int PART = KC < 4 ? KC : 4;
+  __shared__ float lds_acc[2][PART][16][64];
+  __shared__ float lds_ml[2][2][64];
+#pragma unroll
+  for (int other = WAVES / 2; other >= 1; other >>= 1) {
+    float f = 1.0f, f2 = 0.0f;
+#pragma unroll
+    for (int t0 = 0; t0 < KC; t0 += PART) {
+      if (wave >= other && wave < 2 * other) {
+        lds_ml[wave - other][0][lane] = m;
+        lds_ml[wave - other][1][lane] = l;
+#pragma unroll
+        for (int t = 0; t < PART; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) lds_acc[wave - other][t][i][lane] = acc[t0 + t][i];
+      }
+      __syncthreads();
+      if (wave < other) {
+        if (t0 == 0) {
+          const float m2 = lds_ml[wave][0][lane], l2 = lds_ml[wave][1][lane], to = fmaxf(m, m2);
+          f = __builtin_amdgcn_exp2f(m - to);
+          f2 = __builtin_amdgcn_exp2f(m2 - to);
+          m = to;
+          l = l * f + l2 * f2;
+        }
+#pragma unroll
+        for (int t = 0; t < PART; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t0 + t][i] = acc[t0 + t][i] * f + lds_acc[wave][t][i][lane] * f2;
+      }
+      __syncthreads();
+    }
+  }
+  if (wave == 0) store_column<D, KIND>(a, k, head, split, m, l, acc);
+}
+
+// ---- many rows: eight waves with 32 rows each walk over the keys together ------------------------------------------
 // grid (KV heads, row tiles, batch * splits): heads in front, so that with 8 of them each XCD keeps one head's cache in
 // its L2; the tiles of the latest queries, which see the most keys, start first.
-template <int D, int KIND, int NT, bool KEYS>
-__global__ void __launch_bounds__(WAVES * 64, NT == 1 && D <= 128 ? 2 : 1) paged_attention_kernel(AttnArgs a) {
-  constexpr int KC = D / 32;           // 16-byte loads of K a lane, and tiles of 32 dims of V
-  constexpr int TILE = KEYS ? 32 * NT : 32 * NT * WAVES;
+//
+// Converting a block to fp16 costs a wave as much as its matrix products (packed fp16 subtractions run at half rate), so
+// the eight waves convert a block once, each an eighth, into LDS, in operand order: a lane reads its 16 bytes of every
+// operand at lane * 16.  Two buffers and one barrier a block: while block j is worked on, j + 1 is converted from
+// registers into the other buffer and j + 2 is on its way from memory.
+template <int D, int KIND>
+__global__ void __launch_bounds__(ROW_WAVES * 64, 2) attention_rows_kernel(AttnArgs a) {
+  constexpr int KC = D / 32, PIECES = 4 * KC, MINE = PIECES / ROW_WAVES;   // operand pieces of a block: K's, then V's
+  __shared__ h8 lds[2][PIECES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, half = lane >> 5;
   const int head = blockIdx.x;
   const int seq = blockIdx.z / a.splits, split = blockIdx.z - seq * a.splits;
   const SeqRows rows = seq_rows(a.q_start, seq, a.tokens);
   const int n_rows = static_cast<int>(rows.count) * a.group;
-  const int tile = gridDim.y - 1 - blockIdx.y;
-  const int row0 = tile * TILE + (KEYS ? 0 : wave * 32 * NT);
-  if (tile * TILE >= n_rows) return;
-  const bool idle = row0 >= n_rows;                    // (prompts) this wave has no rows, but the barriers are not its own
-  if (!KEYS && idle) return;
-  const int kv_len = min(max(a.kv_lens[seq], 0), MAX_KV);
-  const int q_len = static_cast<int>(rows.count);
-
-  // Keys that the wave's rows see: [lo of the first row, lim of the last one).
-  auto limit = [&](int query) { return min(max(kv_len - q_len + query + 1, 0), kv_len); };
-  auto lower = [&](int query) { return a.window > 0 ? max(kv_len - q_len + query + 1 - a.window, 0) : 0; };
-  const int last_row = min(row0 + 32 * NT, n_rows) - 1;
-  const int first_q = row0 / a.group, last_q = last_row / a.group;
-  const int lim_first = limit(first_q), lim_last = limit(last_q);
-  const int lo_first = lower(first_q), lo_last = lower(last_q);
-  // Chunks are laid from the first block that the first query of the tile sees.
-  const int tile_lo = KEYS ? lo_first : lower(tile * TILE / a.group);
-  int blk = lo_first >> 5;
-  int blk_end = (lim_last + 31) >> 5;
+  const int tile0 = (gridDim.y - 1 - blockIdx.y) * ROW_TILE, row0 = tile0 + wave * 32;
+  if (tile0 >= n_rows) return;
+  const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
+  // Blocks that the tile, and that this wave sees.
+  int blk = sight.lower(tile0 / a.group) >> 5;
+  int blk_end = (sight.limit((min(tile0 + ROW_TILE, n_rows) - 1) / a.group) + 31) >> 5;
   if (a.splits > 1) {
-    const int from = (tile_lo >> 5) + split * a.chunk;
-    blk = max(blk, from);
-    if (split + 1 < a.splits) blk_end = min(blk_end, from + a.chunk);   // the last chunk takes what a longer cache than announced holds
+    blk += split * a.chunk;
+    if (split + 1 < a.splits) blk_end = min(blk_end, blk + a.chunk);
   }
+  const int first_q = min(row0, n_rows - 1) / a.group, last_q = (min(row0 + 32, n_rows) - 1) / a.group;
+  const int lim_first = sight.limit(first_q), lo_last = sight.lower(last_q);
+  const int own = sight.lower(first_q) >> 5, own_end = row0 < n_rows ? (sight.limit(last_q) + 31) >> 5 : 0;
 
-  // Q^T as the MFMA's second operand: lane (column, half) holds dims 32 i + 16 half + 8 b .. + 7.
-  h8 q[NT][2 * KC];
-  float q_exp[NT];
-  int lim[NT], lo[NT];
-  bool valid[NT];
-  int64_t out_at[NT];
+  const Column<D> k = load_column<D, KIND>(a, rows, sight, row0 + (lane & 31), n_rows, head);
+  f16v acc[KC];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = row0 + 32 * n + col;
-    valid[n] = r < n_rows;
-    const int query = valid[n] ? r / a.group : 0, member = valid[n] ? r - query * a.group : 0;
-    lim[n] = limit(query);
-    lo[n] = lower(query);
-    const int64_t row = rows.first + query;
-    const int64_t at = static_cast<int64_t>(head * a.group + member) * D;
-    out_at[n] = row * a.out_stride + at;
-    float x[2 * KC][8];
-    float amax = 0.0f;
+  for (int t = 0; t < KC; ++t) acc[t] = f16v{0};
+  float m = NEVER, l = 0.0f, lv_top = -__builtin_inff();
+  const float one = opaque_one();
+  Blocks blocks, before;          // `before`: the last lookup but one, for scales of blocks still to be worked on
+  blocks.step = before.step = 1;
+  uint2 raw[MINE];
+  auto fetch = [&](int which) {
+    const int64_t at = blocks.at(which) * (D * KV_BLOCK);
 #pragma unroll
-    for (int i = 0; i < 2 * KC; ++i) {
-      load8_f32<KIND>(a.q, row * a.q_stride + at + 32 * (i >> 1) + 16 * half + 8 * (i & 1), x[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[i][j]));
-    }
-    int e = 0;
-    if constexpr (KIND == KIND_BF16) {
-      amax = fmaxf(amax, other_half(amax));
-      e = max(static_cast<int>(float_to_bits(amax) >> 23), 1) - 127;
-    }
-    q_exp[n] = ldexpf(1.0f, e) * a.scale;
-#pragma unroll
-    for (int i = 0; i < 2 * KC; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[n][i][j] = static_cast<_Float16>(KIND == KIND_BF16 ? ldexpf(x[i][j], -e) : x[i][j]);
-  }
-
-  f16v acc[KC][NT];
-  float m[NT], l[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = NEVER;
-    l[n] = 0.0f;
-#pragma unroll
-    for (int t = 0; t < KC; ++t) acc[t][n] = f16v{0};
-  }
-
-  const int step = KEYS ? WAVES : 1;
-  int j = blk + (KEYS ? wave : 0);
-  // Block numbers and scales of the next 64 of the wave's blocks, one a lane.
-  int base = j;
-  int64_t block_of = -1;
-  float ks_of = 0.0f, lv_of = 0.0f, iv_of = 0.0f;
-  auto lookup = [&] {
-    base = j;
-    const int mine = j + lane * step;
-    block_of = mine < blk_end ? kv_block_index(a.cache, seq, mine, head) : -1;
-    if (block_of >= 0) {
-      const float vs = a.cache.v_scale[block_of];
-      const float v_clean = fmaxf(vs, KV_SCALE_FLOOR);          // of a NaN: the floor
-      ks_of = a.cache.k_scale[block_of];
-      lv_of = vs == vs ? log2f(v_clean) : vs;
-      iv_of = 1.0f / v_clean;
+    for (int r = 0; r < MINE; ++r) {
+      const int piece = wave + ROW_WAVES * r, i = piece % (2 * KC);
+      const uint8_t* from = piece < 2 * KC ? a.cache.k + lane * 16 : a.cache.v + (lane & 31) * 32 + (lane >> 5) * 16;
+      raw[r] = *reinterpret_cast<const uint2*>(from + at + (i >> 1) * 1024 + (i & 1) * 8);
     }
   };
-  auto block_at = [&](int which) -> int64_t {
-    const int k = (which - base) / step;
-    const uint32_t lo32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(block_of), k));
-    const uint32_t hi32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(block_of >> 32), k));
-    return static_cast<int64_t>((static_cast<uint64_t>(hi32) << 32) | lo32);
+  auto convert = [&](int buffer) {
+#pragma unroll
+    for (int r = 0; r < MINE; ++r) lds[buffer][wave + ROW_WAVES * r][lane] = bytes8_to_half(raw[r].x, raw[r].y);
   };
-  float lv_top = -__builtin_inff();
-  const int k_off = lane * 16, v_off = col * 32 + half * 16;
-
-  while (j < blk_end) {
-    if (j == blk + (KEYS ? wave : 0) || j - base >= 64 * step) lookup();
-    const int slot = (j - base) / step;
-    const int64_t block = block_at(j);
-    if (block < 0) { j += step; continue; }              // a bad page: its keys are not there
-    const uint8_t* kp = a.cache.k + block * (D * KV_BLOCK);
-    const uint8_t* vp = a.cache.v + block * (D * KV_BLOCK);
-    uint4 kr[KC], vr[KC];
+  if (blk < blk_end) {
+    blocks.lookup(a.cache, seq, head, blk, blk_end);
+    before = blocks;
+    fetch(blk);
+    convert(0);
+    fetch(blk + 1);                // (behind the end: block 0's bytes, never used)
+    for (int j = blk; j < blk_end; ++j) {
+      const int buffer = (j - blk) & 1;
+      lds_barrier();               // block j is in LDS, and nobody reads the other buffer any more
+      const bool mine = j >= own && j < own_end;
+      f16v s = f16v{0};
+      if (mine) {
 #pragma unroll
-    for (int i = 0; i < KC; ++i) kr[i] = *reinterpret_cast<const uint4*>(kp + i * 1024 + k_off);
-#pragma unroll
-    for (int i = 0; i < KC; ++i) vr[i] = *reinterpret_cast<const uint4*>(vp + i * 1024 + v_off);
-    const float ks = read_lane_f(ks_of, slot), lv = read_lane_f(lv_of, slot), iv = read_lane_f(iv_of, slot);
-
-    f16v s[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n] = f16v{0};
-#pragma unroll
-    for (int i = 0; i < KC; ++i) {
-      const h8 k0 = bytes8_to_half(kr[i].x, kr[i].y), k1 = bytes8_to_half(kr[i].z, kr[i].w);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, q[n][2 * i], s[n], 0, 0, 0);
-        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, q[n][2 * i + 1], s[n], 0, 0, 0);
+        for (int i = 0; i < 2 * KC; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds[buffer][i][lane], k.q[i], s, 0, 0, 0);
       }
-    }
-
-    // A block whose V scale is less than a quarter of the largest so far: its w may be lost in fp16 although its p counts
-    // in the sum, which then takes p itself, at the price of 16 more exponentials.
-    lv_top = fmaxf(lv_top, lv);
-    const bool far = lv < lv_top - 2.0f;
-    const int key0 = j * KV_BLOCK;
-    const bool masked = key0 + KV_BLOCK > lim_first || key0 < lo_last;   // some row does not see the whole block
-    h8 p[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float c = ks * q_exp[n];
-      // s is raw here; the argument of row n is fma(s, c, lv), and c > 0 keeps the order.
-      float top = -__builtin_inff();
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
-          if (key < lim[n] && key >= lo[n]) top = fmaxf(top, s[n][i]);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
+      convert(buffer ^ 1);
+      if (blocks.slot(j + 2) >= 64) {
+        before = blocks;
+        blocks.lookup(a.cache, seq, head, j + 2, blk_end);
       }
-      top = fmaxf(top, other_half(top));
-      const float high = fmaf(top, c, lv);                // NaN (a poisoned block, or nothing seen at a zero c) moves nothing
-      if (__any(high > m[n] + HEADROOM)) {
-        const float to = fmaxf(m[n], high);
-        const float f = __builtin_amdgcn_exp2f(m[n] - to);
-        m[n] = to;
-        l[n] *= f;
+      fetch(j + 2);
+      if (mine) {
+        const Scales b = scales_of(j >= blocks.base ? blocks : before, j, lv_top);
+        const int key0 = j * KV_BLOCK;
+        h8 p[2];
+        softmax_block<D>(s, k, b, key0 + KV_BLOCK > lim_first || key0 < lo_last, key0, one, m, l, p, [&](float f) {
 #pragma unroll
-        for (int t = 0; t < KC; ++t)
+          for (int t = 0; t < KC; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t][n][i] *= f;
+            for (int i = 0; i < 16; ++i) acc[t][i] *= f;
+        });
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int t = 0; t < KC; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds[buffer][2 * KC + 2 * t + h][lane], p[h], acc[t], 0, 0, 0);
       }
-      const float shift = lv - m[n] + OFFSET;
-      float w[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, shift));
-      if (masked) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
-          w[i] = key < lim[n] && key >= lo[n] ? w[i] : 0.0f;
-        }
-      }
-      if (far) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, OFFSET - m[n]));
-          l[n] += !masked || (key < lim[n] && key >= lo[n]) ? e : 0.0f;
-        }
-      }
-      float sum = 0.0f;
-      const h2 one = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const h2 r = __builtin_convertvector((f2v{w[i], w[i + 1]}), h2);
-        p[n][i >> 3][i & 7] = r.x;
-        p[n][i >> 3][(i & 7) + 1] = r.y;
-        sum = __builtin_amdgcn_fdot2(r, one, sum, false);
-      }
-      if (!far) l[n] = fmaf(sum, iv, l[n]);
-    }
-
-#pragma unroll
-    for (int t = 0; t < KC; ++t) {
-      const h8 v0 = bytes8_to_half(vr[t].x, vr[t].y), v1 = bytes8_to_half(vr[t].z, vr[t].w);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, p[n][0], acc[t][n], 0, 0, 0);
-        acc[t][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, p[n][1], acc[t][n], 0, 0, 0);
-      }
-    }
-    j += step;
-  }
-
-#pragma unroll
-  for (int n = 0; n < NT; ++n) l[n] += other_half(l[n]);
-
-  if constexpr (KEYS) {
-    // Join the four waves: 2 and 3 into 0 and 1, then 1 into 0; through at most 32 KB of LDS.
-    constexpr int PART = KC < 4 ? KC : 4;
-    __shared__ float lds_acc[2][PART][NT][16][64];
-    __shared__ float lds_ml[2][NT][2][64];
-#pragma unroll
-    for (int other = WAVES / 2; other >= 1; other >>= 1) {
-      const bool gives = wave >= other && wave < 2 * other;
-      float f[NT], f2[NT];
-#pragma unroll
-      for (int t0 = 0; t0 < KC; t0 += PART) {
-        if (gives) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            lds_ml[wave - other][n][0][lane] = m[n];
-            lds_ml[wave - other][n][1][lane] = l[n];
-#pragma unroll
-            for (int t = 0; t < PART; ++t)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) lds_acc[wave - other][t][n][i][lane] = acc[t0 + t][n][i];
-          }
-        }
-        __syncthreads();
-        if (wave < other) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            if (t0 == 0) {
-              const float m2 = lds_ml[wave][n][0][lane], l2 = lds_ml[wave][n][1][lane], to = fmaxf(m[n], m2);
-              f[n] = __builtin_amdgcn_exp2f(m[n] - to);
-              f2[n] = __builtin_amdgcn_exp2f(m2 - to);
-              m[n] = to;
-              l[n] = l[n] * f[n] + l2 * f2[n];
-            }
-#pragma unroll
-            for (int t = 0; t < PART; ++t)
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                acc[t0 + t][n][i] = acc[t0 + t][n][i] * f[n] + lds_acc[wave][t][n][i][lane] * f2[n];
-          }
-        }
-        __syncthreads();
-      }
-    }
-    if (wave != 0) return;
-  }
-
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    if (!valid[n]) continue;
-    if (a.splits > 1) {
-      const int64_t query = (row0 + 32 * n + col) / a.group, member = (row0 + 32 * n + col) - query * a.group;
-      const int64_t at = (static_cast<int64_t>(split) * a.tokens + rows.first + query) * a.q_heads + head * a.group + member;
-      if (half == 0) {
-        a.part_ml[2 * at] = m[n];
-        a.part_ml[2 * at + 1] = l[n];
-      }
-#pragma unroll
-      for (int t = 0; t < KC; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4*>(a.part_acc + at * D + 32 * t + 2 * i + 4 * half) =
-              make_float4(acc[t][n][i], acc[t][n][i + 1], acc[t][n][i + 2], acc[t][n][i + 3]);
-    } else {
-      const float r = l[n] == 0.0f ? 0.0f : 1.0f / l[n];   // a row that saw no key gives zeros
-#pragma unroll
-      for (int t = 0; t < KC; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          uint32_t w[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            w[b] = half_bits<KIND>(acc[t][n][i + 2 * b] * r) | (half_bits<KIND>(acc[t][n][i + 2 * b + 1] * r) << 16);
-          __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(a.out) + out_at[n] + 32 * t + 2 * i + 4 * half, 2), w, 8);
-        }
     }
   }
+  l += other_half(l);
+  store_column<D, KIND>(a, k, head, split, m, l, acc);
 }
 
 // Joins the chunks of one output row: grid (rows a sequence, batch), one wave a row, D / 64 dims a lane.
@@ -429,8 +542,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
 
 // How a call is cut: decided from sizes alone, so that the workspace can be sized before the call.
 struct Plan {
-  bool keys;          // the waves of a workgroup share rows and split keys
-  int nt;
+  bool keys;          // few rows: the waves of a workgroup share them and split keys
   int tile_rows;
   int64_t tiles;
   int most_splits;    // what the workspace is sized for: no fewer for fewer keys
@@ -443,14 +555,13 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   Plan p;
   const int64_t rows = max_q * (q_heads / kv_heads);
   p.keys = rows <= 64;
-  p.nt = 1;
-  p.tile_rows = p.keys ? 32 * p.nt : 32 * p.nt * WAVES;
+  p.tile_rows = p.keys ? 32 : ROW_TILE;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // Keys that a tile can see.
   int64_t span = max_kv;
   if (window > 0 && window + max_q + 31 < span) span = window + max_q + 31;
   const int64_t blocks = (span + 31) / 32 + (window > 0 ? 1 : 0);
-  const int64_t groups = batch * kv_heads * p.tiles, want = 2 * CUS;
+  const int64_t groups = batch * kv_heads * p.tiles, want = p.keys ? 2 * CUS : CUS;
   int64_t splits = (want + groups - 1) / groups;
   const int64_t least = p.keys ? 16 : 32;               // blocks worth a workgroup of its own
   const int64_t most = (blocks + least - 1) / least;
@@ -479,9 +590,8 @@ int64_t workspace_of(int splits, int64_t tokens, int64_t q_heads, int64_t dim) {
 template <int D, int KIND>
 int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64_t kv_heads, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.tiles), static_cast<unsigned>(batch * p.splits));
-  const dim3 threads(WAVES * 64);
-  if (p.keys) hipLaunchKernelGGL((paged_attention_kernel<D, KIND, 1, true>), grid, threads, 0, stream, a);
-  else hipLaunchKernelGGL((paged_attention_kernel<D, KIND, 1, false>), grid, threads, 0, stream, a);
+  if (p.keys) hipLaunchKernelGGL((attention_keys_kernel<D, KIND>), grid, dim3(WAVES * 64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(ROW_WAVES * 64), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
   const dim3 join(static_cast<unsigned>((max_q * a.q_heads + 3) / 4), static_cast<unsigned>(batch));
@@ -543,5 +653,5 @@ extern "C" int hipengine_gfx950_paged_attention_q8(const void* q, void* out, int
 
 int hipengine_gfx950::paged_attention_load() {
   hipFuncAttributes attr;
-  return static_cast<int>(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(paged_attention_kernel<128, KIND_BF16, 1, true>)));
+  return static_cast<int>(hipFuncGetAttributes(&attr, reinterpret_cast<const void*>(attention_keys_kernel<128, KIND_BF16>)));
 }
