@@ -40,8 +40,6 @@ typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int WAVES = 4;               // of attention_keys_kernel
-constexpr int ROW_WAVES = 8;           // of attention_rows_kernel, each with 32 rows
-constexpr int ROW_TILE = 32 * ROW_WAVES;
 constexpr int MAX_KV = 1 << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEVER = -1e30f;        // a maximum before any key: finite, so that differences to it are no NaN
@@ -396,36 +394,44 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
   if (wave == 0) store_column<D, KIND>(a, k, head, split, m, l, acc);
 }
 
-// ---- many rows: eight waves with 32 rows each walk over the keys together ------------------------------------------
+// ---- many rows: the waves of a workgroup have 32 rows each and walk over the keys together --------------------------
 // grid (KV heads, row tiles, batch * splits): heads in front, so that with 8 of them each XCD keeps one head's cache in
 // its L2; the tiles of the latest queries, which see the most keys, start first.
 //
 // Converting a block to fp16 costs a wave as much as its matrix products (packed fp16 subtractions run at half rate), so
-// the eight waves convert a block once, each an eighth, into LDS, in operand order: a lane reads its 16 bytes of every
-// operand at lane * 16.  Two buffers and one barrier a block: while block j is worked on, j + 1 is converted from
-// registers into the other buffer and j + 2 is on its way from memory.
+// the waves convert a block once, each its share, into LDS, in operand order: a lane reads its 16 bytes of every operand
+// at lane * 16.  Softmax and matrix products of one block depend on each other, so the products K Q^T of the next block run
+// behind the exponentials of this one: in step j a wave reads K of j + 1 and V of j, converts K of j + 2 and V of j + 1
+// into the buffers that step j - 1 read, and asks memory for K of j + 3 and V of j + 2.  One barrier a step.
+template <int D>
+struct RowShape {
+  static constexpr int WAVES = D <= 128 ? 8 : 4;       // heads of 256: 192 registers a wave for O and Q alone
+  static constexpr int TILE = 32 * WAVES;
+};
+
 template <int D, int KIND>
-__global__ void __launch_bounds__(ROW_WAVES * 64, 2) attention_rows_kernel(AttnArgs a) {
-  constexpr int KC = D / 32, PIECES = 4 * KC, MINE = PIECES / ROW_WAVES;   // operand pieces of a block: K's, then V's
-  __shared__ h8 lds[2][PIECES][64];
+__global__ void __launch_bounds__(RowShape<D>::WAVES * 64, D <= 128 ? 2 : 1) attention_rows_kernel(AttnArgs a) {
+  constexpr int W = RowShape<D>::WAVES, TILE = RowShape<D>::TILE;
+  constexpr int KC = D / 32, PIECES = 2 * KC, MINE = PIECES > W ? PIECES / W : 1;   // operand pieces of K, and of V
+  __shared__ h8 lds_k[2][PIECES][64];
+  __shared__ h8 lds_v[2][PIECES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.x;
   const int seq = blockIdx.z / a.splits, split = blockIdx.z - seq * a.splits;
   const SeqRows rows = seq_rows(a.q_start, seq, a.tokens);
   const int n_rows = static_cast<int>(rows.count) * a.group;
-  const int tile0 = (gridDim.y - 1 - blockIdx.y) * ROW_TILE, row0 = tile0 + wave * 32;
+  const int tile0 = (gridDim.y - 1 - blockIdx.y) * TILE, row0 = tile0 + wave * 32;
   if (tile0 >= n_rows) return;
   const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
-  // Blocks that the tile, and that this wave sees.
+  // Blocks that the tile sees; a wave's own rows may see fewer, it masks the rest.
   int blk = sight.lower(tile0 / a.group) >> 5;
-  int blk_end = (sight.limit((min(tile0 + ROW_TILE, n_rows) - 1) / a.group) + 31) >> 5;
+  int blk_end = (sight.limit((min(tile0 + TILE, n_rows) - 1) / a.group) + 31) >> 5;
   if (a.splits > 1) {
     blk += split * a.chunk;
     if (split + 1 < a.splits) blk_end = min(blk_end, blk + a.chunk);
   }
-  const int first_q = min(row0, n_rows - 1) / a.group, last_q = (min(row0 + 32, n_rows) - 1) / a.group;
-  const int lim_first = sight.limit(first_q), lo_last = sight.lower(last_q);
-  const int own = sight.lower(first_q) >> 5, own_end = row0 < n_rows ? (sight.limit(last_q) + 31) >> 5 : 0;
+  const int lim_first = sight.limit(min(row0, n_rows - 1) / a.group);
+  const int lo_last = sight.lower((min(row0 + 32, n_rows) - 1) / a.group);
 
   const Column<D> k = load_column<D, KIND>(a, rows, sight, row0 + (lane & 31), n_rows, head);
   f16v acc[KC];
@@ -433,59 +439,142 @@ __global__ void __launch_bounds__(ROW_WAVES * 64, 2) attention_rows_kernel(AttnA
   for (int t = 0; t < KC; ++t) acc[t] = f16v{0};
   float m = NEVER, l = 0.0f, lv_top = -__builtin_inff();
   const float one = opaque_one();
-  Blocks blocks, before;          // `before`: the last lookup but one, for scales of blocks still to be worked on
-  blocks.step = before.step = 1;
-  uint2 raw[MINE];
-  auto fetch = [&](int which) {
-    const int64_t at = blocks.at(which) * (D * KV_BLOCK);
+  Blocks blocks;
+  blocks.step = 1;
+  // Of the blocks whose K was asked for last, last but one and so on: number, scales.
+  int64_t n_last = 0;
+  Scales s1{}, s2{}, s3{};
+  uint2 raw_k[MINE], raw_v[MINE];
+  auto piece_of = [&](int r) { return (wave + W * r) % PIECES; };     // (fewer pieces than waves: some convert the same one)
+  auto fetch_v = [&] {
+    const uint8_t* from = a.cache.v + n_last * (D * KV_BLOCK) + (lane & 31) * 32 + (lane >> 5) * 16;
 #pragma unroll
     for (int r = 0; r < MINE; ++r) {
-      const int piece = wave + ROW_WAVES * r, i = piece % (2 * KC);
-      const uint8_t* from = piece < 2 * KC ? a.cache.k + lane * 16 : a.cache.v + (lane & 31) * 32 + (lane >> 5) * 16;
-      raw[r] = *reinterpret_cast<const uint2*>(from + at + (i >> 1) * 1024 + (i & 1) * 8);
+      const int i = piece_of(r);
+      raw_v[r] = *reinterpret_cast<const uint2*>(from + (i >> 1) * 1024 + (i & 1) * 8);
     }
   };
-  auto convert = [&](int buffer) {
+  auto fetch_k = [&](int which) {
+    if (blocks.slot(which) >= 64) blocks.lookup(a.cache, seq, head, which, blk_end);
+    n_last = blocks.at(which);
+    const int slot = blocks.slot(which);
+    s1 = s2;
+    s2 = s3;
+    s3 = Scales{read_lane_f(blocks.ks, slot), read_lane_f(blocks.lv, slot), read_lane_f(blocks.iv, slot), false};
+    const uint8_t* from = a.cache.k + n_last * (D * KV_BLOCK) + lane * 16;
 #pragma unroll
-    for (int r = 0; r < MINE; ++r) lds[buffer][wave + ROW_WAVES * r][lane] = bytes8_to_half(raw[r].x, raw[r].y);
+    for (int r = 0; r < MINE; ++r) {
+      const int i = piece_of(r);
+      raw_k[r] = *reinterpret_cast<const uint2*>(from + (i >> 1) * 1024 + (i & 1) * 8);
+    }
+  };
+  auto convert_k = [&](int buffer) {
+#pragma unroll
+    for (int r = 0; r < MINE; ++r) lds_k[buffer][piece_of(r)][lane] = bytes8_to_half(raw_k[r].x, raw_k[r].y);
+  };
+  auto convert_v = [&](int buffer) {
+#pragma unroll
+    for (int r = 0; r < MINE; ++r) lds_v[buffer][piece_of(r)][lane] = bytes8_to_half(raw_v[r].x, raw_v[r].y);
+  };
+  // The softmax's constants of a block for this lane's column, and its raw products made ready: keys that the column does
+  // not see at -infinity (at 0 under a weight of 0 where it sees none: a block's NaN must not reach it).
+  const int half = lane >> 5;
+  f16v s = f16v{0};
+  float c = 0.0f, shift = 0.0f, p_shift = 0.0f, iv = 0.0f;
+  bool far = false;
+  auto ready = [&](int j, const Scales& b) {
+    const int key0 = j * KV_BLOCK;
+    c = b.ks * k.c;
+    c = c < 1e-37f ? 1e-37f : c;                   // (a NaN stays)
+    float lv = b.lv;
+    bool none = false;
+    if (key0 + KV_BLOCK > lim_first || key0 < lo_last) {
+      none = key0 >= k.lim || key0 + KV_BLOCK <= k.lo;
+      c = none ? 0.0f : c;
+      lv = none ? -__builtin_inff() : lv;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
+        s[i] = key < k.lim && key >= k.lo ? s[i] : none ? 0.0f : -__builtin_inff();
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+    top = fmaxf(top, other_half(top));
+    const float high = fmaf(top, c, lv);           // a NaN (a poisoned block) moves nothing
+    if (__any(high > m + HEADROOM)) {
+      const float to = fmaxf(m, high);
+      const float f = __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l *= f;
+#pragma unroll
+      for (int t = 0; t < KC; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] *= f;
+    }
+    lv_top = fmaxf(lv_top, b.lv);
+    far = b.lv < lv_top - 2.0f && b.lv > -__builtin_inff();
+    shift = lv - m + OFFSET;
+    p_shift = none ? -__builtin_inff() : OFFSET - m;
+    iv = far ? 0.0f : b.iv;
   };
   if (blk < blk_end) {
     blocks.lookup(a.cache, seq, head, blk, blk_end);
-    before = blocks;
-    fetch(blk);
-    convert(0);
-    fetch(blk + 1);                // (behind the end: block 0's bytes, never used)
+    fetch_k(blk);
+    fetch_v();
+    convert_k(0);
+    convert_v(0);
+    fetch_k(blk + 1);              // (behind the end: block 0's bytes under a weight of 0)
+    convert_k(1);
+    fetch_v();                     // of blk + 1
+    fetch_k(blk + 2);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_k[0][i][lane], k.q[i], s, 0, 0, 0);
+    ready(blk, s1);
     for (int j = blk; j < blk_end; ++j) {
-      const int buffer = (j - blk) & 1;
-      lds_barrier();               // block j is in LDS, and nobody reads the other buffer any more
-      const bool mine = j >= own && j < own_end;
-      f16v s = f16v{0};
-      if (mine) {
+      const int here = (j - blk) & 1;
+      lds_barrier();               // K of j + 1 and V of j are in LDS, and nobody reads what step j - 1 did
+      if (far) {
+        // w may be lost in fp16 although p counts in the sum, which then takes p itself: 16 more exponentials.
+        float e = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2 * KC; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds[buffer][i][lane], k.q[i], s, 0, 0, 0);
+        for (int i = 0; i < 16; ++i) e += __builtin_amdgcn_exp2f(fmaf(s[i], c, p_shift));
+        l += e;
       }
-      convert(buffer ^ 1);
-      if (blocks.slot(j + 2) >= 64) {
-        before = blocks;
-        blocks.lookup(a.cache, seq, head, j + 2, blk_end);
+      h8 kf[PIECES], vf[PIECES];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) kf[i] = lds_k[here ^ 1][i][lane];
+      f16v next = f16v{0};
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], k.q[i], next, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) vf[i] = lds_v[here][i][lane];
+      convert_k(here);
+      convert_v(here ^ 1);
+      // P of block j, summed as rounded, its subnormals too (the dot product instruction would take those as 0):
+      // v_fma_mix_f32 with a `one` that the compiler does not see through.
+      h8 p[2];
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float w0 = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, shift));
+        const h2 r = __builtin_convertvector((f2v{w0, w1}), h2);
+        p[i >> 3][i & 7] = r.x;
+        p[i >> 3][(i & 7) + 1] = r.y;
+        sum = fmaf(static_cast<float>(r.x), one, sum);
+        sum = fmaf(static_cast<float>(r.y), one, sum);
       }
-      fetch(j + 2);
-      if (mine) {
-        const Scales b = scales_of(j >= blocks.base ? blocks : before, j, lv_top);
-        const int key0 = j * KV_BLOCK;
-        h8 p[2];
-        softmax_block<D>(s, k, b, key0 + KV_BLOCK > lim_first || key0 < lo_last, key0, one, m, l, p, [&](float f) {
+      l = fmaf(sum, iv, l);
 #pragma unroll
-          for (int t = 0; t < KC; ++t)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[t][i] *= f;
-        });
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int t = 0; t < KC; ++t)
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds[buffer][2 * KC + 2 * t + h][lane], p[h], acc[t], 0, 0, 0);
-      }
+        for (int t = 0; t < KC; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[2 * t + h], p[h], acc[t], 0, 0, 0);
+      fetch_v();                   // of j + 2
+      fetch_k(j + 3);
+      s = next;
+      ready(j + 1, s1);
     }
   }
   l += other_half(l);
@@ -555,7 +644,7 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   Plan p;
   const int64_t rows = max_q * (q_heads / kv_heads);
   p.keys = rows <= 64;
-  p.tile_rows = p.keys ? 32 : ROW_TILE;
+  p.tile_rows = p.keys ? 32 : dim <= 128 ? RowShape<128>::TILE : RowShape<256>::TILE;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // Keys that a tile can see.
   int64_t span = max_kv;
@@ -591,7 +680,7 @@ template <int D, int KIND>
 int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64_t kv_heads, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.tiles), static_cast<unsigned>(batch * p.splits));
   if (p.keys) hipLaunchKernelGGL((attention_keys_kernel<D, KIND>), grid, dim3(WAVES * 64), 0, stream, a);
-  else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(ROW_WAVES * 64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(RowShape<D>::WAVES * 64), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
   const dim3 join(static_cast<unsigned>((max_q * a.q_heads + 3) / 4), static_cast<unsigned>(batch));
