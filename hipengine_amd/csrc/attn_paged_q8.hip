@@ -40,10 +40,12 @@ typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int WAVES = 4;               // of attention_keys_kernel
+constexpr int ROW_WAVES = 4;           // of attention_rows_kernel, each with 32 rows
 constexpr int MAX_KV = 1 << 30;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NEVER = -1e30f;        // a maximum before any key: finite, so that differences to it are no NaN
+constexpr float NEVER = -3e38f;        // a maximum before any key: finite, so that differences to it are no NaN
 constexpr float HEADROOM = 8.0f;       // log2 by which a row's maximum may pass its reference before rows are rescaled
+constexpr float RANGE = 32768.0f;      // of a sum of P above which the reference is moved (fp16 ends at 65504)
 constexpr float OFFSET = 7.0f;         // log2 of P at the reference: P <= 2^15, and fp16's least step is 2^-31 of it
 
 struct AttnArgs {
@@ -109,8 +111,6 @@ struct Column {
   h8 q[D / 16];
   float c;             // argument of the softmax, in log2, per raw product and unit of K's scale
   int lim, lo;
-  bool valid;
-  int64_t row, member; // of the batch; of the KV head's group
 };
 
 template <int D, int KIND>
@@ -118,30 +118,32 @@ __device__ __forceinline__ Column<D> load_column(const AttnArgs& a, const SeqRow
   constexpr int P = D / 16;
   const int half = (threadIdx.x & 63) >> 5;
   Column<D> k;
-  k.valid = r < n_rows;
-  const int query = k.valid ? r / a.group : 0;
-  k.member = k.valid ? r - query * a.group : 0;
+  if (r >= n_rows) r = 0;              // (some row, never stored)
+  const int query = r / a.group, member = r - query * a.group;
   k.lim = sight.limit(query);
   k.lo = sight.lower(query);
-  k.row = rows.first + query;
-  const int64_t at = k.row * a.q_stride + (head * a.group + k.member) * static_cast<int64_t>(D);
-  float x[P][8], amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < P; ++i) {
-    load8_f32<KIND>(a.q, at + 32 * (i >> 1) + 16 * half + 8 * (i & 1), x[i]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[i][j]));
-  }
+  const int64_t at = (rows.first + query) * a.q_stride + (head * a.group + member) * static_cast<int64_t>(D);
+  auto dims = [&](int i) { return at + 32 * (i >> 1) + 16 * half + 8 * (i & 1); };
+  float x[8];
   int e = 0;
-  if constexpr (KIND == KIND_BF16) {
+  if constexpr (KIND == KIND_BF16) {   // read twice, the second time from L1: kept, the row would be D registers
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      load8_f32<KIND>(a.q, dims(i), x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
+    }
     amax = fmaxf(amax, other_half(amax));
     e = max(static_cast<int>(float_to_bits(amax) >> 23), 1) - 127;
+    asm volatile("" ::: "memory");
   }
   k.c = ldexpf(1.0f, e) * a.scale;
 #pragma unroll
   for (int i = 0; i < P; ++i) {
+    load8_f32<KIND>(a.q, dims(i), x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) k.q[i][j] = static_cast<_Float16>(KIND == KIND_BF16 ? ldexpf(x[i][j], -e) : x[i][j]);
+    for (int j = 0; j < 8; ++j) k.q[i][j] = static_cast<_Float16>(KIND == KIND_BF16 ? ldexpf(x[j], -e) : x[j]);
     // (keeps the conversion in front of the loop: the compiler sinks it into the loop otherwise, 97 instructions a block)
     asm volatile("" : "+v"(k.q[i]));
   }
@@ -254,13 +256,13 @@ __device__ __forceinline__ float opaque_one() {
 
 // A column's result: to the output, or with splits to the workspace.
 template <int D, int KIND>
-__device__ __forceinline__ void store_column(const AttnArgs& a, const Column<D>& k, int head, int split, float m, float l,
-                                             const f16v (&acc)[D / 32]) {
-  if (!k.valid) return;
-  const int half = (threadIdx.x & 63) >> 5;
-  const int64_t q_head = head * a.group + k.member;
+__device__ __forceinline__ void store_column(const AttnArgs& a, const SeqRows& rows, int r, int n_rows, int head, int split,
+                                             float m, float l, const f16v (&acc)[D / 32]) {
+  if (r >= n_rows) return;
+  const int half = (threadIdx.x & 63) >> 5, query = r / a.group;
+  const int64_t q_head = head * a.group + (r - query * a.group), row = rows.first + query;
   if (a.splits > 1) {
-    const int64_t at = (static_cast<int64_t>(split) * a.tokens + k.row) * a.q_heads + q_head;
+    const int64_t at = (static_cast<int64_t>(split) * a.tokens + row) * a.q_heads + q_head;
     if (half == 0) {
       a.part_ml[2 * at] = m;
       a.part_ml[2 * at + 1] = l;
@@ -273,8 +275,8 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const Column<D>&
             make_float4(acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]);
     return;
   }
-  const float r = l == 0.0f ? 0.0f : 1.0f / l;   // a row that saw no key gives zeros
-  uint16_t* out = static_cast<uint16_t*>(a.out) + k.row * a.out_stride + q_head * D + 4 * half;
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;   // a row that saw no key gives zeros
+  uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_stride + q_head * D + 4 * half;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -282,7 +284,7 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const Column<D>&
       uint32_t w[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        w[b] = half_bits<KIND>(acc[t][i + 2 * b] * r) | (half_bits<KIND>(acc[t][i + 2 * b + 1] * r) << 16);
+        w[b] = half_bits<KIND>(acc[t][i + 2 * b] * f) | (half_bits<KIND>(acc[t][i + 2 * b + 1] * f) << 16);
       __builtin_memcpy(__builtin_assume_aligned(out + 32 * t + 2 * i, 2), w, 8);
     }
 }
@@ -391,28 +393,30 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
       __syncthreads();
     }
   }
-  if (wave == 0) store_column<D, KIND>(a, k, head, split, m, l, acc);
+  if (wave == 0) store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, split, m, l, acc);
 }
 
 // ---- many rows: the waves of a workgroup have 32 rows each and walk over the keys together --------------------------
 // grid (KV heads, row tiles, batch * splits): heads in front, so that with 8 of them each XCD keeps one head's cache in
 // its L2; the tiles of the latest queries, which see the most keys, start first.
 //
-// Converting a block to fp16 costs a wave as much as its matrix products (packed fp16 subtractions run at half rate), so
+// Converting a block to fp16 costs a wave more than its matrix products (packed fp16 subtractions run at half rate), so
 // the waves convert a block once, each its share, into LDS, in operand order: a lane reads its 16 bytes of every operand
-// at lane * 16.  Softmax and matrix products of one block depend on each other, so the products K Q^T of the next block run
-// behind the exponentials of this one: in step j a wave reads K of j + 1 and V of j, converts K of j + 2 and V of j + 1
-// into the buffers that step j - 1 read, and asks memory for K of j + 3 and V of j + 2.  One barrier a step.
-template <int D>
-struct RowShape {
-  static constexpr int WAVES = D <= 128 ? 8 : 4;       // heads of 256: 192 registers a wave for O and Q alone
-  static constexpr int TILE = 32 * WAVES;
-};
-
+// at lane * 16.  Two buffers and one barrier a step: at its end a wave converts its share of block j + 1 from registers
+// into the other buffer and asks memory for block j + 2.
+// There is no running maximum: P is taken against the reference as it is, and only where a column's sum says that P has
+// grown out of its range is the maximum looked for, the reference moved and P taken again.
+//
+// What bounds it: 8192 tokens, 40 / 8 heads of 128, 695 us: vector instructions 60 % and matrix instructions 45 % of the
+// cycles, at 2.1 GHz. Four waves, three such workgroups a CU, let one wave's softmax run in another's products.  Measured
+// and not taken: eight waves (half the conversions a wave, but two waves a SIMD) 735 us; products of the next block behind
+// the softmax of this one (250 registers, two waves a SIMD) 765 to 780 us; 64 rows a wave 1053 us; K and V converted by
+// every wave from registers 899 us; wave priorities around the products or the softmax, no difference.
 template <int D, int KIND>
-__global__ void __launch_bounds__(RowShape<D>::WAVES * 64, D <= 128 ? 2 : 1) attention_rows_kernel(AttnArgs a) {
-  constexpr int W = RowShape<D>::WAVES, TILE = RowShape<D>::TILE;
-  constexpr int KC = D / 32, PIECES = 2 * KC, MINE = PIECES > W ? PIECES / W : 1;   // operand pieces of K, and of V
+__global__ void __launch_bounds__(ROW_WAVES * 64, D <= 128 ? 3 : 2) attention_rows_kernel(AttnArgs a) {
+  constexpr int W = ROW_WAVES, TILE = 32 * W;
+  constexpr int KC = D / 32, PIECES = 2 * KC;          // operand pieces of K, and of V; a 16-byte load gives two of them
+  constexpr int LOADS = 2 * KC, MINE = LOADS / W;      // of a block: K's, then V's
   __shared__ h8 lds_k[2][PIECES][64];
   __shared__ h8 lds_v[2][PIECES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -441,144 +445,114 @@ __global__ void __launch_bounds__(RowShape<D>::WAVES * 64, D <= 128 ? 2 : 1) att
   const float one = opaque_one();
   Blocks blocks;
   blocks.step = 1;
-  // Of the blocks whose K was asked for last, last but one and so on: number, scales.
-  int64_t n_last = 0;
-  Scales s1{}, s2{}, s3{};
-  uint2 raw_k[MINE], raw_v[MINE];
-  auto piece_of = [&](int r) { return (wave + W * r) % PIECES; };     // (fewer pieces than waves: some convert the same one)
-  auto fetch_v = [&] {
-    const uint8_t* from = a.cache.v + n_last * (D * KV_BLOCK) + (lane & 31) * 32 + (lane >> 5) * 16;
-#pragma unroll
-    for (int r = 0; r < MINE; ++r) {
-      const int i = piece_of(r);
-      raw_v[r] = *reinterpret_cast<const uint2*>(from + (i >> 1) * 1024 + (i & 1) * 8);
-    }
-  };
-  auto fetch_k = [&](int which) {
+  Scales s1{}, s2{};               // of the two blocks that were asked for last
+  uint4 raw[MINE];
+  auto load_of = [&](int r) { return wave + W * r; };
+  auto fetch = [&](int which) {
     if (blocks.slot(which) >= 64) blocks.lookup(a.cache, seq, head, which, blk_end);
-    n_last = blocks.at(which);
     const int slot = blocks.slot(which);
+    const int64_t at = blocks.at(which) * (D * KV_BLOCK);
     s1 = s2;
-    s2 = s3;
-    s3 = Scales{read_lane_f(blocks.ks, slot), read_lane_f(blocks.lv, slot), read_lane_f(blocks.iv, slot), false};
-    const uint8_t* from = a.cache.k + n_last * (D * KV_BLOCK) + lane * 16;
+    s2 = Scales{read_lane_f(blocks.ks, slot), read_lane_f(blocks.lv, slot), read_lane_f(blocks.iv, slot), false};
 #pragma unroll
     for (int r = 0; r < MINE; ++r) {
-      const int i = piece_of(r);
-      raw_k[r] = *reinterpret_cast<const uint2*>(from + (i >> 1) * 1024 + (i & 1) * 8);
+      const int i = load_of(r);
+      const uint8_t* from = i < KC ? a.cache.k + at + i * 1024 + lane * 16
+                                   : a.cache.v + at + (i - KC) * 1024 + (lane & 31) * 32 + (lane >> 5) * 16;
+      raw[r] = *reinterpret_cast<const uint4*>(from);
     }
   };
-  auto convert_k = [&](int buffer) {
+  auto convert = [&](int buffer) {
 #pragma unroll
-    for (int r = 0; r < MINE; ++r) lds_k[buffer][piece_of(r)][lane] = bytes8_to_half(raw_k[r].x, raw_k[r].y);
+    for (int r = 0; r < MINE; ++r) {
+      const int i = load_of(r);
+      h8(*to)[64] = i < KC ? &lds_k[buffer][2 * i] : &lds_v[buffer][2 * (i - KC)];
+      to[0][lane] = bytes8_to_half(raw[r].x, raw[r].y);
+      to[1][lane] = bytes8_to_half(raw[r].z, raw[r].w);
+    }
   };
-  auto convert_v = [&](int buffer) {
-#pragma unroll
-    for (int r = 0; r < MINE; ++r) lds_v[buffer][piece_of(r)][lane] = bytes8_to_half(raw_v[r].x, raw_v[r].y);
-  };
-  // The softmax's constants of a block for this lane's column, and its raw products made ready: keys that the column does
-  // not see at -infinity (at 0 under a weight of 0 where it sees none: a block's NaN must not reach it).
   const int half = lane >> 5;
-  f16v s = f16v{0};
-  float c = 0.0f, shift = 0.0f, p_shift = 0.0f, iv = 0.0f;
-  bool far = false;
-  auto ready = [&](int j, const Scales& b) {
-    const int key0 = j * KV_BLOCK;
-    c = b.ks * k.c;
-    c = c < 1e-37f ? 1e-37f : c;                   // (a NaN stays)
-    float lv = b.lv;
-    bool none = false;
-    if (key0 + KV_BLOCK > lim_first || key0 < lo_last) {
-      none = key0 >= k.lim || key0 + KV_BLOCK <= k.lo;
-      c = none ? 0.0f : c;
-      lv = none ? -__builtin_inff() : lv;
+  // P of a block from its raw products s (see above), and what it adds to the sum.
+  auto weigh = [&](const f16v& s, float c, float shift, h8 (&p)[2]) {
+    float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
-        s[i] = key < k.lim && key >= k.lo ? s[i] : none ? 0.0f : -__builtin_inff();
-      }
+    for (int i = 0; i < 16; i += 2) {
+      const float w0 = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, shift));
+      const h2 r = __builtin_convertvector((f2v{w0, w1}), h2);
+      p[i >> 3][i & 7] = r.x;
+      p[i >> 3][(i & 7) + 1] = r.y;
+      // summed as rounded, subnormals too (the dot product instruction takes those as 0): v_fma_mix_f32 with a 1 that the
+      // compiler does not see through
+      sum = fmaf(static_cast<float>(r.x), one, sum);
+      sum = fmaf(static_cast<float>(r.y), one, sum);
     }
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-    top = fmaxf(top, other_half(top));
-    const float high = fmaf(top, c, lv);           // a NaN (a poisoned block) moves nothing
-    if (__any(high > m + HEADROOM)) {
-      const float to = fmaxf(m, high);
-      const float f = __builtin_amdgcn_exp2f(m - to);
-      m = to;
-      l *= f;
-#pragma unroll
-      for (int t = 0; t < KC; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[t][i] *= f;
-    }
-    lv_top = fmaxf(lv_top, b.lv);
-    far = b.lv < lv_top - 2.0f && b.lv > -__builtin_inff();
-    shift = lv - m + OFFSET;
-    p_shift = none ? -__builtin_inff() : OFFSET - m;
-    iv = far ? 0.0f : b.iv;
+    return sum;
   };
   if (blk < blk_end) {
     blocks.lookup(a.cache, seq, head, blk, blk_end);
-    fetch_k(blk);
-    fetch_v();
-    convert_k(0);
-    convert_v(0);
-    fetch_k(blk + 1);              // (behind the end: block 0's bytes under a weight of 0)
-    convert_k(1);
-    fetch_v();                     // of blk + 1
-    fetch_k(blk + 2);
-    lds_barrier();
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_k[0][i][lane], k.q[i], s, 0, 0, 0);
-    ready(blk, s1);
+    fetch(blk);
+    convert(0);
+    fetch(blk + 1);                // (behind the end: block 0's bytes, not worked on)
     for (int j = blk; j < blk_end; ++j) {
       const int here = (j - blk) & 1;
-      lds_barrier();               // K of j + 1 and V of j are in LDS, and nobody reads what step j - 1 did
-      if (far) {
-        // w may be lost in fp16 although p counts in the sum, which then takes p itself: 16 more exponentials.
-        float e = 0.0f;
+      lds_barrier();               // block j is in LDS, and nobody reads the other buffer any more
+      const Scales b = s1;
+      f16v s = f16v{0};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) e += __builtin_amdgcn_exp2f(fmaf(s[i], c, p_shift));
-        l += e;
+      for (int i = 0; i < PIECES; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_k[here][i][lane], k.q[i], s, 0, 0, 0);
+      const int key0 = j * KV_BLOCK;
+      float c = b.ks * k.c;
+      c = c < 1e-37f ? 1e-37f : c;   // (a NaN stays)
+      float lv = b.lv;
+      bool none = false;
+      if (key0 + KV_BLOCK > lim_first || key0 < lo_last) {
+        // Keys that the column does not see count as -infinity; where it sees none, everything as 0 under a weight of 0: a
+        // NaN scale must not reach it.
+        none = key0 >= k.lim || key0 + KV_BLOCK <= k.lo;
+        c = none ? 0.0f : c;
+        lv = none ? -__builtin_inff() : lv;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
+          s[i] = key < k.lim && key >= k.lo ? s[i] : none ? 0.0f : -__builtin_inff();
+        }
       }
-      h8 kf[PIECES], vf[PIECES];
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) kf[i] = lds_k[here ^ 1][i][lane];
-      f16v next = f16v{0};
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) next = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i], k.q[i], next, 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) vf[i] = lds_v[here][i][lane];
-      convert_k(here);
-      convert_v(here ^ 1);
-      // P of block j, summed as rounded, its subnormals too (the dot product instruction would take those as 0):
-      // v_fma_mix_f32 with a `one` that the compiler does not see through.
       h8 p[2];
-      float sum = 0.0f;
+      float sum = weigh(s, c, lv - m + OFFSET, p);
+      if (__any(sum > RANGE)) {
+        float top = s[0];
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float w0 = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c, shift));
-        const h2 r = __builtin_convertvector((f2v{w0, w1}), h2);
-        p[i >> 3][i & 7] = r.x;
-        p[i >> 3][(i & 7) + 1] = r.y;
-        sum = fmaf(static_cast<float>(r.x), one, sum);
-        sum = fmaf(static_cast<float>(r.y), one, sum);
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = fmaxf(top, other_half(top));
+        const float to = fmaxf(m, fmaf(top, c, lv)), f = __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int t = 0; t < KC; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][i] *= f;
+        sum = weigh(s, c, lv - m + OFFSET, p);
       }
-      l = fmaf(sum, iv, l);
+      lv_top = fmaxf(lv_top, b.lv);
+      if (b.lv < lv_top - 2.0f && b.lv > -__builtin_inff()) {
+        // V's scale is less than a quarter of the largest so far: w may be lost in fp16 although p counts in the sum, which
+        // then takes p itself, at the price of 16 more exponentials.
+        const float shift = none ? -__builtin_inff() : OFFSET - m;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(s[i], c, shift));
+      } else {
+        l = fmaf(sum, b.iv, l);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < KC; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[2 * t + h], p[h], acc[t], 0, 0, 0);
-      fetch_v();                   // of j + 2
-      fetch_k(j + 3);
-      s = next;
-      ready(j + 1, s1);
+        for (int t = 0; t < KC; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_v[here][2 * t + h][lane], p[h], acc[t], 0, 0, 0);
+      convert(here ^ 1);
+      fetch(j + 2);
     }
   }
   l += other_half(l);
-  store_column<D, KIND>(a, k, head, split, m, l, acc);
+  store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, split, m, l, acc);
 }
 
 // Joins the chunks of one output row: grid (rows a sequence, batch), one wave a row, D / 64 dims a lane.
@@ -644,16 +618,17 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   Plan p;
   const int64_t rows = max_q * (q_heads / kv_heads);
   p.keys = rows <= 64;
-  p.tile_rows = p.keys ? 32 : dim <= 128 ? RowShape<128>::TILE : RowShape<256>::TILE;
+  p.tile_rows = p.keys ? 32 : 32 * ROW_WAVES;
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // Keys that a tile can see.
   int64_t span = max_kv;
   if (window > 0 && window + max_q + 31 < span) span = window + max_q + 31;
   const int64_t blocks = (span + 31) / 32 + (window > 0 ? 1 : 0);
-  const int64_t groups = batch * kv_heads * p.tiles, want = p.keys ? 2 * CUS : CUS;
-  int64_t splits = (want + groups - 1) / groups;
-  const int64_t least = p.keys ? 16 : 32;               // blocks worth a workgroup of its own
-  const int64_t most = (blocks + least - 1) / least;
+  // Two workgroups a CU; with a workgroup a CU from the rows alone, prompts are not split (they would be joined for less
+  // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts). A part has at least 16 blocks.
+  const int64_t groups = batch * kv_heads * p.tiles;
+  int64_t splits = !p.keys && groups >= CUS ? 1 : (2 * CUS + groups - 1) / groups;
+  const int64_t most = (blocks + 15) / 16;
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   p.most_splits = static_cast<int>(splits);
@@ -680,7 +655,7 @@ template <int D, int KIND>
 int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64_t kv_heads, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.tiles), static_cast<unsigned>(batch * p.splits));
   if (p.keys) hipLaunchKernelGGL((attention_keys_kernel<D, KIND>), grid, dim3(WAVES * 64), 0, stream, a);
-  else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(RowShape<D>::WAVES * 64), 0, stream, a);
+  else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(ROW_WAVES * 64), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
   const dim3 join(static_cast<unsigned>((max_q * a.q_heads + 3) / 4), static_cast<unsigned>(batch));
