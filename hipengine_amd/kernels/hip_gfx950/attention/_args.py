@@ -11,6 +11,15 @@ KINDS = {"f32": KIND_F32, "bf16": KIND_BF16, "fp16": KIND_F16}
 HEAD_DIMS = frozenset({64, 128, 256})
 
 
+# The wrappers test their arguments in one expression and take the argument by argument checks below only where it fails,
+# for the message: a launch of a few microseconds is not to wait for its own checks.
+def are_pointers(*values: int | None) -> bool:
+    for value in values:
+        if type(value) is not int or value <= 0:
+            return False
+    return True
+
+
 def kind_of(name: str, argument: str, allowed: tuple[str, ...] = ("f32", "bf16", "fp16")) -> int:
     if name not in allowed:
         raise ValueError(f"{argument} must be one of {', '.join(allowed)}")

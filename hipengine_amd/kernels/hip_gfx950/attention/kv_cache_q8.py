@@ -16,14 +16,15 @@ included; :mod:`paged_attention_q8` takes the same arrays.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
 
 from hipengine_amd.core.hip import HipRuntime
 from hipengine_amd.kernels.hip_gfx950 import _launch
 from hipengine_amd.kernels.hip_gfx950._launch import I32, I64, VOID, check_launch, entry, validate_pointers
 from hipengine_amd.kernels.hip_gfx950.attention._args import (
     F32,
+    HEAD_DIMS,
     KINDS,
+    are_pointers,
     check_head_dim,
     check_positive,
     check_rotation,
@@ -33,6 +34,7 @@ from hipengine_amd.kernels.hip_gfx950.attention._args import (
 from hipengine_amd.kernels.registry import KernelKey, register
 
 BLOCK_TOKENS = 32
+_PAGE_SIZES = frozenset(1 << i for i in range(5, 21))
 
 _APPEND_ARGS = [VOID, VOID, I32, I64, I64, VOID, VOID, VOID, I64, I32, F32, F32] + [VOID] * 5 + [I64] + [VOID] * 2 + [I64] * 7 + [VOID]
 _READ_ARGS = [VOID] * 5 + [I64] + [VOID] * 4 + [I32] + [I64] * 8 + [VOID]
@@ -43,29 +45,25 @@ def v_place(token: int) -> int:
     return (token & 3) | ((token >> 3 & 3) << 2) | ((token >> 2 & 1) << 4)
 
 
-@dataclass(frozen=True)
 class KVCacheQ8:
-    """The buffers and sizes of one layer's cache."""
+    """The buffers and sizes of one layer's cache, checked once when it is made."""
 
-    k_ptr: int
-    v_ptr: int
-    k_scale_ptr: int
-    v_scale_ptr: int
-    pages: int
-    page_size: int
-    kv_heads: int
-    head_dim: int
+    __slots__ = ("k_ptr", "v_ptr", "k_scale_ptr", "v_scale_ptr", "pages", "page_size", "kv_heads", "head_dim")
 
-    def __post_init__(self) -> None:
-        check_positive(pages=self.pages, kv_heads=self.kv_heads)
-        if self.pages > 2**31 - 1 or self.kv_heads > 65535:
-            raise ValueError("pages must fit int32 page numbers and kv_heads be at most 65535")
-        if self.page_size < BLOCK_TOKENS or self.page_size > 1 << 20 or self.page_size & (self.page_size - 1):
-            raise ValueError("page_size must be a power of two, 32 .. 2^20")
-        check_head_dim(self.head_dim)
-        validate_pointers(k_ptr=self.k_ptr, v_ptr=self.v_ptr, k_scale_ptr=self.k_scale_ptr, v_scale_ptr=self.v_scale_ptr)
-        if (self.k_ptr | self.v_ptr) & 15:
+    def __init__(self, k_ptr: int, v_ptr: int, k_scale_ptr: int, v_scale_ptr: int, pages: int, page_size: int,
+                 kv_heads: int, head_dim: int) -> None:
+        if not (0 < pages < 1 << 31 and 0 < kv_heads <= 65535 and page_size in _PAGE_SIZES and head_dim in HEAD_DIMS
+                and are_pointers(k_ptr, v_ptr, k_scale_ptr, v_scale_ptr) and (k_ptr | v_ptr) & 15 == 0):
+            check_positive(pages=pages, kv_heads=kv_heads)
+            if pages > 2**31 - 1 or kv_heads > 65535:
+                raise ValueError("pages must fit int32 page numbers and kv_heads be at most 65535")
+            if page_size not in _PAGE_SIZES:
+                raise ValueError("page_size must be a power of two, 32 .. 2^20")
+            check_head_dim(head_dim)
+            validate_pointers(k_ptr=k_ptr, v_ptr=v_ptr, k_scale_ptr=k_scale_ptr, v_scale_ptr=v_scale_ptr)
             raise ValueError("k_ptr and v_ptr must be 16-byte aligned")
+        self.k_ptr, self.v_ptr, self.k_scale_ptr, self.v_scale_ptr = k_ptr, v_ptr, k_scale_ptr, v_scale_ptr
+        self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
 
     @staticmethod
     def value_bytes(pages: int, page_size: int, kv_heads: int, head_dim: int) -> int:
@@ -91,12 +89,17 @@ def kv_append_q8(cache: KVCacheQ8, k_ptr: int, v_ptr: int, page_table_ptr: int, 
     earlier tokens are rescaled then; a block whose first token is appended starts anew; bytes behind the new tokens
     stay. A NaN or infinity makes its block's scale NaN until the block starts anew. No two sequences may append to the
     same block in one call."""
-    if _launch.VALIDATE:
+    width = cache.kv_heads * cache.head_dim
+    if _launch.VALIDATE and not (
+            tokens > 0 and batch > 0 and max_q_len > 0 and table_stride > 0 and in_kind in KINDS and eps >= 0.0
+            and (k_stride == 0 or k_stride >= width) and (v_stride == 0 or v_stride >= width)
+            and (16 <= rotary_dim <= cache.head_dim and rotary_dim & 15 == 0 if inv_freq_ptr else rotary_dim == 0)
+            and are_pointers(k_ptr, v_ptr, page_table_ptr, q_start_ptr, kv_lens_ptr)):
         check_positive(tokens=tokens, batch=batch, max_q_len=max_q_len, table_stride=table_stride)
         kind_of(in_kind, "in_kind")
         check_rotation(inv_freq_ptr, rotary_dim, cache.head_dim)
-        check_stride("k_stride", k_stride, cache.kv_heads * cache.head_dim)
-        check_stride("v_stride", v_stride, cache.kv_heads * cache.head_dim)
+        check_stride("k_stride", k_stride, width)
+        check_stride("v_stride", v_stride, width)
         if not eps >= 0.0:
             raise ValueError("eps must not be negative")
         validate_pointers(k_ptr=k_ptr, v_ptr=v_ptr, page_table_ptr=page_table_ptr, q_start_ptr=q_start_ptr,
@@ -115,11 +118,15 @@ def kv_read_q8(cache: KVCacheQ8, k_out_ptr: int | None, v_out_ptr: int | None, p
     """Read the last ``row_start[b + 1] - row_start[b]`` cached tokens of every sequence b into rows ``row_start[b]`` ..
     of the outputs ``[tokens, kv_heads, head_dim]``. One of the outputs may be None. Tokens on a page that is not in the
     cache read as zeros."""
-    if _launch.VALIDATE:
+    width = cache.kv_heads * cache.head_dim
+    if _launch.VALIDATE and not (
+            tokens > 0 and batch > 0 and table_stride > 0 and out_kind in KINDS and (k_out_ptr or v_out_ptr)
+            and (k_out_stride == 0 or k_out_stride >= width) and (v_out_stride == 0 or v_out_stride >= width)
+            and are_pointers(page_table_ptr, row_start_ptr, kv_lens_ptr)):
         check_positive(tokens=tokens, batch=batch, table_stride=table_stride)
         kind_of(out_kind, "out_kind")
-        check_stride("k_out_stride", k_out_stride, cache.kv_heads * cache.head_dim)
-        check_stride("v_out_stride", v_out_stride, cache.kv_heads * cache.head_dim)
+        check_stride("k_out_stride", k_out_stride, width)
+        check_stride("v_out_stride", v_out_stride, width)
         if not k_out_ptr and not v_out_ptr:
             raise ValueError("k_out_ptr or v_out_ptr must be a non-null device pointer")
         validate_pointers(page_table_ptr=page_table_ptr, row_start_ptr=row_start_ptr, kv_lens_ptr=kv_lens_ptr)

@@ -8,12 +8,21 @@ places up to its own, with ``window > 0`` the last ``window`` of them. A query t
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 from hipengine_amd.core.hip import HipRuntime
 from hipengine_amd.kernels.hip_gfx950 import _launch
 from hipengine_amd.kernels.hip_gfx950._launch import I32, I64, VOID, check_launch, entry, validate_pointers
-from hipengine_amd.kernels.hip_gfx950.attention._args import F32, KINDS, check_head_dim, check_positive, check_stride, kind_of
+from hipengine_amd.kernels.hip_gfx950.attention._args import (
+    F32,
+    KINDS,
+    are_pointers,
+    check_head_dim,
+    check_positive,
+    check_stride,
+    kind_of,
+)
 from hipengine_amd.kernels.hip_gfx950.attention.kv_cache_q8 import KVCacheQ8
 from hipengine_amd.kernels.registry import KernelKey, register
 
@@ -35,11 +44,24 @@ def _check_shape(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_hea
 def paged_attention_q8_workspace_bytes(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int,
                                        kv_heads: int, head_dim: int, *, library: ctypes.CDLL | None = None) -> int:
     """Bytes of scratch that a call of these sizes needs, whatever its window; 0 where it needs none."""
+    if library is not None:
+        return _workspace_bytes(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim, library)
+    return _default_workspace_bytes(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim)
+
+
+def _workspace_bytes(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int,
+                     library: ctypes.CDLL | None) -> int:
     _check_shape(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim)
     out = I64(0)
     check_launch(entry("hipengine_gfx950_paged_attention_q8_workspace_bytes", _WORKSPACE_ARGS, library)(
         tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim, ctypes.byref(out)), None)
     return int(out.value)
+
+
+@functools.lru_cache(maxsize=64)   # a function of the sizes alone, asked for at every step of a decode loop
+def _default_workspace_bytes(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int, kv_heads: int,
+                             head_dim: int) -> int:
+    return _workspace_bytes(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim, None)
 
 
 def paged_attention_q8(cache: KVCacheQ8, q_ptr: int, out_ptr: int, page_table_ptr: int, table_stride: int,
@@ -51,16 +73,23 @@ def paged_attention_q8(cache: KVCacheQ8, q_ptr: int, out_ptr: int, page_table_pt
     """q and out ``[tokens, q_heads, head_dim]`` (bf16 or fp16 bits, both of one kind). ``max_q_len`` and ``max_kv_len``
     are at least the longest sequence's; ``scale`` defaults to ``head_dim ** -0.5``. The workspace (16-byte aligned) is
     scratch of the size ``paged_attention_q8_workspace_bytes`` gives; calls that overlap in time need one each."""
-    if _launch.VALIDATE:
-        _check_shape(tokens, batch, max_q_len, max_kv_len, q_heads, cache.kv_heads, cache.head_dim)
+    kv_heads, head_dim = cache.kv_heads, cache.head_dim
+    width = q_heads * head_dim
+    if _launch.VALIDATE and not (
+            0 < tokens <= 1 << 26 and 0 < batch <= 65535 and max_q_len > 0 and 0 <= max_kv_len <= 1 << 30
+            and 0 < q_heads <= 4096 and q_heads % kv_heads == 0 and table_stride > 0 and (kind == "bf16" or kind == "fp16")
+            and (scale is None or 0.0 < scale < math.inf) and 0 <= window <= 1 << 30
+            and (q_stride == 0 or q_stride >= width) and (out_stride == 0 or out_stride >= width) and q_ptr != out_ptr
+            and are_pointers(q_ptr, out_ptr, page_table_ptr, q_start_ptr, kv_lens_ptr)):
+        _check_shape(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim)
         check_positive(table_stride=table_stride)
         kind_of(kind, "kind", ("bf16", "fp16"))
         if scale is not None and not 0.0 < scale < math.inf:
             raise ValueError("scale must be positive and finite")
         if window < 0 or window > 1 << 30:
             raise ValueError("window must be 0 (none) .. 2^30")
-        check_stride("q_stride", q_stride, q_heads * cache.head_dim)
-        check_stride("out_stride", out_stride, q_heads * cache.head_dim)
+        check_stride("q_stride", q_stride, width)
+        check_stride("out_stride", out_stride, width)
         validate_pointers(q_ptr=q_ptr, out_ptr=out_ptr, page_table_ptr=page_table_ptr, q_start_ptr=q_start_ptr,
                           kv_lens_ptr=kv_lens_ptr)
         if q_ptr == out_ptr:
@@ -68,7 +97,7 @@ def paged_attention_q8(cache: KVCacheQ8, q_ptr: int, out_ptr: int, page_table_pt
     check_launch(entry("hipengine_gfx950_paged_attention_q8", _ARGS, library)(
         q_ptr, out_ptr, KINDS[kind], q_stride, out_stride, cache.k_ptr, cache.v_ptr, cache.k_scale_ptr, cache.v_scale_ptr,
         page_table_ptr, table_stride, q_start_ptr, kv_lens_ptr, tokens, batch, max_q_len, max_kv_len, q_heads,
-        cache.kv_heads, cache.head_dim, cache.pages, cache.page_size, cache.head_dim ** -0.5 if scale is None else scale,
+        kv_heads, head_dim, cache.pages, cache.page_size, head_dim ** -0.5 if scale is None else scale,
         window, workspace_ptr, workspace_bytes, stream), runtime)
 
 

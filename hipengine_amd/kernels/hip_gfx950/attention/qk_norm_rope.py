@@ -15,7 +15,9 @@ from hipengine_amd.kernels.hip_gfx950 import _launch
 from hipengine_amd.kernels.hip_gfx950._launch import I32, I64, VOID, check_launch, entry, validate_pointers
 from hipengine_amd.kernels.hip_gfx950.attention._args import (
     F32,
+    HEAD_DIMS,
     KINDS,
+    are_pointers,
     check_head_dim,
     check_positive,
     check_rotation,
@@ -38,7 +40,16 @@ def qk_norm_rope(q_ptr: int | None, k_ptr: int | None, q_out_ptr: int | None, k_
     the norm, a null ``inv_freq_ptr`` the rotation, 0 heads one of the two tensors. Strides count elements from one
     token to the next (0: packed), so q and k may be columns of one projection's output. An output may be its input
     where kind and stride agree."""
-    if _launch.VALIDATE:
+    q_width, k_width = q_heads * head_dim, kv_heads * head_dim
+    if _launch.VALIDATE and not (
+            0 < tokens <= 4194303 and 0 <= q_heads <= 4096 and 0 <= kv_heads <= 4096 and q_heads + kv_heads > 0
+            and head_dim in HEAD_DIMS and in_kind in KINDS and out_kind in KINDS and eps >= 0.0
+            and (16 <= rotary_dim <= head_dim and rotary_dim & 15 == 0 and are_pointers(positions_ptr) if inv_freq_ptr
+                 else rotary_dim == 0)
+            and (q_heads == 0 or are_pointers(q_ptr, q_out_ptr)) and (kv_heads == 0 or are_pointers(k_ptr, k_out_ptr))
+            and (q_stride == 0 or q_stride >= q_width) and (q_out_stride == 0 or q_out_stride >= q_width)
+            and (k_stride == 0 or k_stride >= k_width) and (k_out_stride == 0 or k_out_stride >= k_width)
+            and (q_heads == 0 or q_ptr != q_out_ptr) and (kv_heads == 0 or k_ptr != k_out_ptr)):
         check_positive(tokens=tokens)
         if tokens > 4194303:
             raise ValueError("tokens must be at most 4194303")

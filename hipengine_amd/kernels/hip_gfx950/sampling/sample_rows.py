@@ -9,6 +9,7 @@ is the first one, by index, up to which the kept weights sum to more than ``unif
 from __future__ import annotations
 
 import ctypes
+import functools
 
 from hipengine_amd.core.hip import HipRuntime
 from hipengine_amd.kernels.hip_gfx950 import _launch
@@ -30,11 +31,20 @@ def _check_shape(rows: int, vocab_size: int) -> None:
 
 def sample_workspace_bytes(rows: int, vocab_size: int, *, library: ctypes.CDLL | None = None) -> int:
     """Bytes of scratch that a call of these sizes needs."""
+    return _default_workspace_bytes(rows, vocab_size) if library is None else _workspace_bytes(rows, vocab_size, library)
+
+
+def _workspace_bytes(rows: int, vocab_size: int, library: ctypes.CDLL | None) -> int:
     _check_shape(rows, vocab_size)
     out = I64(0)
     check_launch(entry("hipengine_gfx950_sample_f32_rows_i32_workspace_bytes", _WORKSPACE_ARGS, library)(
         rows, vocab_size, ctypes.byref(out)), None)
     return int(out.value)
+
+
+@functools.lru_cache(maxsize=64)   # a function of the sizes alone, asked for at every step of a decode loop
+def _default_workspace_bytes(rows: int, vocab_size: int) -> int:
+    return _workspace_bytes(rows, vocab_size, None)
 
 
 def sample_f32_rows_i32(logits_ptr: int, uniform_ptr: int, out_ids_ptr: int, rows: int, vocab_size: int, *,
