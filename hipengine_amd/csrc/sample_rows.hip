@@ -31,8 +31,11 @@ constexpr int THREADS = 256;
 constexpr int LAST = 1024;               // threads of pass 4
 constexpr int BINS = 512;
 constexpr int LIST = 16384;
+constexpr int FEW = 128;
 constexpr int64_t MAX_VOCAB = 1 << 22;   // 1024 chunks; 2^22 weights of 2^40 stay under 2^63
 constexpr int MAX_CHUNKS = static_cast<int>(MAX_VOCAB / CHUNK);
+
+struct Cut;
 
 struct Args {
   const float* logits;
@@ -49,6 +52,7 @@ struct Args {
   // workspace
   uint64_t* best;             // [rows][chunks] key << 32 | ~index of the chunk's first token in the order
   uint64_t* sums;             // [rows][chunks]
+  Cut* cuts;                  // [rows]
   uint64_t* bin_weight;       // [rows][BINS]
   uint64_t* list;             // [rows][cap] key << 32 | ~index
   uint32_t* bin_count;        // [rows][BINS]
@@ -138,14 +142,6 @@ __device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* lds) {
   return v;
 }
 
-__device__ __forceinline__ uint64_t row_best(const Args& a, int64_t row, int threads, uint64_t* lds) {
-  uint64_t v = 0;
-  for (int c = threadIdx.x; c < a.chunks; c += threads) {
-    const uint64_t o = a.best[row * a.chunks + c];
-    v = o > v ? o : v;
-  }
-  return threads == LAST ? block_max<LAST>(v, lds) : block_max<THREADS>(v, lds);
-}
 
 // A thread's 16 logits of a chunk: groups of 4 at (g * 256 + thread) * 4.  Behind the row's end: NaN.
 __device__ __forceinline__ int chunk_index(int chunk, int i) {
@@ -196,9 +192,16 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
   const int chunk = blockIdx.x;
   float l[16];
   load_chunk(a, row, chunk, l);
-  const uint64_t best = row_best(a, row, THREADS, lds);
+  uint64_t best = 0;
+  for (int c = threadIdx.x; c < a.chunks; c += THREADS) {
+    const uint64_t o = a.best[row * a.chunks + c];
+    best = o > best ? o : best;
+  }
+  best = block_max<THREADS>(best, lds);
   const Row r = row_of(a, row, logit_of(best));
   if (best == 0 || r.greedy || !cuts(r)) return;
+  // With top-k the border is found by counting, else by weight: one atomic a token.
+  const bool count = r.k > 0;
   for (int i = threadIdx.x; i < BINS; i += THREADS) { weights[i] = 0; counts[i] = 0; }
   __syncthreads();
 #pragma unroll
@@ -206,37 +209,53 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
     const uint64_t o = order_of(l[i], 0);
     if (o == 0) continue;
     const double y = depth(r, logit_of(o));
-    const int b = bin_of(y);
-    atomicAdd(&counts[b], 1u);
-    if (b < BINS - 1) atomicAdd(&weights[b], static_cast<unsigned long long>(weight(y)));   // the last bin's are 0
+    if (count) {
+      atomicAdd(&counts[bin_of(y)], 1u);
+    } else {
+      const uint64_t w = weight(y);
+      if (w) atomicAdd(&weights[bin_of(y)], static_cast<unsigned long long>(w));
+    }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < BINS; i += THREADS) {
-    if (counts[i] == 0) continue;
-    atomicAdd(&a.bin_count[row * BINS + i], counts[i]);
+    if (counts[i]) atomicAdd(&a.bin_count[row * BINS + i], counts[i]);
     if (weights[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.bin_weight[row * BINS + i]), weights[i]);
   }
 }
 
 enum Mode : int { ALL, BOUND, PREFIX, FULL };
 
-// What passes 3 and 4 know from the histogram.
+// What is known of a row before pass 3.
 struct Cut {
-  int mode;
-  int bin;              // B
+  uint64_t best;        // the first token in the order; 0: there is none
   uint64_t above;       // weight of the bins before B (BOUND)
   uint64_t need;        // top-p: a token stays if less than this lies before it (BOUND)
+  int mode;
+  int bin;              // B
+  int reached;          // whether `need` is reached within B (else min-p's border is there)
 };
 
 __device__ __forceinline__ uint64_t border(double p, uint64_t total) {   // smallest whole number >= p * total
   return static_cast<uint64_t>(ceil(p * static_cast<double>(total)));
 }
 
-// By the first 64 threads, 8 bins each, then told to all.
-__device__ __forceinline__ Cut find_cut(const Args& a, int64_t row, const Row& r, Cut* told) {
-  if (!cuts(r)) return {ALL, BINS, 0, 0};
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
+// Between passes 2 and 3: one wave a row, 8 bins a lane.
+__global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  uint64_t best = 0;
+  for (int c = lane; c < a.chunks; c += 64) {
+    const uint64_t o = a.best[row * a.chunks + c];
+    best = o > best ? o : best;
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(best), off);
+    best = o > best ? o : best;
+  }
+  const Row r = row_of(a, row, logit_of(best));
+  Cut cut{best, 0, 0, ALL, BINS, 0};
+  if (best != 0 && !r.greedy && cuts(r)) {
     uint64_t w[8], ws = 0;
     uint32_t c[8], cs = 0;
 #pragma unroll
@@ -266,63 +285,66 @@ __device__ __forceinline__ Cut find_cut(const Args& a, int64_t row, const Row& r
       wp += w[i];
       cp += c[i];
       if (r.k > 0 && cp >= static_cast<uint32_t>(r.k)) k_bin = min(k_bin, lane * 8 + i);
-      if (wp >= need) p_bin = min(p_bin, lane * 8 + i);
+      if (r.k == 0 && wp >= need) p_bin = min(p_bin, lane * 8 + i);
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       k_bin = min(k_bin, __shfl_xor(k_bin, off));
       p_bin = min(p_bin, __shfl_xor(p_bin, off));
     }
-    Cut cut;
     cut.need = need;
-    cut.above = 0;
-    // A border in the last bin cuts nothing: its weights are 0.
-    const bool by_k = k_bin < BINS - 1;
-    cut.bin = by_k ? k_bin : min(p_bin, min_bin);
-    // Tokens and weight before and in the bin.
-    uint64_t in_w = 0;
-    uint32_t in_c = 0, to_c = 0;
-    wp = wi - ws;
-    cp = ci - cs;
+    cut.reached = p_bin <= min_bin;
+    if (r.k > 0) {
+      // A border in the last bin cuts nothing (its weights are 0); what top-p and min-p then cut is not known by weight.
+      cut.bin = k_bin;
+      uint32_t to = ci - cs, up_to = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (lane * 8 + i == cut.bin) { in_w = wp; in_c = c[i]; to_c = cp + c[i]; }
-      wp += w[i];
-      cp += c[i];
+      for (int i = 0; i < 8; ++i) {
+        to += c[i];
+        if (lane * 8 + i == k_bin) up_to = to;
+      }
+      up_to = __shfl(up_to, k_bin >> 3);
+      if (k_bin < BINS - 1) cut.mode = up_to <= static_cast<uint32_t>(a.cap) ? PREFIX : FULL;
+      else cut.mode = r.p < 1.0 || r.octaves < __builtin_inf() ? FULL : ALL;
+    } else {
+      cut.bin = min(p_bin, min_bin);
+      uint64_t before = 0;
+      wp = wi - ws;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (lane * 8 + i == cut.bin) before = wp;
+        wp += w[i];
+      }
+      cut.above = __shfl(static_cast<unsigned long long>(before), cut.bin >> 3);
+      cut.mode = cut.bin < BINS - 1 ? BOUND : ALL;
     }
-    const int owner = cut.bin >> 3;
-    cut.above = __shfl(static_cast<unsigned long long>(in_w), owner);
-    const uint32_t in_bin = __shfl(in_c, owner), up_to = __shfl(to_c, owner);
-    if (by_k) cut.mode = up_to <= static_cast<uint32_t>(a.cap) ? PREFIX : FULL;
-    else if (cut.bin == BINS - 1) { cut.mode = ALL; cut.bin = BINS; }
-    else cut.mode = in_bin <= static_cast<uint32_t>(a.cap) ? BOUND : FULL;
-    if (lane == 0) *told = cut;
+    if (cut.mode == ALL) cut.bin = BINS;
   }
-  __syncthreads();
-  return *told;
+  if (lane == 0) a.cuts[row] = cut;
 }
 
 // Pass 3.
 __global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
   __shared__ uint64_t lds[THREADS / 64];
-  __shared__ Cut told;
   __shared__ uint32_t here, base;
   const int64_t row = blockIdx.y;
   const int chunk = blockIdx.x;
   float l[16];
   load_chunk(a, row, chunk, l);
-  const uint64_t best = row_best(a, row, THREADS, lds);
-  const Row r = row_of(a, row, logit_of(best));
-  if (best == 0 || r.greedy) return;
+  const Cut cut = a.cuts[row];
+  const Row r = row_of(a, row, logit_of(cut.best));
+  if (cut.best == 0 || r.greedy || cut.mode == FULL) return;
   if (threadIdx.x == 0) here = 0;
-  const Cut cut = find_cut(a, row, r, &told);
-  if (cut.mode == FULL) return;
-  __syncthreads();                                  // `here` is 0 for everyone, also where find_cut returned at once
+  __syncthreads();
+  // A logit that lies more than half a bin behind B's end is passed over by one comparison.
+  const float floor = cut.bin < BINS - 1 ? static_cast<float>(static_cast<double>(r.top) - (cut.bin + 1.5) * 0.125 / r.per)
+                                         : -__builtin_inff();
   uint64_t sum = 0;
   uint32_t slot[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     slot[i] = ~0u;
+    if (!(l[i] >= floor)) continue;
     const uint64_t o = order_of(l[i], 0);
     if (o == 0) continue;
     const double y = depth(r, logit_of(o));
@@ -350,6 +372,7 @@ struct Digits {
   uint32_t counts[256];
   uint64_t before;       // found: weight (or count) of the buckets before the one
   uint64_t in;           // found: tokens in it
+  unsigned long long some, all;
   int digit;
 };
 
@@ -367,22 +390,41 @@ struct Tokens {
   }
 };
 
-// Walks down a 64-bit number digit by digit (8 bits, from `bits` on) to the token at which a running sum first exceeds
-// `before` (the sum up to and including it is more than that).  value(order): the number, larger is earlier.  add(order):
-// what the token adds (0: not among them).  Counts or weights: any whole numbers.  Returns the number; ends early where
-// one token is left in the bucket.
+// Walks down a number digit by digit (8 bits) to the token at which a running sum first exceeds `before` (the sum up to and
+// including it is more than that).  value(order): the number, larger is earlier, no two tokens' the same.  add(order): what
+// the token adds (0: not among them).  Counts or weights: any whole numbers.  Returns the number.  Leading bits that all
+// tokens have in common are passed over, and it ends early where one token is left.
 template <typename V, typename A>
-__device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, int bits, uint64_t before, V value, A add) {
-  uint64_t prefix = 0;
-  for (int shift = bits - 8; shift >= 0; shift -= 8) {
+__device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t before, V value, A add) {
+  uint64_t some = 0, all = ~uint64_t{0};
+  t.each([&](uint64_t o) {
+    const uint64_t v = value(o);
+    some |= v;
+    all &= v;
+  });
+  if (threadIdx.x == 0) { d.some = 0; d.all = ~0ull; }
+  __syncthreads();
+  if (all != ~uint64_t{0} || some != 0) {
+    atomicOr(&d.some, static_cast<unsigned long long>(some));
+    atomicAnd(&d.all, static_cast<unsigned long long>(all));
+  }
+  __syncthreads();
+  some = d.some;
+  const uint64_t differ = some & ~d.all;
+  int high = differ ? 64 - __builtin_clzll(differ) : 0;       // bits still to be found
+  uint64_t prefix = high < 64 ? some >> high : 0;
+  while (high > 0) {
+    const int low = high > 8 ? high - 8 : 0;
+    const uint64_t mask = (1u << (high - low)) - 1;
+    __syncthreads();
     for (int i = threadIdx.x; i < 256; i += LAST) { d.weights[i] = 0; d.counts[i] = 0; }
     __syncthreads();
     t.each([&](uint64_t o) {
       const uint64_t v = value(o);
-      if (shift + 8 < 64 && (v >> (shift + 8)) != prefix) return;
+      if (high < 64 && (v >> high) != prefix) return;
       const uint64_t w = add(o);
       if (w == 0) return;
-      const int digit = static_cast<int>(v >> shift) & 255;
+      const int digit = static_cast<int>((v >> low) & mask);
       atomicAdd(&d.weights[digit], static_cast<unsigned long long>(w));
       atomicAdd(&d.counts[digit], 1u);
     });
@@ -410,35 +452,107 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, int bits, u
       }
     }
     __syncthreads();
-    prefix = (prefix << 8) | static_cast<uint64_t>(d.digit);
+    prefix = (prefix << (high - low)) | static_cast<uint64_t>(d.digit);
     before -= d.before;
-    const uint64_t in = d.in;
-    __syncthreads();
-    if (in == 1 && shift > 0) {     // its remaining digits
-      if (threadIdx.x == 0) d.before = 0;
+    high = low;
+    if (d.in == 1 && high > 0) {     // the one token's remaining digits
       __syncthreads();
       t.each([&](uint64_t o) {
         const uint64_t v = value(o);
-        if ((v >> shift) == prefix && add(o)) d.before = v;
+        if ((v >> high) == prefix && add(o)) d.before = v;
       });
       __syncthreads();
       prefix = d.before;
-      __syncthreads();
-      return prefix;
+      high = 0;
     }
   }
+  __syncthreads();                   // `d` may be used again
   return prefix;
+}
+
+__device__ __forceinline__ void answer(const Args& a, int64_t row, const Row& r, const float* logits, int id, uint64_t total) {
+  a.ids[row] = id;
+  if (!a.logprobs) return;
+  const float l = fminf(logits[id] + 0.0f, 3.4028234663852886e+38f);
+  a.logprobs[row] = static_cast<float>(-((static_cast<double>(r.top) - static_cast<double>(l)) * r.per +
+                                         log2(static_cast<double>(total)) - 40.0) * 0.6931471805599453);
+}
+
+__device__ __forceinline__ uint64_t target_of(const Args& a, int64_t row, uint64_t total) {
+  const float u = a.uniform[row];
+  const uint64_t target = static_cast<uint64_t>((u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0) * static_cast<double>(total));
+  return target < total ? target : total - 1;      // the largest weight is 2^40, so there is a total
+}
+
+// Top-k has left a list of at most 128 tokens: each is compared with every other one, 8 threads a token.
+struct Few {
+  uint64_t order[FEW], weight[FEW];
+  unsigned long long before[FEW], by_index[FEW];    // weight of the tokens earlier in the order; of the kept ones of lower index
+  uint32_t rank[FEW];
+  unsigned long long total, kept;
+};
+
+__device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const Row& r, const uint64_t* list, int n,
+                                              const float* logits, Few& f) {
+  const int i = threadIdx.x % FEW, part = threadIdx.x / FEW;
+  const bool mine = i < n;
+  uint64_t order = 0, w = 0;
+  double y = 0.0;
+  if (mine) {
+    order = list[i];
+    y = depth(r, logit_of(order));
+    w = weight(y);
+  }
+  if (part == 0) {
+    f.order[i] = order;
+    f.weight[i] = w;
+    f.before[i] = f.by_index[i] = 0;
+    f.rank[i] = 0;
+    if (i == 0) f.total = f.kept = 0;
+  }
+  __syncthreads();
+  uint32_t rank = 0;
+  uint64_t before = 0;
+  for (int j = part; j < n; j += LAST / FEW) {
+    const bool earlier = f.order[j] > order;
+    rank += earlier ? 1 : 0;
+    before += earlier ? f.weight[j] : 0;
+  }
+  if (mine && rank) {
+    atomicAdd(&f.rank[i], rank);
+    atomicAdd(&f.before[i], static_cast<unsigned long long>(before));
+  }
+  __syncthreads();
+  bool keep = mine && f.rank[i] < static_cast<uint32_t>(r.k);
+  if (part == 0 && keep) atomicAdd(&f.total, static_cast<unsigned long long>(w));
+  __syncthreads();
+  const uint64_t need = r.p < 1.0 ? border(r.p, f.total) : ~uint64_t{0};
+  keep = keep && (f.before[i] < need || f.rank[i] == 0) && y <= r.octaves;
+  __syncthreads();
+  if (part == 0) {
+    if (!keep) f.weight[i] = 0;
+    else atomicAdd(&f.kept, static_cast<unsigned long long>(w));
+  }
+  __syncthreads();
+  uint64_t lower = 0;
+  for (int j = part; j < n; j += LAST / FEW)
+    if (static_cast<uint32_t>(f.order[j]) > static_cast<uint32_t>(order)) lower += f.weight[j];   // (complement of the index)
+  if (mine && lower) atomicAdd(&f.by_index[i], static_cast<unsigned long long>(lower));
+  __syncthreads();
+  const uint64_t target = target_of(a, row, f.kept);
+  if (part == 0 && keep && f.by_index[i] <= target && target < f.by_index[i] + w) answer(a, row, r, logits, index_of(order), f.kept);
 }
 
 __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   __shared__ uint64_t lds[LAST / 64];
-  __shared__ Cut told;
   __shared__ Digits digits;
   __shared__ unsigned long long chunk_sum[MAX_CHUNKS];
   __shared__ int chosen_chunk;
+  __shared__ Few few;
   __shared__ uint64_t rest;
   const int64_t row = blockIdx.x;
-  const uint64_t best = row_best(a, row, LAST, lds);
+  Cut cut = a.cuts[row];
+  const uint64_t best = cut.best;
   const Row r = row_of(a, row, logit_of(best));
   if (best == 0 || r.greedy) {
     if (threadIdx.x == 0) {
@@ -447,12 +561,17 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     }
     return;
   }
-  const Cut cut = find_cut(a, row, r, &told);
+  const uint32_t listed = a.listed[row];
+  if (listed > static_cast<uint32_t>(a.cap)) cut.mode = FULL;   // (BOUND: the bin did not fit the list)
   const float* logits = a.logits + row * a.stride;
+  if (cut.mode == PREFIX && listed <= FEW) {
+    choose_of_few(a, row, r, a.list + row * a.cap, static_cast<int>(listed), logits, few);
+    return;
+  }
   Tokens t;
   t.list = cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr;
   t.logits = logits;
-  t.n = cut.mode == FULL ? a.vocab : cut.mode == ALL ? 0 : min(a.listed[row], static_cast<uint32_t>(a.cap));
+  t.n = cut.mode == FULL ? a.vocab : cut.mode == ALL ? 0 : static_cast<int>(listed);
   const uint64_t above = cut.mode == BOUND ? cut.above : 0;
   auto self = [](uint64_t o) { return o; };
   auto w_of = [&](uint64_t o) { return weight(depth(r, logit_of(o))); };
@@ -467,7 +586,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
         t.each([&](uint64_t) { ++there; });
         there = block_sum<LAST>(there, lds);
         if (there > static_cast<uint64_t>(r.k))
-          least = walk(t, digits, 64, static_cast<uint64_t>(r.k) - 1, self, [](uint64_t) { return uint64_t{1}; });
+          least = walk(t, digits, static_cast<uint64_t>(r.k) - 1, self, [](uint64_t) { return uint64_t{1}; });
       }
       t.each([&](uint64_t o) { if (o >= least) total += w_of(o); });
       total = block_sum<LAST>(total, lds);
@@ -477,13 +596,11 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
       if (need == 0) {
         least = best;            // p = 0: the first token
       } else {
-        // The token up to which the sum reaches `need`, that is exceeds need - 1.
-        uint64_t in = 0;
-        t.each([&](uint64_t o) { if (o >= least) in += w_of(o); });
-        in = block_sum<LAST>(in, lds);
-        if (above + in >= need) {
+        // The token up to which the sum reaches `need`, that is exceeds need - 1: there is one, unless min-p's border
+        // comes first.
+        if (cut.mode != BOUND || cut.reached) {
           const uint64_t from = least;
-          least = walk(t, digits, 64, need - above - 1, self, [&](uint64_t o) { return o >= from ? w_of(o) : uint64_t{0}; });
+          least = walk(t, digits, need - above - 1, self, [&](uint64_t o) { return o >= from ? w_of(o) : uint64_t{0}; });
         }
       }
     }
@@ -509,10 +626,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     t.each([&](uint64_t o) { total += kept_weight(o); });
   }
   total = block_sum<LAST>(total, lds);
-  const float u = a.uniform[row];
-  uint64_t target = static_cast<uint64_t>((u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0) * static_cast<double>(total));
-  if (target >= total) target = total - 1;        // the largest weight is 2^40, so there is a total
-
+  const uint64_t target = target_of(a, row, total);
   int id;
   if (by_chunk) {
     if (threadIdx.x < 64) {
@@ -571,17 +685,10 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     id = digits.digit;
   } else {
     // Smaller indices first: the complement of the index orders them so, in 24 bits.
-    const uint64_t v = walk(t, digits, 24, target, [](uint64_t o) { return o & 0xFFFFFFu; }, kept_weight);
+    const uint64_t v = walk(t, digits, target, [](uint64_t o) { return o & 0xFFFFFFu; }, kept_weight);
     id = static_cast<int>(~static_cast<uint32_t>(v) & 0xFFFFFFu);
   }
-  if (threadIdx.x == 0) {
-    a.ids[row] = id;
-    if (a.logprobs) {
-      const float l = fminf(logits[id] + 0.0f, 3.4028234663852886e+38f);
-      a.logprobs[row] = static_cast<float>(-((static_cast<double>(r.top) - static_cast<double>(l)) * r.per +
-                                             log2(static_cast<double>(total)) - 40.0) * 0.6931471805599453);
-    }
-  }
+  if (threadIdx.x == 0) answer(a, row, r, logits, id, total);
 }
 
 constexpr int BAD = static_cast<int>(hipErrorInvalidValue);
@@ -590,7 +697,7 @@ bool shape_ok(int64_t rows, int64_t vocab) { return rows > 0 && rows <= 65535 &&
 int64_t chunks_of(int64_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
 int64_t cap_of(int64_t vocab) { return vocab < LIST ? vocab : LIST; }
 int64_t workspace_of(int64_t rows, int64_t vocab) {
-  return rows * (16 * chunks_of(vocab) + 12 * BINS + 8 * cap_of(vocab) + 4);
+  return rows * (16 * chunks_of(vocab) + static_cast<int64_t>(sizeof(Cut)) + 12 * BINS + 8 * cap_of(vocab) + 4);
 }
 
 }  // namespace
@@ -614,10 +721,11 @@ extern "C" int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t
   const int64_t chunks = chunks_of(vocab_size);
   uint64_t* w = static_cast<uint64_t*>(workspace);
   Args a{logits, logits_stride, uniform, temperature, top_k, top_p, min_p, out_ids, out_logprobs, static_cast<int>(vocab_size),
-         static_cast<int>(chunks), static_cast<int>(cap_of(vocab_size)), nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+         static_cast<int>(chunks), static_cast<int>(cap_of(vocab_size)), nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   a.best = w;
   a.sums = a.best + rows * chunks;
-  a.bin_weight = a.sums + rows * chunks;
+  a.cuts = reinterpret_cast<Cut*>(a.sums + rows * chunks);
+  a.bin_weight = reinterpret_cast<uint64_t*>(a.cuts + rows);
   a.list = a.bin_weight + rows * BINS;
   a.bin_count = reinterpret_cast<uint32_t*>(a.list + rows * a.cap);
   a.listed = a.bin_count + rows * BINS;
@@ -626,6 +734,8 @@ extern "C" int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return static_cast<int>(err);
   hipLaunchKernelGGL(sample_histogram_kernel, grid, threads, 0, stream, a);
+  if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
+  hipLaunchKernelGGL(sample_cut_kernel, dim3(static_cast<unsigned>(rows)), dim3(64), 0, stream, a);
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
   hipLaunchKernelGGL(sample_collect_kernel, grid, threads, 0, stream, a);
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
