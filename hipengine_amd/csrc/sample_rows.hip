@@ -32,6 +32,8 @@ constexpr int LAST = 1024;               // threads of pass 4
 constexpr int BINS = 512;
 constexpr int LIST = 16384;
 constexpr int FEW = 128;
+constexpr int NOTHING = 8 * 42;          // from this bin on a weight is less than 2^-40
+constexpr int CACHED = 2048;             // tokens of a list that pass 4 keeps in LDS
 constexpr int64_t MAX_VOCAB = 1 << 22;   // 1024 chunks; 2^22 weights of 2^40 stay under 2^63
 constexpr int MAX_CHUNKS = static_cast<int>(MAX_VOCAB / CHUNK);
 
@@ -80,6 +82,7 @@ __device__ __forceinline__ int index_of(uint64_t order) { return static_cast<int
 struct Row {
   float top;             // largest logit
   double per;            // octaves of weight per unit of logit: log2(e) / temperature
+  float per8;            // bins
   bool greedy;
   int k;                 // 0: all
   double p;              // 1: all
@@ -92,6 +95,7 @@ __device__ __forceinline__ Row row_of(const Args& a, int64_t row, float top) {
   const float t = a.temperature ? a.temperature[row] : 1.0f;
   r.greedy = !(t > 0.0f);
   r.per = r.greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(t);
+  r.per8 = static_cast<float>(fmin(r.per * 8.0, 3e38));
   const int k = a.top_k ? a.top_k[row] : 0;
   r.k = k > 0 && k < a.vocab ? k : 0;
   const float p = a.top_p ? a.top_p[row] : 1.0f;
@@ -102,17 +106,19 @@ __device__ __forceinline__ Row row_of(const Args& a, int64_t row, float top) {
 }
 __device__ __forceinline__ bool cuts(const Row& r) { return r.k > 0 || r.p < 1.0 || r.octaves < __builtin_inf(); }
 
-// Octaves below the largest weight.
+// Octaves below the largest weight, exactly enough for weights and for min-p.
 __device__ __forceinline__ double depth(const Row& r, float l) {
-  return fmin((static_cast<double>(r.top) - static_cast<double>(l)) * r.per, 2000.0);
+  return (static_cast<double>(r.top) - static_cast<double>(l)) * r.per;
 }
-__device__ __forceinline__ int bin_of(double y) { return min(static_cast<int>(y * 8.0), BINS - 1); }
-__device__ __forceinline__ uint64_t weight(double y) {   // 2^-y * 2^40
-  const double n = rint(y);
-  const uint32_t e = float_to_bits(__builtin_amdgcn_exp2f(static_cast<float>(n - y)));   // 0.7 .. 1.42
-  const int shift = 17 + static_cast<int>(e >> 23) - 127 - static_cast<int>(n);          // 40 - 23
-  const uint64_t m = (e & 0x7FFFFFu) | 0x800000u;
-  return shift >= 0 ? m << shift : shift > -32 ? m >> -shift : 0;
+// A bin need not be exact, only monotonous in the logit: float32.
+__device__ __forceinline__ int bin_of(const Row& r, float l) {
+  return static_cast<int>(fminf(fminf(r.top - l, 3e38f) * r.per8, static_cast<float>(BINS - 1)));
+}
+__device__ __forceinline__ uint64_t weight(double y) {   // 2^-y * 2^40, downwards
+  const double n = rint(fmin(y, 100.0));
+  const uint32_t e = float_to_bits(__builtin_amdgcn_exp2f(static_cast<float>(n - y)));   // 0.7 .. 1.42 (0 behind 100)
+  const uint32_t m = (e & 0x7FFFFFu) | 0x800000u;
+  return (static_cast<uint64_t>(m) << 18) >> min(static_cast<int>(n) + 128 - static_cast<int>(e >> 23), 63);
 }
 
 template <int N>
@@ -208,12 +214,12 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
   for (int i = 0; i < 16; ++i) {
     const uint64_t o = order_of(l[i], 0);
     if (o == 0) continue;
-    const double y = depth(r, logit_of(o));
+    const float x = logit_of(o);
+    const int bin = bin_of(r, x);
     if (count) {
-      atomicAdd(&counts[bin_of(y)], 1u);
-    } else {
-      const uint64_t w = weight(y);
-      if (w) atomicAdd(&weights[bin_of(y)], static_cast<unsigned long long>(w));
+      atomicAdd(&counts[bin], 1u);
+    } else if (bin < NOTHING) {
+      atomicAdd(&weights[bin], static_cast<unsigned long long>(weight(depth(r, x))));
     }
   }
   __syncthreads();
@@ -231,7 +237,7 @@ struct Cut {
   uint64_t above;       // weight of the bins before B (BOUND)
   uint64_t need;        // top-p: a token stays if less than this lies before it (BOUND)
   int mode;
-  int bin;              // B
+  int bin, last;        // B; min-p's border may lie in either of two bins
   int reached;          // whether `need` is reached within B (else min-p's border is there)
 };
 
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
     best = o > best ? o : best;
   }
   const Row r = row_of(a, row, logit_of(best));
-  Cut cut{best, 0, 0, ALL, BINS, 0};
+  Cut cut{best, 0, 0, ALL, BINS, BINS, 0};
   if (best != 0 && !r.greedy && cuts(r)) {
     uint64_t w[8], ws = 0;
     uint32_t c[8], cs = 0;
@@ -275,7 +281,9 @@ __global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
     }
     const uint64_t total = __shfl(static_cast<unsigned long long>(wi), 63);
     const uint64_t need = r.p < 1.0 ? border(r.p, total) : ~uint64_t{0};
-    const int min_bin = r.octaves < __builtin_inf() ? bin_of(fmin(r.octaves, 2000.0)) : BINS - 1;
+    // Bins below min_bin lie on this side of min-p's border whatever float32 makes of it, those above max_bin behind it.
+    const int min_bin = static_cast<int>(fmin(r.octaves * 8.0 * (1.0 - 1e-6), BINS - 1.0));
+    const int max_bin = static_cast<int>(fmin(r.octaves * 8.0 * (1.0 + 1e-6), BINS - 1.0));
     // First bin up to which k tokens, or `need`, are reached.
     int k_bin = BINS - 1, p_bin = BINS - 1;
     uint64_t wp = wi - ws;
@@ -293,10 +301,9 @@ __global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
       p_bin = min(p_bin, __shfl_xor(p_bin, off));
     }
     cut.need = need;
-    cut.reached = p_bin <= min_bin;
     if (r.k > 0) {
       // A border in the last bin cuts nothing (its weights are 0); what top-p and min-p then cut is not known by weight.
-      cut.bin = k_bin;
+      cut.bin = cut.last = k_bin;
       uint32_t to = ci - cs, up_to = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -308,6 +315,8 @@ __global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
       else cut.mode = r.p < 1.0 || r.octaves < __builtin_inf() ? FULL : ALL;
     } else {
       cut.bin = min(p_bin, min_bin);
+      cut.last = p_bin < min_bin ? p_bin : min(p_bin, max_bin);
+      cut.reached = p_bin <= cut.last;
       uint64_t before = 0;
       wp = wi - ws;
 #pragma unroll
@@ -318,7 +327,7 @@ __global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
       cut.above = __shfl(static_cast<unsigned long long>(before), cut.bin >> 3);
       cut.mode = cut.bin < BINS - 1 ? BOUND : ALL;
     }
-    if (cut.mode == ALL) cut.bin = BINS;
+    if (cut.mode == ALL) cut.bin = cut.last = BINS;
   }
   if (lane == 0) a.cuts[row] = cut;
 }
@@ -337,7 +346,7 @@ __global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
   if (threadIdx.x == 0) here = 0;
   __syncthreads();
   // A logit that lies more than half a bin behind B's end is passed over by one comparison.
-  const float floor = cut.bin < BINS - 1 ? static_cast<float>(static_cast<double>(r.top) - (cut.bin + 1.5) * 0.125 / r.per)
+  const float floor = cut.last < BINS - 1 ? static_cast<float>(static_cast<double>(r.top) - (cut.last + 1.5) * 0.125 / r.per)
                                          : -__builtin_inff();
   uint64_t sum = 0;
   uint32_t slot[16];
@@ -347,10 +356,13 @@ __global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
     if (!(l[i] >= floor)) continue;
     const uint64_t o = order_of(l[i], 0);
     if (o == 0) continue;
-    const double y = depth(r, logit_of(o));
-    const int b = bin_of(y);
-    if (cut.mode != PREFIX && b < cut.bin) sum += weight(y);
-    if (cut.mode == PREFIX ? b <= cut.bin : b == cut.bin) slot[i] = atomicAdd(&here, 1u);
+    const float x = logit_of(o);
+    const int bin = bin_of(r, x);
+    if (cut.mode != PREFIX && bin < cut.bin) {
+      if (bin < NOTHING) sum += weight(depth(r, x));
+    } else if (bin <= cut.last) {
+      slot[i] = atomicAdd(&here, 1u);
+    }
   }
   if (cut.mode != PREFIX) {
     sum = block_sum<THREADS>(sum, lds);
@@ -376,28 +388,30 @@ struct Digits {
   int digit;
 };
 
-// The tokens that pass 4 looks through: a list, or the whole row.
+// The tokens that pass 4 looks through: a list (with its weights, where it is kept in LDS), or the whole row.
 struct Tokens {
+  const Row& r;
   const uint64_t* list;
+  const uint64_t* weights;
   const float* logits;
   int n;
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     for (int i = threadIdx.x; i < n; i += LAST) {
       const uint64_t o = list ? list[i] : order_of(logits[i], i);
-      if (o) f(o);
+      if (o) f(o, [&] { return weights ? weights[i] : weight(depth(r, logit_of(o))); });
     }
   }
 };
 
 // Walks down a number digit by digit (8 bits) to the token at which a running sum first exceeds `before` (the sum up to and
-// including it is more than that).  value(order): the number, larger is earlier, no two tokens' the same.  add(order): what
-// the token adds (0: not among them).  Counts or weights: any whole numbers.  Returns the number.  Leading bits that all
+// including it is more than that).  value(order): the number, larger is earlier, no two tokens' the same.  add(order, weight):
+// what the token adds (0: not among them).  Counts or weights: any whole numbers.  Returns the number.  Leading bits that all
 // tokens have in common are passed over, and it ends early where one token is left.
 template <typename V, typename A>
 __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t before, V value, A add) {
   uint64_t some = 0, all = ~uint64_t{0};
-  t.each([&](uint64_t o) {
+  t.each([&](uint64_t o, auto) {
     const uint64_t v = value(o);
     some |= v;
     all &= v;
@@ -419,10 +433,10 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t be
     __syncthreads();
     for (int i = threadIdx.x; i < 256; i += LAST) { d.weights[i] = 0; d.counts[i] = 0; }
     __syncthreads();
-    t.each([&](uint64_t o) {
+    t.each([&](uint64_t o, auto w_of) {
       const uint64_t v = value(o);
       if (high < 64 && (v >> high) != prefix) return;
-      const uint64_t w = add(o);
+      const uint64_t w = add(o, w_of);
       if (w == 0) return;
       const int digit = static_cast<int>((v >> low) & mask);
       atomicAdd(&d.weights[digit], static_cast<unsigned long long>(w));
@@ -457,9 +471,9 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t be
     high = low;
     if (d.in == 1 && high > 0) {     // the one token's remaining digits
       __syncthreads();
-      t.each([&](uint64_t o) {
+      t.each([&](uint64_t o, auto w_of) {
         const uint64_t v = value(o);
-        if ((v >> high) == prefix && add(o)) d.before = v;
+        if ((v >> high) == prefix && add(o, w_of)) d.before = v;
       });
       __syncthreads();
       prefix = d.before;
@@ -549,6 +563,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   __shared__ unsigned long long chunk_sum[MAX_CHUNKS];
   __shared__ int chosen_chunk;
   __shared__ Few few;
+  __shared__ uint64_t kept_order[CACHED], kept_weight[CACHED];
   __shared__ uint64_t rest;
   const int64_t row = blockIdx.x;
   Cut cut = a.cuts[row];
@@ -568,13 +583,20 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     choose_of_few(a, row, r, a.list + row * a.cap, static_cast<int>(listed), logits, few);
     return;
   }
-  Tokens t;
-  t.list = cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr;
-  t.logits = logits;
-  t.n = cut.mode == FULL ? a.vocab : cut.mode == ALL ? 0 : static_cast<int>(listed);
+  Tokens t{r, cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr, nullptr, logits,
+           cut.mode == FULL ? a.vocab : cut.mode == ALL ? 0 : static_cast<int>(listed)};
+  if (t.list && t.n <= CACHED) {
+    for (int i = threadIdx.x; i < t.n; i += LAST) {
+      const uint64_t o = t.list[i];
+      kept_order[i] = o;
+      kept_weight[i] = weight(depth(r, logit_of(o)));
+    }
+    t.list = kept_order;
+    t.weights = kept_weight;
+    __syncthreads();
+  }
   const uint64_t above = cut.mode == BOUND ? cut.above : 0;
   auto self = [](uint64_t o) { return o; };
-  auto w_of = [&](uint64_t o) { return weight(depth(r, logit_of(o))); };
 
   // Borders: a token stays if its order is `least` or more and its weight min-p's or more.
   uint64_t least = 0;
@@ -583,12 +605,12 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     if (cut.mode != BOUND) {
       if (r.k > 0) {
         uint64_t there = 0;
-        t.each([&](uint64_t) { ++there; });
+        t.each([&](uint64_t, auto) { ++there; });
         there = block_sum<LAST>(there, lds);
         if (there > static_cast<uint64_t>(r.k))
-          least = walk(t, digits, static_cast<uint64_t>(r.k) - 1, self, [](uint64_t) { return uint64_t{1}; });
+          least = walk(t, digits, static_cast<uint64_t>(r.k) - 1, self, [](uint64_t, auto) { return uint64_t{1}; });
       }
-      t.each([&](uint64_t o) { if (o >= least) total += w_of(o); });
+      t.each([&](uint64_t o, auto w_of) { if (o >= least) total += w_of(); });
       total = block_sum<LAST>(total, lds);
     }
     if (r.p < 1.0) {
@@ -600,30 +622,29 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
         // comes first.
         if (cut.mode != BOUND || cut.reached) {
           const uint64_t from = least;
-          least = walk(t, digits, need - above - 1, self, [&](uint64_t o) { return o >= from ? w_of(o) : uint64_t{0}; });
+          least = walk(t, digits, need - above - 1, self,
+                       [&](uint64_t o, auto w_of) { return o >= from ? w_of() : uint64_t{0}; });
         }
       }
     }
   }
-  auto kept = [&](uint64_t o, double y) { return o >= least && y <= r.octaves; };
-  auto kept_weight = [&](uint64_t o) {
-    const double y = depth(r, logit_of(o));
-    return kept(o, y) ? weight(y) : uint64_t{0};
-  };
+  const bool by_depth = r.octaves < __builtin_inf();
+  auto stays = [&](uint64_t o) { return o >= least && (!by_depth || depth(r, logit_of(o)) <= r.octaves); };
+  auto weight_left = [&](uint64_t o, auto w_of) { return stays(o) ? w_of() : uint64_t{0}; };
 
   uint64_t total = 0;
   const bool by_chunk = cut.mode == ALL || cut.mode == BOUND;
   if (by_chunk) {
     for (int c = threadIdx.x; c < a.chunks; c += LAST) chunk_sum[c] = a.sums[row * a.chunks + c];
     __syncthreads();
-    t.each([&](uint64_t o) {
-      const uint64_t w = kept_weight(o);
+    t.each([&](uint64_t o, auto w_of) {
+      const uint64_t w = weight_left(o, w_of);
       if (w) atomicAdd(&chunk_sum[index_of(o) / CHUNK], static_cast<unsigned long long>(w));
     });
     __syncthreads();
     for (int c = threadIdx.x; c < a.chunks; c += LAST) total += chunk_sum[c];
   } else {
-    t.each([&](uint64_t o) { total += kept_weight(o); });
+    t.each([&](uint64_t o, auto w_of) { total += weight_left(o, w_of); });
   }
   total = block_sum<LAST>(total, lds);
   const uint64_t target = target_of(a, row, total);
@@ -658,9 +679,9 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
       w[i] = 0;
       const uint64_t o = first + i < a.vocab ? order_of(logits[first + i], first + i) : 0;
       if (o) {
-        const double y = depth(r, logit_of(o));
-        const int b = bin_of(y);
-        if (b < cut.bin || (b == cut.bin && kept(o, y))) w[i] = weight(y);
+        const float x = logit_of(o);
+        const int bin = bin_of(r, x);
+        if (bin < cut.bin || (bin <= cut.last && stays(o))) w[i] = weight(depth(r, x));
       }
       s += w[i];
     }
@@ -685,7 +706,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     id = digits.digit;
   } else {
     // Smaller indices first: the complement of the index orders them so, in 24 bits.
-    const uint64_t v = walk(t, digits, target, [](uint64_t o) { return o & 0xFFFFFFu; }, kept_weight);
+    const uint64_t v = walk(t, digits, target, [](uint64_t o) { return o & 0xFFFFFFu; }, weight_left);
     id = static_cast<int>(~static_cast<uint32_t>(v) & 0xFFFFFFu);
   }
   if (threadIdx.x == 0) answer(a, row, r, logits, id, total);
