@@ -39,22 +39,23 @@ struct Piece {
   int64_t row;         // row of the batch that token `first` is
 };
 
+// Every wave finds it for itself, 64 sequences at a time and without a barrier.
 __device__ __forceinline__ bool find_piece(const int32_t* __restrict__ q_start, const int32_t* __restrict__ kv_lens,
-                                           int64_t tokens, int batch, int per_seq, int64_t unit, int* found, Piece& p) {
-  int seq;
+                                           int64_t tokens, int batch, int per_seq, int64_t unit, Piece& p) {
+  int seq = -1;
   int64_t local;
   if (per_seq > 0) {
     seq = static_cast<int>(unit / per_seq);
     local = unit - static_cast<int64_t>(seq) * per_seq;
   } else {
-    if (threadIdx.x == 0) *found = -1;
-    __syncthreads();
-    int mine = -1;
-    for (int b = threadIdx.x; b < batch; b += THREADS)
-      if ((max(q_start[b], 0) >> 5) + 2 * static_cast<int64_t>(b) <= unit) mine = b;
-    if (mine >= 0) atomicMax(found, mine);
-    __syncthreads();
-    seq = *found;
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < batch; b0 += 64) {
+      const int b = b0 + lane;
+      const bool before = b < batch && (max(q_start[b], 0) >> 5) + 2 * static_cast<int64_t>(b) <= unit;
+      const unsigned long long all = __ballot(before);
+      if (all) seq = b0 + 63 - __builtin_clzll(all);
+      if (all != ~0ull) break;                        // (blocks in front grow from sequence to sequence)
+    }
     if (seq < 0) return false;
     local = unit - ((max(q_start[seq], 0) >> 5) + 2 * static_cast<int64_t>(seq));
   }
@@ -65,7 +66,7 @@ __device__ __forceinline__ bool find_piece(const int32_t* __restrict__ q_start, 
   p.seq = seq;
   p.block = (from >> 5) + local;
   const int64_t base = p.block << 5;
-  if (base >= end || rows.count <= 0) return false;
+  if (local < 0 || base >= end || rows.count <= 0) return false;
   p.first = static_cast<int>(max(from - base, int64_t{0}));
   p.last = static_cast<int>(min(end - base, int64_t{KV_BLOCK}));
   p.row = rows.first + (base + p.first - begin);
@@ -87,25 +88,38 @@ struct AppendArgs {
   float eps, rope_scale;
 };
 
-__device__ __forceinline__ uint32_t quantize(float x, float scale) {
-  return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(rintf(x / scale), -127.0f), 127.0f)) + 128);
+// 128 + rint(x / scale) in the low byte: the quotient by the reciprocal, corrected by its exact remainder (rounded as the
+// division is), and the rounding by adding 1.5 * 2^23.  |x| is at most 127 scales up to the scale's own rounding, which rint
+// takes off again: nothing is to be clamped.
+__device__ __forceinline__ uint32_t quantize(float x, float scale, float reciprocal) {
+  const float q = x * reciprocal, exact = fmaf(fmaf(-scale, q, x), reciprocal, q);
+  return float_to_bits(exact + 12583040.0f);
+}
+// The low bytes of four.
+__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
 }
 __device__ __forceinline__ uint32_t requantize(uint32_t byte, float ratio) {
   return static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(static_cast<int>(byte) - 128) * ratio)) + 128);
 }
 
-// grid (units, heads, 2): z 0 is K, z 1 is V.
-template <int KIND, int D>
-__global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendArgs a) {
-  constexpr int LANES = D / 8, ROWS = THREADS / LANES, PAD = D + 4;
-  __shared__ float x[KV_BLOCK * PAD];
-  __shared__ float2 turn[ROWS][D / 2];
-  __shared__ float amax_of[THREADS / 64];
-  __shared__ int found;
-  const bool is_v = blockIdx.z != 0;
+template <int D>
+struct AppendLds {
+  static constexpr int ROWS = THREADS / (D / 8), PAD = D + 4;
+  float x[KV_BLOCK * PAD];
+  float2 turn[ROWS][D / 2];
+  uint32_t amax_of[THREADS / 64];
+};
+
+template <int KIND, int D, bool is_v>
+__device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& lds) {
+  constexpr int LANES = D / 8, ROWS = AppendLds<D>::ROWS, PAD = AppendLds<D>::PAD;
+  float* x = lds.x;
+  auto& turn = lds.turn;
+  auto& amax_of = lds.amax_of;
   const int head = blockIdx.y;
   Piece p;
-  if (!find_piece(a.q_start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, &found, p)) return;
+  if (!find_piece(a.q_start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, p)) return;
   const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
   if (block < 0) return;
 
@@ -113,17 +127,24 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendArgs a) {
   const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const void* src = is_v ? a.v : a.k;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
-  float amax = 0.0f;
-  bool finite = true;
-  for (int t0 = p.first; t0 < p.last; t0 += ROWS) {
-    const int t = t0 + sub;
-    const int64_t row = p.row + (t - p.first);
-    float y[8];
-    if (t < p.last) load8_f32<KIND>(src, row * stride + static_cast<int64_t>(head) * D + 8 * slot, y);
+  constexpr int PASSES = KV_BLOCK / ROWS;
+  float y[PASSES][8];
+  uint32_t amax_bits = 0;         // magnitudes order like their bits, infinity and NaN above all numbers
+  // All rows are asked for at once; the angles are computed while they are on their way.
+  auto row_at = [&](int t) { return (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D; };
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int t = p.first + i * ROWS + sub;
+    if (t < p.last) load8_f32<KIND>(src, row_at(t) + 8 * slot, y[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int t0 = p.first + i * ROWS, t = t0 + sub;
+    if (t0 >= p.last) break;
     if (!is_v && a.inv_freq) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < ROWS * (a.rotary_dim / 2); i += THREADS) {
-        const int r = i / (a.rotary_dim / 2), j = i - r * (a.rotary_dim / 2);
+      if (i > 0) __syncthreads();
+      for (int k = threadIdx.x; k < ROWS * (a.rotary_dim / 2); k += THREADS) {
+        const int r = k / (a.rotary_dim / 2), j = k - r * (a.rotary_dim / 2);
         if (t0 + r < p.last) {
           const int64_t at = a.positions ? a.positions[p.row + (t0 + r - p.first)] : (p.block << 5) + t0 + r;
           turn[r][j] = rotation(at, a.inv_freq[j], a.rope_scale);
@@ -133,65 +154,72 @@ __global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendArgs a) {
     }
     if (t < p.last) {
       if (!is_v)
-        norm_rotate8<KIND, D>(y, src, row * stride + static_cast<int64_t>(head) * D, slot, a.k_weight, a.eps, turn[sub],
-                              a.rotary_dim, a.interleaved != 0);
+        norm_rotate8<KIND, D>(y[i], src, row_at(t), slot, a.k_weight, a.eps, turn[sub], a.rotary_dim, a.interleaved != 0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[t * PAD + 8 * slot + i] = y[i];
-        amax = fmaxf(amax, fabsf(y[i]));
-        finite = finite && fabsf(y[i]) <= 3.4028234663852886e+38f;
+      for (int k = 0; k < 8; ++k) {
+        x[t * PAD + 8 * slot + k] = y[i][k];
+        amax_bits = max(amax_bits, float_to_bits(y[i][k]) & 0x7FFFFFFFu);
       }
     }
   }
-  if (!finite) amax = __builtin_inff();
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-  if ((threadIdx.x & 63) == 0) amax_of[threadIdx.x >> 6] = amax;
+  for (int off = 1; off < 64; off <<= 1) amax_bits = max(amax_bits, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax_bits), off)));
+  if ((threadIdx.x & 63) == 0) amax_of[threadIdx.x >> 6] = amax_bits;
   __syncthreads();
-  amax = fmaxf(fmaxf(amax_of[0], amax_of[1]), fmaxf(amax_of[2], amax_of[3]));
+  amax_bits = max(max(amax_of[0], amax_of[1]), max(amax_of[2], amax_of[3]));
+  const float amax = bits_to_float(amax_bits);
 
   float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
   const float old = p.first > 0 ? *scale_at : 0.0f;
-  const bool poisoned = !(amax <= 3.4028234663852886e+38f) || old != old;
+  const bool poisoned = amax_bits >= 0x7F800000u || old != old;
   const float scale = fmaxf(fmaxf(old, amax / 127.0f), KV_SCALE_FLOOR);
-  const float ratio = old / scale;                    // 1 where the scale stays
+  const float ratio = old / scale, reciprocal = 1.0f / scale;      // ratio: 1 where the scale stays
   uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
   __syncthreads();                                     // every thread has read the old scale
   if (threadIdx.x == 0) *scale_at = poisoned ? __builtin_nanf("") : scale;
 
+  const bool grown = ratio != 1.0f && !poisoned, whole = p.first == 0 && p.last == KV_BLOCK && !poisoned;
   for (int item = threadIdx.x; item < 2 * D; item += THREADS) {
     // 16 bytes: of K one token's 16 dims, of V one dim's 16 tokens.
     const int t_k = item & 31, d_k = (item >> 5) * 16;
     const int d_v = item >> 1, place0 = (item & 1) * 16;
-    const bool grown = ratio != 1.0f && !poisoned;
-    bool keeps, takes;                                  // whether it holds tokens that stay (or lie behind), or new ones
-    if (is_v) {
-      keeps = p.first > 0 || p.last < KV_BLOCK;
-      takes = true;
+    auto at = [&](int k) { return is_v ? v_token(place0 + k) * PAD + d_v : t_k * PAD + d_k + k; };
+    uint32_t w[4];
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = pack_bytes(quantize(x[at(4 * i)], scale, reciprocal), quantize(x[at(4 * i + 1)], scale, reciprocal),
+                          quantize(x[at(4 * i + 2)], scale, reciprocal), quantize(x[at(4 * i + 3)], scale, reciprocal));
     } else {
-      keeps = t_k < p.first;
-      takes = t_k >= p.first && t_k < p.last;
-    }
-    if (!takes && !(keeps && grown)) continue;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (keeps) u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
-    uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      const bool keeps = is_v || t_k < p.first, takes = is_v || (t_k >= p.first && t_k < p.last);
+      if (!takes && !(keeps && grown)) continue;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (keeps) u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t r = 0;
+      for (int i = 0; i < 4; ++i) {
+        uint32_t r = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = is_v ? v_token(place0 + 4 * i + j) : t_k;
-        const int d = is_v ? d_v : d_k + 4 * i + j;
-        uint32_t b = (w[i] >> (8 * j)) & 0xFFu;
-        if (t >= p.first && t < p.last) b = poisoned ? 128u : quantize(x[t * PAD + d], scale);
-        else if (t < p.first && grown) b = requantize(b, ratio);
-        r |= b << (8 * j);
+        for (int j = 0; j < 4; ++j) {
+          const int t = is_v ? v_token(place0 + 4 * i + j) : t_k;
+          uint32_t b = (w[i] >> (8 * j)) & 0xFFu;
+          if (t >= p.first && t < p.last) b = poisoned ? 128u : quantize(x[at(4 * i + j)], scale, reciprocal) & 0xFFu;
+          else if (t < p.first && grown) b = requantize(b, ratio);
+          r |= b << (8 * j);
+        }
+        w[i] = r;
       }
-      w[i] = r;
     }
     *reinterpret_cast<uint4*>(bytes + item_offset(item)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+
+// grid (units, heads, 2): z 0 is K, z 1 is V.
+template <int KIND, int D>
+__global__ void __launch_bounds__(THREADS) kv_append_kernel(AppendArgs a) {
+  __shared__ AppendLds<D> lds;
+  if (blockIdx.z == 0) append_piece<KIND, D, false>(a, lds);
+  else append_piece<KIND, D, true>(a, lds);
 }
 
 struct ReadArgs {
@@ -211,13 +239,12 @@ template <int KIND, int D>
 __global__ void __launch_bounds__(THREADS) kv_read_kernel(ReadArgs a) {
   constexpr int LANES = D / 8, ROWS = THREADS / LANES, V_ROW = KV_BLOCK + 4;   // V rows padded: 8 lanes read 8 dims apart
   __shared__ __align__(16) uint8_t lds[D * V_ROW];
-  __shared__ int found;
   const bool is_v = blockIdx.z != 0;
   void* dst = is_v ? a.v : a.k;
   if (!dst) return;
   const int head = blockIdx.y;
   Piece p;
-  if (!find_piece(a.start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, &found, p)) return;
+  if (!find_piece(a.start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, p)) return;
   const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
   const float scale = block < 0 ? 0.0f : (is_v ? a.cache.v_scale : a.cache.k_scale)[block];
   if (block >= 0) {
