@@ -78,14 +78,17 @@ __device__ __forceinline__ void load8_f32(const void* base, int64_t idx, float (
   }
 }
 
-// bf16 stores keep NaN a NaN (float_to_bf16_bits carries a NaN's low mantissa into the sign).
-__device__ __forceinline__ uint32_t bf16_bits_nan(float v) {
-  return v != v ? 0x7FC0u : static_cast<uint32_t>(float_to_bf16_bits(v));
-}
-
+// Two values as bf16 or fp16, rounded to nearest even, in one conversion instruction; a NaN stays one.
 template <int KIND>
-__device__ __forceinline__ uint32_t half_bits(float v) {
-  return KIND == KIND_BF16 ? bf16_bits_nan(v) : static_cast<uint32_t>(float_to_f16_bits(v));
+__device__ __forceinline__ uint32_t half_bits2(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  if constexpr (KIND == KIND_BF16) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+  } else {
+    typedef half_t h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
+  }
 }
 
 template <int KIND>
@@ -95,7 +98,7 @@ __device__ __forceinline__ void store8_f32(void* base, int64_t idx, const float 
   } else {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = half_bits<KIND>(v[2 * i]) | (half_bits<KIND>(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) w[i] = half_bits2<KIND>(v[2 * i], v[2 * i + 1]);
     __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(base) + idx, 2), w, 16);
   }
 }
@@ -112,44 +115,40 @@ __device__ __forceinline__ float2 rotation(int64_t position, float inv_freq, flo
   return make_float2(c * scale, s * scale);
 }
 
-// One head's RMS norm and rotation by the lanes that hold it, 8 values a lane.  `x` is the lane's own 8 values (head
-// dims 8 * slot ..), `src` the head in memory: a lane that needs the other half of its pairs reads them again (they are
-// in L1) instead of asking its neighbours.
+// Sum over an aligned group of 8, 16 or 32 lanes, in all of them; no LDS.
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp_f<DPP_QUAD_XOR1>(v);
+  v += dpp_f<DPP_QUAD_XOR2>(v);
+  v += dpp_f<DPP_ROW_HALF_MIRROR>(v);
+  if constexpr (LANES >= 16) v += dpp_f<0x140>(v);          // row_mirror: lane i <-> lane 15-i
+  if constexpr (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(float_to_bits(v), float_to_bits(v), false, false);
+    v = bits_to_float(r[0]) + bits_to_float(r[1]);          // one of the two is the lane's own, the other its partner's
+  }
+  return v;
+}
+
+// One head's RMS norm and rotation by the D / 8 neighbouring lanes that hold it, 8 values a lane (x: head dims 8 * slot ..).
 // `turn` holds (cos, sin) of the rotary_dim / 2 pairs.  rotary_dim is a multiple of 16, so a lane's 8 values lie on one
-// side of every border.
-template <int KIND, int D>
-__device__ __forceinline__ void norm_rotate8(float (&x)[8], const void* src, int64_t src_idx, int slot,
-                                             const float* __restrict__ weight, float eps, const float2* turn,
-                                             int rotary_dim, bool interleaved) {
+// side of every border and their partners all in one other lane.
+template <int D>
+__device__ __forceinline__ void norm_rotate8(float (&x)[8], int slot, const float* __restrict__ weight, float eps,
+                                             const float2* turn, int rotary_dim, bool interleaved) {
   constexpr int LANES = D / 8;
   const int d0 = 8 * slot, pairs = rotary_dim >> 1;
-  const bool split = !interleaved && d0 < rotary_dim;
-  float y[8];
-  const int other = d0 < pairs ? d0 + pairs : d0 - pairs;
-  if (split) load8_f32<KIND>(src, src_idx + other, y);
   if (weight) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-    for (int off = 1; off < LANES; off <<= 1) sum += __shfl_xor(sum, off);
-    const float r = 1.0f / sqrtf(sum * (1.0f / D) + eps);
-    float w[8];
+    float w[8], sum = 0.0f;
     load8_f32<KIND_F32>(weight, d0, w);
 #pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+    sum = group_sum<LANES>(sum);
+    const float r = 1.0f / sqrtf(sum * (1.0f / D) + eps);
+#pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
-    if (split) {
-      load8_f32<KIND_F32>(weight, other, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
-    }
   }
-  if (split) {
-    const float sign = d0 < pairs ? -1.0f : 1.0f;
-    const float2* cs = turn + (d0 < pairs ? d0 : other);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i].x, sign * y[i] * cs[i].y);
-  } else if (interleaved && d0 < rotary_dim) {
+  if (d0 >= rotary_dim) return;
+  if (interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 cs = turn[(d0 >> 1) + i];
@@ -157,6 +156,15 @@ __device__ __forceinline__ void norm_rotate8(float (&x)[8], const void* src, int
       x[2 * i] = fmaf(a, cs.x, -b * cs.y);
       x[2 * i + 1] = fmaf(b, cs.x, a * cs.y);
     }
+  } else {
+    const bool low = d0 < pairs;
+    const int other = low ? d0 + pairs : d0 - pairs, lane = (static_cast<int>(threadIdx.x) & 63 & ~(LANES - 1)) + (other >> 3);
+    const float2* cs = turn + (low ? d0 : other);
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i].x, (low ? -y[i] : y[i]) * cs[i].y);
   }
 }
 

@@ -108,6 +108,8 @@ struct AppendLds {
   static constexpr int ROWS = THREADS / (D / 8), PAD = D + 4;
   float x[KV_BLOCK * PAD];
   float2 turn[ROWS][D / 2];
+  int64_t position[KV_BLOCK];
+  float freq[D / 2];
   uint32_t amax_of[THREADS / 64];
 };
 
@@ -137,24 +139,29 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
     const int t = p.first + i * ROWS + sub;
     if (t < p.last) load8_f32<KIND>(src, row_at(t) + 8 * slot, y[i]);
   }
+  const int pairs = a.rotary_dim / 2;
+  if (!is_v && pairs > 0) {
+    if (threadIdx.x < static_cast<unsigned>(pairs)) lds.freq[threadIdx.x] = a.inv_freq[threadIdx.x];
+    const int t = p.first + static_cast<int>(threadIdx.x) - THREADS / 2;      // (other threads than those)
+    if (t >= p.first && t < p.last)
+      lds.position[t] = a.positions ? a.positions[p.row + (t - p.first)] : (p.block << 5) + t;
+    __syncthreads();
+  }
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int t0 = p.first + i * ROWS, t = t0 + sub;
     if (t0 >= p.last) break;
-    if (!is_v && a.inv_freq) {
+    if (!is_v && pairs > 0) {
       if (i > 0) __syncthreads();
-      for (int k = threadIdx.x; k < ROWS * (a.rotary_dim / 2); k += THREADS) {
-        const int r = k / (a.rotary_dim / 2), j = k - r * (a.rotary_dim / 2);
-        if (t0 + r < p.last) {
-          const int64_t at = a.positions ? a.positions[p.row + (t0 + r - p.first)] : (p.block << 5) + t0 + r;
-          turn[r][j] = rotation(at, a.inv_freq[j], a.rope_scale);
-        }
+      for (int k = threadIdx.x; k < ROWS * pairs; k += THREADS) {
+        const int r = k / pairs, j = k - r * pairs;
+        if (t0 + r < p.last) turn[r][j] = rotation(lds.position[t0 + r], lds.freq[j], a.rope_scale);
       }
       __syncthreads();
     }
     if (t < p.last) {
       if (!is_v)
-        norm_rotate8<KIND, D>(y[i], src, row_at(t), slot, a.k_weight, a.eps, turn[sub], a.rotary_dim, a.interleaved != 0);
+        norm_rotate8<D>(y[i], slot, a.k_weight, a.eps, turn[sub], a.rotary_dim, a.interleaved != 0);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         x[t * PAD + 8 * slot + k] = y[i][k];

@@ -284,7 +284,7 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const SeqRows& r
       uint32_t w[2];
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        w[b] = half_bits<KIND>(acc[t][i + 2 * b] * f) | (half_bits<KIND>(acc[t][i + 2 * b + 1] * f) << 16);
+        w[b] = half_bits2<KIND>(acc[t][i + 2 * b] * f, acc[t][i + 2 * b + 1] * f);
       __builtin_memcpy(__builtin_assume_aligned(out + 32 * t + 2 * i, 2), w, 8);
     }
 }
@@ -599,8 +599,10 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* dst = static_cast<uint16_t*>(a.out) + (rows.first + query) * a.out_stride + static_cast<int64_t>(q_head) * D + lane * V;
+  uint32_t w[(V + 1) / 2];
 #pragma unroll
-  for (int v = 0; v < V; ++v) dst[v] = static_cast<uint16_t>(half_bits<KIND>(o[v] * f));
+  for (int v = 0; v < V; v += 2) w[v / 2] = half_bits2<KIND>(o[v] * f, v + 1 < V ? o[v + 1] * f : 0.0f);
+  __builtin_memcpy(__builtin_assume_aligned(dst, 2), w, 2 * V);
 }
 
 // How a call is cut: decided from sizes alone, so that the workspace can be sized before the call.
