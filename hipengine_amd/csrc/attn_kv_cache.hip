@@ -109,7 +109,7 @@ struct AppendLds {
   float x[KV_BLOCK * PAD];
   float2 turn[ROWS][D / 2];
   int64_t position[KV_BLOCK];
-  float freq[D / 2];
+  double freq[D / 2];
   uint32_t amax_of[THREADS / 64];
 };
 
@@ -141,7 +141,7 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
   }
   const int pairs = a.rotary_dim / 2;
   if (!is_v && pairs > 0) {
-    if (threadIdx.x < static_cast<unsigned>(pairs)) lds.freq[threadIdx.x] = a.inv_freq[threadIdx.x];
+    if (threadIdx.x < static_cast<unsigned>(pairs)) lds.freq[threadIdx.x] = turns_of(a.inv_freq[threadIdx.x]);
     const int t = p.first + static_cast<int>(threadIdx.x) - THREADS / 2;      // (other threads than those)
     if (t >= p.first && t < p.last)
       lds.position[t] = a.positions ? a.positions[p.row + (t - p.first)] : (p.block << 5) + t;

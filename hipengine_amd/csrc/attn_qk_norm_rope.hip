@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_kernel(QkArgs a) {
     load8_f32<IN>(is_q ? a.q : a.k, at + 8 * slot, x);
   };
   const bool turns = threadIdx.x < static_cast<unsigned>(pairs);
-  const float freq = turns ? a.inv_freq[threadIdx.x] : 0.0f;
+  const double freq = turns ? turns_of(a.inv_freq[threadIdx.x]) : 0.0;
   int64_t position = turns ? a.positions[blockIdx.x] : 0;
   float x[8];
   load(blockIdx.x, first, x);
