@@ -156,16 +156,25 @@ struct Blocks {
   int base, step;
   int64_t number;
   float ks, lv, iv;    // scale of K, log2 of V's, 1 / V's
-  __device__ __forceinline__ void lookup(const KvCacheQ8& c, int seq, int head, int from, int end) {
+  bool found;
+  __device__ __forceinline__ void find(const KvCacheQ8& c, int seq, int head, int from, int end) {
     base = from;
     const int mine = from + static_cast<int>(threadIdx.x & 63) * step;
-    const int64_t found = mine < end ? kv_block_index(c, seq, mine, head) : -1;
-    number = max(found, int64_t{0});
+    number = mine < end ? kv_block_index(c, seq, mine, head) : -1;
+    found = number >= 0;
+    number = max(number, int64_t{0});
+  }
+  // Apart, so that the blocks themselves can be asked for first.
+  __device__ __forceinline__ void scales(const KvCacheQ8& c) {
     const float v = c.v_scale[number], k = c.k_scale[number];
     const float v_clean = fmaxf(v, KV_SCALE_FLOOR);          // of a NaN: the floor
-    ks = found < 0 ? 0.0f : fmaxf(k, k != k ? k : KV_SCALE_FLOOR);
-    lv = found < 0 ? -__builtin_inff() : v == v ? log2f(v_clean) : v;
-    iv = found < 0 ? 0.0f : 1.0f / v_clean;
+    ks = !found ? 0.0f : fmaxf(k, k != k ? k : KV_SCALE_FLOOR);
+    lv = !found ? -__builtin_inff() : v == v ? __builtin_amdgcn_logf(v_clean) : v;
+    iv = !found ? 0.0f : 1.0f / v_clean;
+  }
+  __device__ __forceinline__ void lookup(const KvCacheQ8& c, int seq, int head, int from, int end) {
+    find(c, seq, head, from, end);
+    scales(c);
   }
   __device__ __forceinline__ int slot(int which) const { return (which - base) / step; }
   __device__ __forceinline__ int64_t at(int which) const {
@@ -309,7 +318,6 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
     blk += split * a.chunk;
     if (split + 1 < a.splits) blk_end = min(blk_end, blk + a.chunk);   // the last chunk takes what a longer cache than announced holds
   }
-  const Column<D> k = load_column<D, KIND>(a, rows, sight, row0 + (lane & 31), n_rows, head);
   f16v acc[KC];
 #pragma unroll
   for (int t = 0; t < KC; ++t) acc[t] = f16v{0};
@@ -324,13 +332,16 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 #pragma unroll
     for (int i = 0; i < KC; ++i) r[i] = *reinterpret_cast<const uint4*>(p + i * 1024 + off);
   };
+  // The chain of a short call: lengths, page, block; everything else is asked for beside it.
+  uint4 kr[KC], vr[KC];
+  blocks.find(a.cache, seq, head, j, blk_end);
+  load(a.cache.k, j, k_off, kr);
+  load(a.cache.v, j, v_off, vr);
+  blocks.scales(a.cache);
+  const Column<D> k = load_column<D, KIND>(a, rows, sight, row0 + (lane & 31), n_rows, head);
   if (j < blk_end) {
     // K's registers are loaded with the next block as soon as the products with them are issued, V's likewise: each load
     // has the other half of a step to arrive in.
-    uint4 kr[KC], vr[KC];
-    blocks.lookup(a.cache, seq, head, j, blk_end);
-    load(a.cache.k, j, k_off, kr);
-    load(a.cache.v, j, v_off, vr);
     for (; j < blk_end; j += WAVES) {
       const Scales b = scales_of(blocks, j, lv_top);
       f16v s = f16v{0};
@@ -361,7 +372,7 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 
   // Join the four waves: 2 and 3 into 0 and 1, then 1 into 0; through at most 32 KB of LDS.
   constexpr int PART = KC < 4 ? KC : 4;
-  __shared__ float lds_acc[2][PART][16][64];
+  __shared__ float4 lds_acc[2][PART][4][64];
   __shared__ float lds_ml[2][2][64];
 #pragma unroll
   for (int other = WAVES / 2; other >= 1; other >>= 1) {
@@ -374,7 +385,9 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 #pragma unroll
         for (int t = 0; t < PART; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) lds_acc[wave - other][t][i][lane] = acc[t0 + t][i];
+          for (int i = 0; i < 4; ++i)
+            lds_acc[wave - other][t][i][lane] = make_float4(acc[t0 + t][4 * i], acc[t0 + t][4 * i + 1], acc[t0 + t][4 * i + 2],
+                                                            acc[t0 + t][4 * i + 3]);
       }
       __syncthreads();
       if (wave < other) {
@@ -388,7 +401,13 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 #pragma unroll
         for (int t = 0; t < PART; ++t)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[t0 + t][i] = acc[t0 + t][i] * f + lds_acc[wave][t][i][lane] * f2;
+          for (int i = 0; i < 4; ++i) {
+            const float4 o = lds_acc[wave][t][i][lane];
+            acc[t0 + t][4 * i] = acc[t0 + t][4 * i] * f + o.x * f2;
+            acc[t0 + t][4 * i + 1] = acc[t0 + t][4 * i + 1] * f + o.y * f2;
+            acc[t0 + t][4 * i + 2] = acc[t0 + t][4 * i + 2] * f + o.z * f2;
+            acc[t0 + t][4 * i + 3] = acc[t0 + t][4 * i + 3] * f + o.w * f2;
+          }
       }
       __syncthreads();
     }
@@ -555,22 +574,23 @@ __global__ void __launch_bounds__(ROW_WAVES * 64, D <= 128 ? 3 : 2) attention_ro
   store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, split, m, l, acc);
 }
 
-// Joins the chunks of one output row: grid (rows a sequence, batch), one wave a row, D / 64 dims a lane.
-template <int D, int KIND>
+// Joins the chunks of output rows: grid (rows a sequence / (4 / TEAM), batch); TEAM waves have a row and take its chunks in
+// turn, D / 64 dims a lane.  What bounds it is the time that a load takes: eight are on their way at once.  With more than
+// 8 chunks four waves join a row (40 rows of 64 chunks, one token behind 32768 others: 11.2 us with one wave a row, 5.4 with
+// four), else one (24576 rows of D 256 and 2 chunks: 13.2 us, with four 38.9).
+template <int D, int KIND, int TEAM>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   constexpr int V = D / 64;
-  const int seq = blockIdx.y, lane = threadIdx.x & 63;
+  __shared__ float part[4][D];
+  const int seq = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const SeqRows rows = seq_rows(a.q_start, seq, a.tokens);
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (r >= rows.count * a.q_heads) return;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (4 / TEAM) + wave / TEAM;
+  if (r >= rows.count * a.q_heads) return;             // (of a team all waves or none: the barrier below is for TEAM 4)
   const int query = static_cast<int>(r / a.q_heads), q_head = static_cast<int>(r - static_cast<int64_t>(query) * a.q_heads);
   // The chunks that a workgroup ran for this row: as the attention kernel laid them for the row's tile.
-  const int kv_len = min(max(a.kv_lens[seq], 0), MAX_KV), q_len = static_cast<int>(rows.count);
+  const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
   const int row = query * a.group + q_head % a.group;
-  const int tile_query = row / tile_rows * tile_rows / a.group;
-  const int lo = a.window > 0 ? max(kv_len - q_len + tile_query + 1 - a.window, 0) : 0;
-  const int lim = min(max(kv_len - q_len + query + 1, 0), kv_len);
-  const int blocks = max(((lim + 31) >> 5) - (lo >> 5), 0);
+  const int blocks = max(((sight.limit(query) + 31) >> 5) - (sight.lower(row / tile_rows * tile_rows / a.group) >> 5), 0);
   const int splits = min((blocks + a.chunk - 1) / a.chunk, a.splits);
   const int64_t at = (rows.first + query) * a.q_heads + q_head, pitch = a.tokens * a.q_heads;
   float m = NEVER;
@@ -587,8 +607,8 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
       l += a.part_ml[i + 1] * f;
     }
     const int n = min(splits - s0, 64);
-#pragma unroll 4
-    for (int k = 0; k < n; ++k) {
+#pragma unroll 8
+    for (int k = wave % TEAM; k < n; k += TEAM) {
       const float w = read_lane_f(f, k);
       const float* src = a.part_acc + ((s0 + k) * pitch + at) * D + lane * V;
 #pragma unroll
@@ -598,11 +618,22 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off);
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* dst = static_cast<uint16_t*>(a.out) + (rows.first + query) * a.out_stride + static_cast<int64_t>(q_head) * D + lane * V;
-  uint32_t w[(V + 1) / 2];
+  uint16_t* dst = static_cast<uint16_t*>(a.out) + (rows.first + query) * a.out_stride + static_cast<int64_t>(q_head) * D;
+  if constexpr (TEAM == 1) {
+    uint32_t w[(V + 1) / 2];
 #pragma unroll
-  for (int v = 0; v < V; v += 2) w[v / 2] = half_bits2<KIND>(o[v] * f, v + 1 < V ? o[v + 1] * f : 0.0f);
-  __builtin_memcpy(__builtin_assume_aligned(dst, 2), w, 2 * V);
+    for (int v = 0; v < V; v += 2) w[v / 2] = half_bits2<KIND>(o[v] * f, v + 1 < V ? o[v + 1] * f : 0.0f);
+    __builtin_memcpy(__builtin_assume_aligned(dst + lane * V, 2), w, 2 * V);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) part[wave][lane * V + v] = o[v];
+    __syncthreads();
+    const int d = 2 * threadIdx.x;
+    if (d >= D) return;
+    const uint32_t w = half_bits2<KIND>((part[0][d] + part[1][d] + part[2][d] + part[3][d]) * f,
+                                        (part[0][d + 1] + part[1][d + 1] + part[2][d + 1] + part[3][d + 1]) * f);
+    __builtin_memcpy(__builtin_assume_aligned(dst + d, 2), &w, 4);
+  }
 }
 
 // How a call is cut: decided from sizes alone, so that the workspace can be sized before the call.
@@ -626,11 +657,13 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   int64_t span = max_kv;
   if (window > 0 && window + max_q + 31 < span) span = window + max_q + 31;
   const int64_t blocks = (span + 31) / 32 + (window > 0 ? 1 : 0);
-  // Two workgroups a CU; with a workgroup a CU from the rows alone, prompts are not split (they would be joined for less
-  // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts). A part has at least 16 blocks.
+  // Two workgroups a CU.  With a workgroup a CU from the rows alone, prompts are not split (they would be joined for less
+  // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts).  A part has at least 16 blocks, and
+  // where waves share its keys at least 256 KB of them: a single token behind 600 others (19 blocks of 128) takes 14.4 us
+  // undivided and 17.3 us in two parts and the joining of them, behind 32768 others 22 us in 32 parts and 26 us in 64.
   const int64_t groups = batch * kv_heads * p.tiles;
   int64_t splits = !p.keys && groups >= CUS ? 1 : (2 * CUS + groups - 1) / groups;
-  const int64_t most = (blocks + 15) / 16;
+  const int64_t least = p.keys ? 4096 / dim : 16, most = (blocks + least - 1) / least;
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   p.most_splits = static_cast<int>(splits);
@@ -660,8 +693,11 @@ int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64
   else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(ROW_WAVES * 64), 0, stream, a);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
-  const dim3 join(static_cast<unsigned>((max_q * a.q_heads + 3) / 4), static_cast<unsigned>(batch));
-  hipLaunchKernelGGL((join_kernel<D, KIND>), join, dim3(256), 0, stream, a, p.tile_rows);
+  const int64_t out_rows = max_q * a.q_heads;
+  if (p.splits > 8)
+    hipLaunchKernelGGL((join_kernel<D, KIND, 4>), dim3(static_cast<unsigned>(out_rows), static_cast<unsigned>(batch)), dim3(256), 0, stream, a, p.tile_rows);
+  else
+    hipLaunchKernelGGL((join_kernel<D, KIND, 1>), dim3(static_cast<unsigned>((out_rows + 3) / 4), static_cast<unsigned>(batch)), dim3(256), 0, stream, a, p.tile_rows);
   return static_cast<int>(hipGetLastError());
 }
 
