@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_kernel(QkArgs a) {
 template <int IN, int OUT>
 int launch_dim(const QkArgs& a, int64_t tokens, int dim, hipStream_t stream) {
   const int lanes = dim / 8;
-  const int64_t want = static_cast<int64_t>(a.q_heads + a.kv_heads) * lanes;
+  // No fewer threads than pairs: each computes one angle.
+  const int64_t values = static_cast<int64_t>(a.q_heads + a.kv_heads) * lanes, want = values > dim / 2 ? values : dim / 2;
   const unsigned threads = static_cast<unsigned>(want >= 1024 ? 1024 : (want + 63) / 64 * 64);
   // As many workgroups as the chip's 256 CUs run at once.
   const int64_t most = 256 * (2048 / threads);

@@ -39,6 +39,9 @@ def inv_freq(rotary, theta=1e6):
     (5, 64, 16, 256, 256, False, "f32", "bf16", 77),      # more heads than one pass of a workgroup holds
     (4, 8, 0, 128, 128, False, "bf16", "fp16", 9),        # only queries
     (4, 0, 8, 128, 0, False, "fp16", "f32", 0),           # only keys, no rotation
+    (3, 1, 0, 256, 256, False, "bf16", "f32", 12345),     # more pairs than lanes that hold the heads
+    (2, 1, 1, 256, 144, True, "f32", "bf16", 99),
+    (5, 1, 0, 64, 64, False, "bf16", "bf16", 31),
 ])
 def test_qk_norm_rope(dev, tokens, hq, hk, dim, rotary, interleaved, kind, out, start):
     rng = np.random.default_rng(tokens * 131 + dim + hq)
