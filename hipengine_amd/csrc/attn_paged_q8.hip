@@ -656,7 +656,8 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   // Keys that a tile can see.
   int64_t span = max_kv;
   if (window > 0 && window + max_q + 31 < span) span = window + max_q + 31;
-  const int64_t blocks = (span + 31) / 32 + (window > 0 ? 1 : 0);
+  int64_t blocks = (span + 31) / 32;
+  if (blocks < (max_kv + 31) / 32) ++blocks;      // (a window may begin anywhere in a block)
   // Two workgroups a CU.  With a workgroup a CU from the rows alone, prompts are not split (they would be joined for less
   // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts).  A part has at least 16 blocks, and
   // where waves share its keys at least 256 KB of them: a single token behind 600 others (19 blocks of 128) takes 14.4 us

@@ -494,6 +494,20 @@ def test_attention_refuses_a_small_workspace(dev):
     c.free()
 
 
+@pytest.mark.parametrize("dim,kv_len", [(128, 1024), (128, 1055), (64, 2048), (256, 512)])
+def test_attention_workspace_is_enough_for_every_window(dev, dim, kv_len):
+    """The size that is asked for without a window, at lengths that are a whole number of parts and windows around them."""
+    rng = np.random.default_rng(91)
+    c = Cache(dev, rng, [kv_len], 64, 1, dim)
+    q = O.round_to(rng.standard_normal((1, 2, dim)), "bf16")
+    start, kv = np.array([0, 1], np.int32), np.array([kv_len], np.int32)
+    for window in (kv_len - 64, kv_len - 34, kv_len - 33, kv_len - 32, kv_len - 1, kv_len, kv_len + 1, 2 * kv_len):
+        want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5, window=window)
+        got = O.from_bits(run_attention(dev, c, q, start, kv, 1, kv_len, 2, "bf16", window=window), "bf16")
+        assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "bf16", kv_len, dim, 127 * c.vs.max())).all()
+    c.free()
+
+
 def test_append_then_attend_as_a_request_runs(dev):
     """A prompt in two chunks and then tokens one by one, q / k norm and rotation included: every step against attention
     over the values that the cache then holds, and the cache against the keys that went in."""
