@@ -94,8 +94,8 @@ __device__ __forceinline__ Row row_of(const Args& a, int64_t row, float top) {
   r.top = top;
   const float t = a.temperature ? a.temperature[row] : 1.0f;
   r.greedy = !(t > 0.0f);
-  r.per = r.greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(t);
-  r.per8 = static_cast<float>(fmin(r.per * 8.0, 3e38));
+  r.per = r.greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(fmaxf(t, 4.70197740e-38f));   // 2^-124: per8 is finite
+  r.per8 = static_cast<float>(r.per * 8.0);
   const int k = a.top_k ? a.top_k[row] : 0;
   r.k = k > 0 && k < a.vocab ? k : 0;
   const float p = a.top_p ? a.top_p[row] : 1.0f;

@@ -54,8 +54,9 @@ def sample_f32_rows_i32(logits_ptr: int, uniform_ptr: int, out_ids_ptr: int, row
                         library: ctypes.CDLL | None = None, runtime: HipRuntime | None = None) -> None:
     """``logits`` float32 ``[rows, vocab_size]`` (0: packed rows), ``uniform`` float32 ``[rows]`` in 0 <= u < 1, int32
     ``out_ids`` and optionally float32 ``out_logprobs`` ``[rows]``. Settings are arrays ``[rows]`` (float32, ``top_k``
-    int32), each of which may be None; a temperature of 0 or less takes the highest logit. A row with nothing but
-    -infinity and NaN gives -1. The workspace (8-byte aligned) is scratch of the size ``sample_workspace_bytes`` gives;
+    int32), each of which may be None; a temperature of 0 or less takes the highest logit, one above 0 counts as at least
+    2^-124. A log-probability is that of the kept tokens' distribution, which the token was drawn from. A row with nothing
+    but -infinity and NaN gives -1. The workspace (8-byte aligned) is scratch of the size ``sample_workspace_bytes`` gives;
     calls that overlap in time need one each."""
     if _launch.VALIDATE:
         _check_shape(rows, vocab_size)

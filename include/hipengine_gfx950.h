@@ -965,7 +965,7 @@ int hipengine_gfx950_paged_attention_q8_workspace_bytes(int64_t tokens, int64_t 
  * with w < min_p (a min_p over 1 counts as 1).  out_ids is the first kept token, by index, up to which the kept weights
  * sum to more than u times their total; out_logprobs (or null) the log of its share.  The four settings are arrays
  * [rows], each of which may be null: 1, all, all, all.  A temperature of 0 (or less, or NaN) takes the first token of the
- * order, with log-probability 0.  Logits of -infinity and NaN are not there; a row of nothing else gives -1 and -infinity.
+ * order, with log-probability 0; one above 0 counts as at least 2^-124.  Logits of -infinity and NaN are not there; a row of nothing else gives -1 and -infinity.
  * `workspace`: scratch, 8-byte aligned, of the size that the function below gives; calls that overlap in time need one
  * each.  Results do not depend on timing. */
 int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t logits_stride, const float* uniform,

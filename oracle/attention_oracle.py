@@ -175,6 +175,7 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, accu
     order = there[np.lexsort((there, -l[there]))]
     if not temperature > 0:
         return {int(order[0]): (0.0, 0.0)}
+    temperature = max(float(temperature), 2.0 ** -124)
     if top_k > 0:
         order = order[:top_k]
     w = np.exp(np.maximum((l[order] - l[order[0]]) / np.float64(temperature), -5000))

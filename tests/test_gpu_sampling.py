@@ -34,7 +34,7 @@ def run(dev, logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p
 
 
 def check(dev, logits, uniform, **settings):
-    stride = settings.pop("stride", None)
+    stride, borders = settings.pop("stride", None), settings.pop("borders", 0)
     ids, logprobs = run(dev, logits, uniform, stride=stride, **settings)
     at = lambda v, r: v if v is None or np.ndim(v) == 0 else v[r]  # noqa: E731
     open_rows = 0
@@ -51,7 +51,7 @@ def check(dev, logits, uniform, **settings):
             assert logprobs[r] == lo
     # of the statement alone: the test decides. In a flat row of 10^5 tokens 2^-22 of the total is a fortieth of a token, at
     # top-p's border and at the token's, above and below: a tenth of such rows is open
-    assert open_rows <= max(1, len(logits) // 2)
+    assert open_rows <= max(1, len(logits) // 2, borders)
 
 
 SETTINGS = [
@@ -129,6 +129,20 @@ def test_masked_infinite_and_nan_logits(dev):
     u = np.array([0.3, 0.3, 0.9, 0.51, 0.7, 0.2, 0.99, 0.613], np.float32)
     for settings in (dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.9), dict(min_p=0.01), dict(temperature=0.0)):
         check(dev, logits, u, **settings)
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-38, 2.0 ** -124, 3e38, np.inf])
+@pytest.mark.parametrize("settings", [dict(), dict(min_p=0.5), dict(top_p=0.5), dict(top_k=2)], ids=str)
+def test_extreme_temperatures(dev, temperature, settings):
+    """Rows whose logits differ by the least there is, by ordinary amounts and by the most."""
+    rows = np.zeros((3, 5), np.float32)
+    rows[0] = np.float32(2.0 ** -126) - np.arange(5, dtype=np.float32) * np.float32(2.0 ** -149)
+    rows[1] = [1.0, 3.0, 3.0, -2.0, 0.5]
+    rows[2] = [3e38, -3e38, 0.0, 3e38, 1.0]
+    for u in (0.1, 0.45, 0.8):
+        # (float32(0.8) is 4/5 + 2^-26: at the border of five equal weights, which the rows have at the highest
+        # temperatures, both answers are within 2^-22)
+        check(dev, rows, [u] * 3, temperature=temperature, borders=3 if u == 0.8 else 0, **settings)
 
 
 def test_uniform_ends(dev):
