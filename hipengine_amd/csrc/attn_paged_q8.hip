@@ -39,8 +39,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2v __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-constexpr int WAVES = 4;               // of attention_keys_kernel
-constexpr int ROW_WAVES = 4;           // of attention_rows_kernel, each with 32 rows
+constexpr int WAVES = 4;               // of a workgroup (of attention_rows_kernel also twice as many)
 constexpr int MAX_KV = 1 << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEVER = -3e38f;        // a maximum before any key: finite, so that differences to it are no NaN
@@ -60,8 +59,8 @@ struct AttnArgs {
   int group;              // query heads per KV head
   int q_heads;
   int window;
-  int splits;             // chunks of keys
-  int chunk;              // blocks of 32 keys in a chunk
+  int splits;             // most chunks of keys
+  int chunk;              // fewest blocks of 32 keys in a chunk
   float* part_acc;        // [splits][tokens * q_heads][D]
   float* part_ml;         // [splits][tokens * q_heads][2]
 };
@@ -103,6 +102,10 @@ struct Sight {
   __device__ __forceinline__ int limit(int query) const { return min(max(kv_len - q_len + query + 1, 0), kv_len); }
   __device__ __forceinline__ int lower(int query) const { return window > 0 ? max(kv_len - q_len + query + 1 - window, 0) : 0; }
 };
+
+// Blocks in each of a tile's chunks, from the blocks that it sees: the announced lengths only say how many chunks there may
+// be, so that a call captured for the longest cache cuts a short one as finely.
+__device__ __forceinline__ int chunk_of(const AttnArgs& a, int blocks) { return max((blocks + a.splits - 1) / a.splits, a.chunk); }
 
 // One column: a row of queries as the matrix instruction's second operand (lane (column, half) holds dims 32 i + 16 half +
 // 8 b .. + 7 of piece 2 i + b), and what goes with it.
@@ -315,8 +318,9 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
   const int lim_first = sight.limit(first_q), lo_last = sight.lower(last_q);
   int blk = sight.lower(first_q) >> 5, blk_end = (sight.limit(last_q) + 31) >> 5;
   if (a.splits > 1) {
-    blk += split * a.chunk;
-    if (split + 1 < a.splits) blk_end = min(blk_end, blk + a.chunk);   // the last chunk takes what a longer cache than announced holds
+    const int chunk = chunk_of(a, blk_end - blk);
+    blk += split * chunk;
+    blk_end = min(blk_end, blk + chunk);
   }
   f16v acc[KC];
 #pragma unroll
@@ -431,9 +435,9 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 // and not taken: eight waves (half the conversions a wave, but two waves a SIMD) 735 us; products of the next block behind
 // the softmax of this one (250 registers, two waves a SIMD) 765 to 780 us; 64 rows a wave 1053 us; K and V converted by
 // every wave from registers 899 us; wave priorities around the products or the softmax, no difference.
-template <int D, int KIND>
-__global__ void __launch_bounds__(ROW_WAVES * 64, D <= 128 ? 3 : 2) attention_rows_kernel(AttnArgs a) {
-  constexpr int W = ROW_WAVES, TILE = 32 * W;
+template <int D, int KIND, int W>
+__global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kernel(AttnArgs a) {
+  constexpr int TILE = 32 * W;
   constexpr int KC = D / 32, PIECES = 2 * KC;          // operand pieces of K, and of V; a 16-byte load gives two of them
   constexpr int LOADS = 2 * KC, MINE = LOADS / W;      // of a block: K's, then V's
   __shared__ h8 lds_k[2][PIECES][64];
@@ -450,8 +454,9 @@ __global__ void __launch_bounds__(ROW_WAVES * 64, D <= 128 ? 3 : 2) attention_ro
   int blk = sight.lower(tile0 / a.group) >> 5;
   int blk_end = (sight.limit((min(tile0 + TILE, n_rows) - 1) / a.group) + 31) >> 5;
   if (a.splits > 1) {
-    blk += split * a.chunk;
-    if (split + 1 < a.splits) blk_end = min(blk_end, blk + a.chunk);
+    const int chunk = chunk_of(a, blk_end - blk);
+    blk += split * chunk;
+    blk_end = min(blk_end, blk + chunk);
   }
   const int lim_first = sight.limit(min(row0, n_rows - 1) / a.group);
   const int lo_last = sight.lower((min(row0 + 32, n_rows) - 1) / a.group);
@@ -590,8 +595,9 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   // The chunks that a workgroup ran for this row: as the attention kernel laid them for the row's tile.
   const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
   const int row = query * a.group + q_head % a.group;
-  const int blocks = max(((sight.limit(query) + 31) >> 5) - (sight.lower(row / tile_rows * tile_rows / a.group) >> 5), 0);
-  const int splits = min((blocks + a.chunk - 1) / a.chunk, a.splits);
+  const int tile0 = row / tile_rows * tile_rows, last_q = (min(tile0 + tile_rows, static_cast<int>(rows.count) * a.group) - 1) / a.group;
+  const int first = sight.lower(tile0 / a.group) >> 5, chunk = chunk_of(a, ((sight.limit(last_q) + 31) >> 5) - first);
+  const int blocks = max(((sight.limit(query) + 31) >> 5) - first, 0), splits = (blocks + chunk - 1) / chunk;
   const int64_t at = (rows.first + query) * a.q_heads + q_head, pitch = a.tokens * a.q_heads;
   float m = NEVER;
   for (int s = lane; s < splits; s += 64) m = fmaxf(m, a.part_ml[2 * (s * pitch + at)]);
@@ -639,6 +645,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
 // How a call is cut: decided from sizes alone, so that the workspace can be sized before the call.
 struct Plan {
   bool keys;          // few rows: the waves of a workgroup share them and split keys
+  int waves;
   int tile_rows;
   int64_t tiles;
   int most_splits;    // what the workspace is sized for: no fewer for fewer keys
@@ -647,29 +654,49 @@ struct Plan {
 
 constexpr int CUS = 256;
 
+// What rows are cut into, and keys where the rows alone are too few.
+void cut(Plan& p, int64_t rows, int64_t blocks, int64_t heads, int64_t slots, int64_t least) {
+  p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
+  const int64_t groups = heads * p.tiles, most = (blocks + least - 1) / least;
+  int64_t splits = !p.keys && groups >= CUS ? 1 : (slots + groups - 1) / groups;
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  p.most_splits = static_cast<int>(splits);
+  p.chunk = static_cast<int>((blocks + splits - 1) / splits);
+  p.splits = p.chunk > 0 ? static_cast<int>((blocks + p.chunk - 1) / p.chunk) : 1;
+  if (p.keys) p.chunk = static_cast<int>(least);
+}
+
 Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t window) {
   Plan p;
   const int64_t rows = max_q * (q_heads / kv_heads);
   p.keys = rows <= 64;
-  p.tile_rows = p.keys ? 32 : 32 * ROW_WAVES;
-  p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
   // Keys that a tile can see.
   int64_t span = max_kv;
   if (window > 0 && window + max_q + 31 < span) span = window + max_q + 31;
   int64_t blocks = (span + 31) / 32;
   if (blocks < (max_kv + 31) / 32) ++blocks;      // (a window may begin anywhere in a block)
   // Two workgroups a CU.  With a workgroup a CU from the rows alone, prompts are not split (they would be joined for less
-  // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts).  A part has at least 16 blocks, and
-  // where waves share its keys at least 256 KB of them: a single token behind 600 others (19 blocks of 128) takes 14.4 us
-  // undivided and 17.3 us in two parts and the joining of them, behind 32768 others 22 us in 32 parts and 26 us in 64.
-  const int64_t groups = batch * kv_heads * p.tiles;
-  int64_t splits = !p.keys && groups >= CUS ? 1 : (2 * CUS + groups - 1) / groups;
-  const int64_t least = p.keys ? 4096 / dim : 16, most = (blocks + least - 1) / least;
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  p.most_splits = static_cast<int>(splits);
-  p.chunk = static_cast<int>((blocks + splits - 1) / splits);
-  p.splits = static_cast<int>((blocks + p.chunk - 1) / p.chunk);
+  // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts).  A part of a prompt has at least
+  // LEAST_ROWS and one of few rows, whose keys four waves share, at least LEAST_KEYS: a single token behind 600 others (19
+  // blocks of 128) takes 14.4 us undivided and 17.3 us in two parts and the joining of them, behind 32768 others 22 us in
+  // 32 parts and 26 us in 64; 512 tokens of D 128 (16 blocks) 23 us undivided and 35 us in two, of D 256 40 and 38 us.
+  const int64_t heads = batch * kv_heads, LEAST_KEYS = 4096 / dim, LEAST_ROWS = 2048 / dim;
+  p.waves = WAVES;
+  p.tile_rows = p.keys ? 32 : 32 * WAVES;
+  cut(p, rows, blocks, heads, 2 * CUS, p.keys ? LEAST_KEYS : LEAST_ROWS);
+  if (!p.keys && dim == 256) {
+    // Eight waves convert a block for twice the rows. Of D 256 a CU holds as many of them either way (of smaller D not: 3
+    // workgroups of four), and they win once there is nearly a workgroup for every CU: 3 chunks of 512 tokens 129 us
+    // against 154, 1024 tokens 48 against 52, but 512 tokens 42 against 38.
+    Plan wide = p;
+    wide.waves = 2 * WAVES;
+    wide.tile_rows = 64 * WAVES;
+    cut(wide, rows, blocks, heads, CUS, LEAST_ROWS);
+    const int most = p.most_splits > wide.most_splits ? p.most_splits : wide.most_splits;   // (a window may decide otherwise)
+    if (heads * wide.tiles * wide.splits >= CUS * 3 / 4) p = wide;
+    p.most_splits = most;
+  }
   return p;
 }
 
@@ -690,8 +717,13 @@ int64_t workspace_of(int splits, int64_t tokens, int64_t q_heads, int64_t dim) {
 template <int D, int KIND>
 int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64_t kv_heads, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.tiles), static_cast<unsigned>(batch * p.splits));
-  if (p.keys) hipLaunchKernelGGL((attention_keys_kernel<D, KIND>), grid, dim3(WAVES * 64), 0, stream, a);
-  else hipLaunchKernelGGL((attention_rows_kernel<D, KIND>), grid, dim3(ROW_WAVES * 64), 0, stream, a);
+  if (p.keys) {
+    hipLaunchKernelGGL((attention_keys_kernel<D, KIND>), grid, dim3(WAVES * 64), 0, stream, a);
+  } else if (p.waves == WAVES) {
+    hipLaunchKernelGGL((attention_rows_kernel<D, KIND, WAVES>), grid, dim3(WAVES * 64), 0, stream, a);
+  } else if constexpr (D == 256) {
+    hipLaunchKernelGGL((attention_rows_kernel<D, KIND, 2 * WAVES>), grid, dim3(2 * WAVES * 64), 0, stream, a);
+  }
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
   const int64_t out_rows = max_q * a.q_heads;

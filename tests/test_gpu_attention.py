@@ -381,6 +381,9 @@ ATTENTION = [
     (128, 1, 8, 64, [1], [9000], 4000, "bf16"),
     (128, 1, 8, 64, [150], [4000], 0, "bf16"),
     (128, 1, 8, 64, [150], [4000], 2500, "fp16"),
+    (256, 2, 8, 128, [200, 64, 0, 331], [200, 1100, 0, 1331], 0, "bf16"),              # workgroups of eight waves, in parts
+    (256, 4, 8, 32, [20] * 63 + [9], list(range(15, 78)) + [9], 0, "fp16"),            # and undivided
+    (256, 4, 8, 32, [20] * 63 + [9], list(range(15, 78)) + [9], 17, "bf16"),
 ]
 
 
@@ -491,6 +494,21 @@ def test_attention_refuses_a_small_workspace(dev):
                                  workspace_ptr=ptr, workspace_bytes=size)
     assert (dev.get(bufs[1], np.uint8, (8 * 128 * 2,)) == 0xA5).all()
     dev.free(*bufs)
+    c.free()
+
+
+@pytest.mark.parametrize("rows,lens", [([1, 2], [3000, 70]), ([3, 150], [40, 2100])])
+def test_attention_announced_for_a_longer_cache_than_there_is(dev, rows, lens):
+    """As a graph does that was captured for the longest cache: the keys are cut into parts by the lengths that there are."""
+    rng = np.random.default_rng(78)
+    dim, heads, group = 128, 1, 4
+    c = Cache(dev, rng, lens, 64, heads, dim)
+    start, kv = _ragged(rows), np.array(lens, np.int32)
+    q = O.round_to(rng.standard_normal((sum(rows), heads * group, dim)), "fp16")
+    want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5)
+    for max_kv in (max(lens), 20000, 1 << 20, 1 << 30):
+        got = O.from_bits(run_attention(dev, c, q, start, kv, max(rows), max_kv, heads * group, "fp16"), "fp16")
+        assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "fp16", max(lens), dim, 127 * c.vs.max())).all()
     c.free()
 
 
