@@ -34,6 +34,7 @@ constexpr int LIST = 16384;
 constexpr int FEW = 128;
 constexpr int NOTHING = 8 * 42;          // from this bin on a weight is less than 2^-40
 constexpr int CACHED = 2048;             // tokens of a list that pass 4 keeps in LDS
+constexpr int LINE = 32;
 constexpr int64_t MAX_VOCAB = 1 << 22;   // 1024 chunks; 2^22 weights of 2^40 stay under 2^63
 constexpr int MAX_CHUNKS = static_cast<int>(MAX_VOCAB / CHUNK);
 
@@ -53,12 +54,11 @@ struct Args {
   int cap;                    // tokens that a row's list holds
   // workspace
   uint64_t* best;             // [rows][chunks] key << 32 | ~index of the chunk's first token in the order
-  uint64_t* sums;             // [rows][chunks]
+  uint64_t* sums;             // [rows][chunks] weight of a chunk, where nothing is cut
+  uint64_t* before;           // [rows][chunks][BINS] weight, or with top-k number, of a chunk's tokens in the bins before one
   Cut* cuts;                  // [rows]
-  uint64_t* bin_weight;       // [rows][BINS]
   uint64_t* list;             // [rows][cap] key << 32 | ~index
-  uint32_t* bin_count;        // [rows][BINS]
-  uint32_t* listed;           // [rows]
+  uint32_t* listed;           // [rows], a line each: the chunks' additions to one line wait for each other
 };
 
 // The order as one number, higher is earlier: the logit's bits made to order like unsigned integers, then the index
@@ -105,6 +105,10 @@ __device__ __forceinline__ Row row_of(const Args& a, int64_t row, float top) {
   return r;
 }
 __device__ __forceinline__ bool cuts(const Row& r) { return r.k > 0 || r.p < 1.0 || r.octaves < __builtin_inf(); }
+
+// A logit as it counts: infinity as the largest number.  What is below MINUS (or NaN) cannot be chosen.
+constexpr float MINUS = -3.4028234663852886e+38f;
+__device__ __forceinline__ float finite(float l) { return fminf(l, -MINUS); }
 
 // Octaves below the largest weight, exactly enough for weights and for min-p.
 __device__ __forceinline__ double depth(const Row& r, float l) {
@@ -167,7 +171,7 @@ __device__ __forceinline__ void load_chunk(const Args& a, int64_t row, int chunk
   }
 }
 
-// Pass 1; also clears what pass 2 adds to.
+// Pass 1; also clears what pass 3 adds to.
 __global__ void __launch_bounds__(THREADS) sample_max_kernel(Args a) {
   __shared__ uint64_t lds[THREADS / 64];
   const int64_t row = blockIdx.y;
@@ -182,18 +186,13 @@ __global__ void __launch_bounds__(THREADS) sample_max_kernel(Args a) {
   }
   v = block_max<THREADS>(v, lds);
   if (threadIdx.x == 0) a.best[row * a.chunks + chunk] = v;
-  for (int i = chunk * THREADS + threadIdx.x; i < BINS; i += a.chunks * THREADS) {
-    a.bin_weight[row * BINS + i] = 0;
-    a.bin_count[row * BINS + i] = 0;
-  }
-  if (chunk == 0 && threadIdx.x == 0) a.listed[row] = 0;
+  if (chunk == 0 && threadIdx.x == 0) a.listed[row * LINE] = 0;
 }
 
 // Pass 2.
 __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
   __shared__ uint64_t lds[THREADS / 64];
   __shared__ unsigned long long weights[BINS];
-  __shared__ uint32_t counts[BINS];
   const int64_t row = blockIdx.y;
   const int chunk = blockIdx.x;
   float l[16];
@@ -206,27 +205,37 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
   best = block_max<THREADS>(best, lds);
   const Row r = row_of(a, row, logit_of(best));
   if (best == 0 || r.greedy || !cuts(r)) return;
-  // With top-k the border is found by counting, else by weight: one atomic a token.
+  // With top-k the border is found by counting, else by weight: one addition a token.
   const bool count = r.k > 0;
-  for (int i = threadIdx.x; i < BINS; i += THREADS) { weights[i] = 0; counts[i] = 0; }
+  for (int i = threadIdx.x; i < BINS; i += THREADS) weights[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const uint64_t o = order_of(l[i], 0);
-    if (o == 0) continue;
-    const float x = logit_of(o);
+    if (!(l[i] >= MINUS)) continue;
+    const float x = finite(l[i]);
     const int bin = bin_of(r, x);
     if (count) {
-      atomicAdd(&counts[bin], 1u);
+      atomicAdd(&weights[bin], 1ull);
     } else if (bin < NOTHING) {
       atomicAdd(&weights[bin], static_cast<unsigned long long>(weight(depth(r, x))));
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < BINS; i += THREADS) {
-    if (counts[i]) atomicAdd(&a.bin_count[row * BINS + i], counts[i]);
-    if (weights[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&a.bin_weight[row * BINS + i]), weights[i]);
+  // Sums over the bins, as the next kernel needs them for the row (it adds the chunks') and pass 4 for the chunk.
+  const int b = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t first = weights[b], own = first + weights[b + 1];
+  uint64_t run = own;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
+    if (lane >= off) run += o;
   }
+  if (lane == 63) lds[wave] = run;
+  __syncthreads();
+  run -= own;
+  for (int w = 0; w < wave; ++w) run += lds[w];
+  const uint64_t before[2] = {run, run + first};
+  __builtin_memcpy(__builtin_assume_aligned(a.before + (row * a.chunks + chunk) * BINS + b, 8), before, 16);
 }
 
 enum Mode : int { ALL, BOUND, PREFIX, FULL };
@@ -245,10 +254,13 @@ __device__ __forceinline__ uint64_t border(double p, uint64_t total) {   // smal
   return static_cast<uint64_t>(ceil(p * static_cast<double>(total)));
 }
 
-// Between passes 2 and 3: one wave a row, 8 bins a lane.
-__global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
+// Between passes 2 and 3: one workgroup a row adds up the chunks, two neighbouring bins a thread and every fourth chunk;
+// then one wave looks for the borders, 8 bins a lane.
+__global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
+  constexpr int PARTS = LAST / (BINS / 2);
+  __shared__ uint64_t before[PARTS][BINS];
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x & 63;
   uint64_t best = 0;
   for (int c = lane; c < a.chunks; c += 64) {
     const uint64_t o = a.best[row * a.chunks + c];
@@ -262,74 +274,57 @@ __global__ void __launch_bounds__(64) sample_cut_kernel(Args a) {
   const Row r = row_of(a, row, logit_of(best));
   Cut cut{best, 0, 0, ALL, BINS, BINS, 0};
   if (best != 0 && !r.greedy && cuts(r)) {
-    uint64_t w[8], ws = 0;
-    uint32_t c[8], cs = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      w[i] = a.bin_weight[row * BINS + lane * 8 + i];
-      c[i] = a.bin_count[row * BINS + lane * 8 + i];
-      ws += w[i];
-      cs += c[i];
+    const int pair = 2 * (threadIdx.x % (BINS / 2)), part = threadIdx.x / (BINS / 2);
+    uint64_t sum[2] = {0, 0};
+#pragma unroll 8
+    for (int c = part; c < a.chunks; c += PARTS) {
+      uint64_t v[2];
+      __builtin_memcpy(v, __builtin_assume_aligned(a.before + (row * a.chunks + c) * BINS + pair, 8), 16);
+      sum[0] += v[0];
+      sum[1] += v[1];
     }
-    uint64_t wi = ws;          // inclusive prefix over lanes
-    uint32_t ci = cs;
+    before[part][pair] = sum[0];
+    before[part][pair + 1] = sum[1];
+    __syncthreads();
+    if (threadIdx.x < BINS) {
+      uint64_t all = 0;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint64_t wo = __shfl_up(static_cast<unsigned long long>(wi), off);
-      const uint32_t co = __shfl_up(ci, off);
-      if (lane >= off) { wi += wo; ci += co; }
+      for (int p = 0; p < PARTS; ++p) all += before[p][threadIdx.x];
+      before[0][threadIdx.x] = all;
     }
-    const uint64_t total = __shfl(static_cast<unsigned long long>(wi), 63);
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    // (Nothing in the last bin counts: it has no weight, and top-k is taken to end in it where it is not reached before.)
+    auto up_to = [&](int bin) { return before[0][min(bin + 1, BINS - 1)]; };
+    const uint64_t total = before[0][BINS - 1];
     const uint64_t need = r.p < 1.0 ? border(r.p, total) : ~uint64_t{0};
-    // Bins below min_bin lie on this side of min-p's border whatever float32 makes of it, those above max_bin behind it.
-    const int min_bin = static_cast<int>(fmin(r.octaves * 8.0 * (1.0 - 1e-6), BINS - 1.0));
-    const int max_bin = static_cast<int>(fmin(r.octaves * 8.0 * (1.0 + 1e-6), BINS - 1.0));
     // First bin up to which k tokens, or `need`, are reached.
-    int k_bin = BINS - 1, p_bin = BINS - 1;
-    uint64_t wp = wi - ws;
-    uint32_t cp = ci - cs;
+    const uint64_t goal = r.k > 0 ? static_cast<uint64_t>(r.k) : need;
+    int reached = BINS - 1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      wp += w[i];
-      cp += c[i];
-      if (r.k > 0 && cp >= static_cast<uint32_t>(r.k)) k_bin = min(k_bin, lane * 8 + i);
-      if (r.k == 0 && wp >= need) p_bin = min(p_bin, lane * 8 + i);
-    }
+    for (int i = 0; i < 8; ++i)
+      if (up_to(lane * 8 + i) >= goal) reached = min(reached, lane * 8 + i);
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      k_bin = min(k_bin, __shfl_xor(k_bin, off));
-      p_bin = min(p_bin, __shfl_xor(p_bin, off));
-    }
+    for (int off = 1; off < 64; off <<= 1) reached = min(reached, __shfl_xor(reached, off));
     cut.need = need;
     if (r.k > 0) {
       // A border in the last bin cuts nothing (its weights are 0); what top-p and min-p then cut is not known by weight.
-      cut.bin = cut.last = k_bin;
-      uint32_t to = ci - cs, up_to = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        to += c[i];
-        if (lane * 8 + i == k_bin) up_to = to;
-      }
-      up_to = __shfl(up_to, k_bin >> 3);
-      if (k_bin < BINS - 1) cut.mode = up_to <= static_cast<uint32_t>(a.cap) ? PREFIX : FULL;
+      cut.bin = cut.last = reached;
+      if (reached < BINS - 1) cut.mode = up_to(reached) <= static_cast<uint64_t>(a.cap) ? PREFIX : FULL;
       else cut.mode = r.p < 1.0 || r.octaves < __builtin_inf() ? FULL : ALL;
     } else {
-      cut.bin = min(p_bin, min_bin);
-      cut.last = p_bin < min_bin ? p_bin : min(p_bin, max_bin);
-      cut.reached = p_bin <= cut.last;
-      uint64_t before = 0;
-      wp = wi - ws;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (lane * 8 + i == cut.bin) before = wp;
-        wp += w[i];
-      }
-      cut.above = __shfl(static_cast<unsigned long long>(before), cut.bin >> 3);
+      // Bins below min_bin lie on this side of min-p's border whatever float32 makes of it, those above max_bin behind it.
+      const int min_bin = static_cast<int>(fmin(r.octaves * 8.0 * (1.0 - 1e-6), BINS - 1.0));
+      const int max_bin = static_cast<int>(fmin(r.octaves * 8.0 * (1.0 + 1e-6), BINS - 1.0));
+      cut.bin = min(reached, min_bin);
+      cut.last = reached < min_bin ? reached : min(reached, max_bin);
+      cut.reached = reached <= cut.last;
+      cut.above = before[0][cut.bin];
       cut.mode = cut.bin < BINS - 1 ? BOUND : ALL;
     }
     if (cut.mode == ALL) cut.bin = cut.last = BINS;
   }
-  if (lane == 0) a.cuts[row] = cut;
+  if (threadIdx.x == 0) a.cuts[row] = cut;
 }
 
 // Pass 3.
@@ -347,30 +342,28 @@ __global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
   __syncthreads();
   // A logit that lies more than half a bin behind B's end is passed over by one comparison.
   const float floor = cut.last < BINS - 1 ? static_cast<float>(static_cast<double>(r.top) - (cut.last + 1.5) * 0.125 / r.per)
-                                         : -__builtin_inff();
+                                         : MINUS;
   uint64_t sum = 0;
   uint32_t slot[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     slot[i] = ~0u;
-    if (!(l[i] >= floor)) continue;
-    const uint64_t o = order_of(l[i], 0);
-    if (o == 0) continue;
-    const float x = logit_of(o);
+    if (!(l[i] >= fmaxf(floor, MINUS))) continue;
+    const float x = finite(l[i]);
     const int bin = bin_of(r, x);
-    if (cut.mode != PREFIX && bin < cut.bin) {
+    if (cut.mode == ALL) {
       if (bin < NOTHING) sum += weight(depth(r, x));
-    } else if (bin <= cut.last) {
+    } else if ((cut.mode == PREFIX || bin >= cut.bin) && bin <= cut.last) {
       slot[i] = atomicAdd(&here, 1u);
     }
   }
-  if (cut.mode != PREFIX) {
+  if (cut.mode == ALL) {
     sum = block_sum<THREADS>(sum, lds);
     if (threadIdx.x == 0) a.sums[row * a.chunks + chunk] = sum;
   }
   __syncthreads();
   if (here == 0) return;
-  if (threadIdx.x == 0) base = atomicAdd(&a.listed[row], here);
+  if (threadIdx.x == 0) base = atomicAdd(&a.listed[row * LINE], here);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 16; ++i)
@@ -416,9 +409,14 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t be
     some |= v;
     all &= v;
   });
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    some |= __shfl_xor(static_cast<unsigned long long>(some), off);
+    all &= __shfl_xor(static_cast<unsigned long long>(all), off);
+  }
   if (threadIdx.x == 0) { d.some = 0; d.all = ~0ull; }
   __syncthreads();
-  if (all != ~uint64_t{0} || some != 0) {
+  if ((threadIdx.x & 63) == 0) {
     atomicOr(&d.some, static_cast<unsigned long long>(some));
     atomicAnd(&d.all, static_cast<unsigned long long>(all));
   }
@@ -576,7 +574,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     }
     return;
   }
-  const uint32_t listed = a.listed[row];
+  const uint32_t listed = a.listed[row * LINE];
   if (listed > static_cast<uint32_t>(a.cap)) cut.mode = FULL;   // (BOUND: the bin did not fit the list)
   const float* logits = a.logits + row * a.stride;
   if (cut.mode == PREFIX && listed <= FEW) {
@@ -585,6 +583,11 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   }
   Tokens t{r, cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr, nullptr, logits,
            cut.mode == FULL ? a.vocab : cut.mode == ALL ? 0 : static_cast<int>(listed)};
+  const bool by_chunk = cut.mode == ALL || cut.mode == BOUND;
+  if (by_chunk) {
+    for (int c = threadIdx.x; c < a.chunks; c += LAST)
+      chunk_sum[c] = cut.mode == ALL ? a.sums[row * a.chunks + c] : a.before[(row * a.chunks + c) * BINS + cut.bin];
+  }
   if (t.list && t.n <= CACHED) {
     for (int i = threadIdx.x; i < t.n; i += LAST) {
       const uint64_t o = t.list[i];
@@ -593,8 +596,8 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     }
     t.list = kept_order;
     t.weights = kept_weight;
-    __syncthreads();
   }
+  __syncthreads();
   const uint64_t above = cut.mode == BOUND ? cut.above : 0;
   auto self = [](uint64_t o) { return o; };
 
@@ -633,10 +636,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   auto weight_left = [&](uint64_t o, auto w_of) { return stays(o) ? w_of() : uint64_t{0}; };
 
   uint64_t total = 0;
-  const bool by_chunk = cut.mode == ALL || cut.mode == BOUND;
   if (by_chunk) {
-    for (int c = threadIdx.x; c < a.chunks; c += LAST) chunk_sum[c] = a.sums[row * a.chunks + c];
-    __syncthreads();
     t.each([&](uint64_t o, auto w_of) {
       const uint64_t w = weight_left(o, w_of);
       if (w) atomicAdd(&chunk_sum[index_of(o) / CHUNK], static_cast<unsigned long long>(w));
@@ -718,7 +718,7 @@ bool shape_ok(int64_t rows, int64_t vocab) { return rows > 0 && rows <= 65535 &&
 int64_t chunks_of(int64_t vocab) { return (vocab + CHUNK - 1) / CHUNK; }
 int64_t cap_of(int64_t vocab) { return vocab < LIST ? vocab : LIST; }
 int64_t workspace_of(int64_t rows, int64_t vocab) {
-  return rows * (16 * chunks_of(vocab) + static_cast<int64_t>(sizeof(Cut)) + 12 * BINS + 8 * cap_of(vocab) + 4);
+  return rows * ((16 + 8 * BINS) * chunks_of(vocab) + static_cast<int64_t>(sizeof(Cut)) + 8 * cap_of(vocab) + 4 * LINE);
 }
 
 }  // namespace
@@ -742,21 +742,20 @@ extern "C" int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t
   const int64_t chunks = chunks_of(vocab_size);
   uint64_t* w = static_cast<uint64_t*>(workspace);
   Args a{logits, logits_stride, uniform, temperature, top_k, top_p, min_p, out_ids, out_logprobs, static_cast<int>(vocab_size),
-         static_cast<int>(chunks), static_cast<int>(cap_of(vocab_size)), nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
-  a.best = w;
+         static_cast<int>(chunks), static_cast<int>(cap_of(vocab_size)), nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  a.before = w;
+  a.best = a.before + rows * chunks * BINS;
   a.sums = a.best + rows * chunks;
   a.cuts = reinterpret_cast<Cut*>(a.sums + rows * chunks);
-  a.bin_weight = reinterpret_cast<uint64_t*>(a.cuts + rows);
-  a.list = a.bin_weight + rows * BINS;
-  a.bin_count = reinterpret_cast<uint32_t*>(a.list + rows * a.cap);
-  a.listed = a.bin_count + rows * BINS;
+  a.list = reinterpret_cast<uint64_t*>(a.cuts + rows);
+  a.listed = reinterpret_cast<uint32_t*>(a.list + rows * a.cap);
   const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(rows)), threads(THREADS);
   hipLaunchKernelGGL(sample_max_kernel, grid, threads, 0, stream, a);
   hipError_t err = hipGetLastError();
   if (err != hipSuccess) return static_cast<int>(err);
   hipLaunchKernelGGL(sample_histogram_kernel, grid, threads, 0, stream, a);
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
-  hipLaunchKernelGGL(sample_cut_kernel, dim3(static_cast<unsigned>(rows)), dim3(64), 0, stream, a);
+  hipLaunchKernelGGL(sample_cut_kernel, dim3(static_cast<unsigned>(rows)), dim3(LAST), 0, stream, a);
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
   hipLaunchKernelGGL(sample_collect_kernel, grid, threads, 0, stream, a);
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
