@@ -3,8 +3,9 @@
 //
 // KV cache. A page holds page_size tokens (a power of two, 32 or more) of every KV head; inside a (page, head) the
 // tokens lie in blocks of 32, and a block has one float32 scale for K and one for V. Values are bytes 128 + q with q in
-// -127..127 (excess-128 needs no sign extension on the way to fp16: a byte under zeros is a subnormal fp16 number). Both block layouts are the operand order of
-// v_mfma_f32_32x32x16_f16, so that a wave's 16-byte loads are contiguous and nothing passes through LDS:
+// -127..127 (excess-128 needs no sign extension on the way to fp16: byte b under 0x64 is the fp16 number 1024 + b). Both
+// block layouts are the operand order of v_mfma_f32_32x32x16_f16, so that a wave's 16-byte loads are contiguous and
+// nothing has to be reordered:
 //   K block  [D/16][32 tokens][16 dims]   lane (token, half) reads dims 16 (2i + half) .. + 15 as one load
 //   V block  [D][32 places]               token t at place (t & 3) | (t >> 3 & 3) << 2 | (t >> 2 & 1) << 4:
 //                                         lane (dim, half) reads the 16 tokens that the 32x32 accumulator of

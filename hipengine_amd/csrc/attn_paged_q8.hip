@@ -4,15 +4,16 @@
 // load of K and V and a tile has no empty rows between queries.  Row r's query sits at place kv_len - q_len + query and
 // sees the keys up to it (and, with a window, no further back than window - 1); a row that sees none gives zeros.
 //
-// One wave holds 32 (or 64) rows and walks over blocks of 32 keys, keeping for each row the running maximum and sum of
-// the softmax.  It computes transposed products on v_mfma_f32_32x32x16_f16: S^T = K Q^T (rows keys, columns queries) and
-// O^T += V^T P^T.  A lane then owns one query column: maximum, sum and rescaling are per lane, the accumulator of S^T is
-// already P^T's operand (the cache's V layout is in the accumulator's key order), and K, V and P never pass through LDS.
+// One wave holds 32 rows and walks once over blocks of 32 keys, keeping for each row a reference near its maximum and the
+// sum of the softmax.  It computes transposed products on v_mfma_f32_32x32x16_f16: S^T = K Q^T (rows keys, columns
+// queries) and O^T += V^T P^T.  A lane then owns one query column: maximum, sum and rescaling are per lane, the
+// accumulator of S^T is already P^T's operand (the cache's V layout is in the accumulator's key order), and P never
+// passes through LDS.
 //
 // Numbers.  K and V are whole numbers up to 127, exact in fp16.  q is bf16 or fp16: bf16 rows are divided by the power
 // of two of their largest magnitude, which makes them exact in fp16 down to 2^-24 of it.  Products and sums are float32.
-// P is rounded to fp16 (relative 2^-11): it lies in 0 .. 2^15 around a reference that follows the running maximum, and
-// the sum of the softmax adds the rounded values, so the rounding does not move the weights' total.
+// P is rounded to fp16 (relative 2^-11): it lies in 0 .. 2^15, 2^7 at the reference, and the sum of the softmax adds the
+// rounded values, so the rounding does not move the weights' total.
 //
 // Scales.  K's block scale goes into the softmax's argument.  V's goes into P: with w = p * v_scale, w = exp2(s + log2
 // v_scale - m) for a maximum m over that sum, O = (sum w v_int) / (sum w / v_scale) - one more constant per block in an
@@ -43,8 +44,8 @@ constexpr int WAVES = 4;               // of a workgroup (of attention_rows_kern
 constexpr int MAX_KV = 1 << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEVER = -3e38f;        // a maximum before any key: finite, so that differences to it are no NaN
-constexpr float HEADROOM = 8.0f;       // log2 by which a row's maximum may pass its reference before rows are rescaled
-constexpr float RANGE = 32768.0f;      // of a sum of P above which the reference is moved (fp16 ends at 65504)
+constexpr float HEADROOM = 8.0f;       // attention_keys_kernel: log2 by which a row's maximum may pass its reference
+constexpr float RANGE = 32768.0f;      // attention_rows_kernel: sum of P above which it is moved (fp16 ends at 65504)
 constexpr float OFFSET = 7.0f;         // log2 of P at the reference: P <= 2^15, and fp16's least step is 2^-31 of it
 
 struct AttnArgs {
@@ -302,8 +303,11 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const SeqRows& r
 }
 
 // ---- few rows: the four waves of a workgroup share 32 rows and take blocks of keys in turn --------------------------
-// grid (KV heads, row tiles, batch * splits).  Bound by the cache's bytes: a wave converts a block's 64 * D bytes in 1200
-// clocks, four times what HBM delivers in that time.
+// grid (KV heads, row tiles, batch * splits).  Nothing passes through LDS but the waves' join at the end.  With work for
+// every CU it is bound by the cache's bytes, K's and V's next blocks being on their way while one is worked on: 8
+// sequences of about 30000 tokens, 8 heads of 128, 276 MB in 63 us, 4.4 TB/s (a large copy: 4.8); 64 of about 7500 of
+// D 64, 278 MB in 59 us.  A short call is bound by its chain of loads (lengths, page, block) and two launches: 600 tokens
+// 10.4 us.
 template <int D, int KIND>
 __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_kernel(AttnArgs a) {
   constexpr int KC = D / 32;           // 16-byte loads of K a lane, and tiles of 32 dims of V
@@ -430,8 +434,9 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 // There is no running maximum: P is taken against the reference as it is, and only where a column's sum says that P has
 // grown out of its range is the maximum looked for, the reference moved and P taken again.
 //
-// What bounds it: 8192 tokens, 40 / 8 heads of 128, 695 us: vector instructions 60 % and matrix instructions 45 % of the
-// cycles, at 2.1 GHz. Four waves, three such workgroups a CU, let one wave's softmax run in another's products.  Measured
+// What bounds it: 8192 tokens, 40 / 8 heads of 128, 695 us (0.99 PFLOP/s; a large bf16 product: 1.37): vector instructions
+// 60 % and matrix instructions 45 % of the cycles, at 2.1 GHz.  Of D 256 it is the occupancy, two waves a SIMD, which wait
+// for each other at the barrier: 0.6 PFLOP/s.  Four waves, three such workgroups a CU, let one wave's softmax run in another's products.  Measured
 // and not taken: eight waves (half the conversions a wave, but two waves a SIMD) 735 us; products of the next block behind
 // the softmax of this one (250 registers, two waves a SIMD) 765 to 780 us; 64 rows a wave 1053 us; K and V converted by
 // every wave from registers 899 us; wave priorities around the products or the softmax, no difference.

@@ -5,7 +5,8 @@
 //   over the first rotary_dim values of a head, pairs (i, i + rotary_dim / 2) or (2i, 2i + 1); the rest stays
 //
 // Statistics and rotation are in float32 and the angle in float64; the result is rounded once, on its way out.
-// A launch reads and writes every value once, so HBM (or, for a few tokens, the launch) is what bounds it.
+// A launch reads and writes every value once, so HBM (or, for a few tokens, the launch) is what bounds it: 8191 tokens of
+// 18 heads of 256 in bf16, 151 MB, take 31 to 36 us, a copy of them 32; one token 3.4 us.
 
 #include "attn_common.hpp"
 
