@@ -143,6 +143,7 @@ def _manifest_field(manifest: Path, name: str) -> str | None:
 
 
 _loaded: dict[Path, ctypes.CDLL] = {}
+_IN_TREE = LIB_DIR / OUTPUT_NAME   # one object, which remembers its hash: every launch asks for the library
 
 
 def load_library(path: Path | None = None) -> ctypes.CDLL:
@@ -152,7 +153,7 @@ def load_library(path: Path | None = None) -> ctypes.CDLL:
     library's per-device set-up runs here, so that every entry point is graph-capturable from its
     first launch."""
     in_tree = path is None
-    target = Path(path) if path else LIB_DIR / OUTPUT_NAME
+    target = Path(path) if path else _IN_TREE
     lib = _loaded.get(target)
     if lib is None:
         if not target.exists():
