@@ -84,6 +84,19 @@ __device__ __forceinline__ float logit_of(uint64_t order) {
 }
 __device__ __forceinline__ int index_of(uint64_t order) { return static_cast<int>(~static_cast<uint32_t>(order)); }
 
+// A row's settings as they are given.  Loaded at once and first of all: which array is null is only asked afterwards (the
+// uniform numbers stand in for it), since loads behind branches wait for each other, a microsecond each in a short call.
+struct Given {
+  float t, p, m;
+  int k;
+};
+__device__ __forceinline__ Given given(const Args& a, int64_t row) {
+  auto at = [&](const void* from) { return static_cast<const uint32_t*>(from ? from : a.uniform)[row]; };
+  const uint32_t t = at(a.temperature), k = at(a.top_k), p = at(a.top_p), m = at(a.min_p);
+  return {a.temperature ? bits_to_float(t) : 1.0f, a.top_p ? bits_to_float(p) : 1.0f, a.min_p ? bits_to_float(m) : 0.0f,
+          a.top_k ? static_cast<int>(k) : 0};
+}
+
 struct Row {
   float top;             // largest logit
   double per;            // octaves of weight per unit of logit: log2(e) / temperature
@@ -94,19 +107,16 @@ struct Row {
   double octaves;        // min-p's border; infinity: none
 };
 
-__device__ __forceinline__ Row row_of(const Args& a, int64_t row, float top) {
+__device__ __forceinline__ Row row_of(const Args& a, const Given& g, float top) {
   Row r;
   r.top = top;
-  const float t = a.temperature ? a.temperature[row] : 1.0f;
+  const float t = g.t;
   r.greedy = !(t > 0.0f);
   r.per = r.greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(fmaxf(t, 4.70197740e-38f));   // 2^-124: per8 is finite
   r.per8 = static_cast<float>(r.per * 8.0);
-  const int k = a.top_k ? a.top_k[row] : 0;
-  r.k = k > 0 && k < a.vocab ? k : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
-  r.p = p < 1.0f ? fmax(static_cast<double>(p), 0.0) : 1.0;
-  const float m = a.min_p ? a.min_p[row] : 0.0f;
-  r.octaves = m > 0.0f ? -log2(fmin(static_cast<double>(m), 1.0)) : __builtin_inf();
+  r.k = g.k > 0 && g.k < a.vocab ? g.k : 0;
+  r.p = g.p < 1.0f ? fmax(static_cast<double>(g.p), 0.0) : 1.0;
+  r.octaves = g.m > 0.0f ? -log2(fmin(static_cast<double>(g.m), 1.0)) : __builtin_inf();
   return r;
 }
 __device__ __forceinline__ bool cuts(const Row& r) { return r.k > 0 || r.p < 1.0 || r.octaves < __builtin_inf(); }
@@ -201,6 +211,7 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
   const int64_t row = blockIdx.y;
   const int chunk = blockIdx.x;
   float l[16];
+  const Given g = given(a, row);
   load_chunk(a, row, chunk, l);
   uint64_t best = 0;
   for (int c = threadIdx.x; c < a.chunks; c += THREADS) {
@@ -208,7 +219,7 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
     best = o > best ? o : best;
   }
   best = block_max<THREADS>(best, lds);
-  const Row r = row_of(a, row, logit_of(best));
+  const Row r = row_of(a, g, logit_of(best));
   if (best == 0 || r.greedy || !cuts(r)) return;
   // With top-k the border is found by counting, else by weight: one addition a token.
   const bool count = r.k > 0;
@@ -247,6 +258,7 @@ enum Mode : int { ALL, BOUND, PREFIX, FULL };
 
 // What is known of a row before pass 3.
 struct Cut {
+  Row row;
   uint64_t best;        // the first token in the order; 0: there is none
   uint64_t above;       // weight of the bins before B (BOUND)
   uint64_t need;        // top-p: a token stays if less than this lies before it (BOUND)
@@ -266,7 +278,18 @@ __global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
   __shared__ uint64_t before[PARTS][BINS];
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 63;
-  uint64_t best = 0;
+  const Given g = given(a, row);
+  uint64_t best = 0, sum[2] = {0, 0};
+  const int pair = 2 * (threadIdx.x % (BINS / 2)), part = threadIdx.x / (BINS / 2);
+  if (g.t > 0.0f) {                                    // (what no histogram was written for is not used)
+#pragma unroll 8
+    for (int c = part; c < a.chunks; c += PARTS) {
+      uint64_t v[2];
+      __builtin_memcpy(v, __builtin_assume_aligned(a.before + (row * a.chunks + c) * BINS + pair, 8), 16);
+      sum[0] += v[0];
+      sum[1] += v[1];
+    }
+  }
   for (int c = lane; c < a.chunks; c += 64) {
     const uint64_t o = a.best[row * a.chunks + c];
     best = o > best ? o : best;
@@ -276,18 +299,9 @@ __global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
     const uint64_t o = __shfl_xor(static_cast<unsigned long long>(best), off);
     best = o > best ? o : best;
   }
-  const Row r = row_of(a, row, logit_of(best));
-  Cut cut{best, 0, 0, ALL, BINS, BINS, 0};
+  const Row r = row_of(a, g, logit_of(best));
+  Cut cut{r, best, 0, 0, ALL, BINS, BINS, 0};
   if (best != 0 && !r.greedy && cuts(r)) {
-    const int pair = 2 * (threadIdx.x % (BINS / 2)), part = threadIdx.x / (BINS / 2);
-    uint64_t sum[2] = {0, 0};
-#pragma unroll 8
-    for (int c = part; c < a.chunks; c += PARTS) {
-      uint64_t v[2];
-      __builtin_memcpy(v, __builtin_assume_aligned(a.before + (row * a.chunks + c) * BINS + pair, 8), 16);
-      sum[0] += v[0];
-      sum[1] += v[1];
-    }
     before[part][pair] = sum[0];
     before[part][pair + 1] = sum[1];
     __syncthreads();
@@ -341,7 +355,7 @@ __global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
   float l[16];
   load_chunk(a, row, chunk, l);
   const Cut cut = a.cuts[row];
-  const Row r = row_of(a, row, logit_of(cut.best));
+  const Row r = cut.row;
   if (cut.best == 0 || r.greedy || cut.mode == FULL) return;
   if (threadIdx.x == 0) here = 0;
   __syncthreads();
@@ -487,16 +501,14 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t be
   return prefix;
 }
 
-__device__ __forceinline__ void answer(const Args& a, int64_t row, const Row& r, const float* logits, int id, uint64_t total) {
+__device__ __forceinline__ void answer(const Args& a, int64_t row, const Row& r, int id, float l, uint64_t total) {
   a.ids[row] = id;
   if (!a.logprobs) return;
-  const float l = fminf(logits[id] + 0.0f, 3.4028234663852886e+38f);
   a.logprobs[row] = static_cast<float>(-((static_cast<double>(r.top) - static_cast<double>(l)) * r.per +
                                          log2(static_cast<double>(total)) - 40.0) * 0.6931471805599453);
 }
 
-__device__ __forceinline__ uint64_t target_of(const Args& a, int64_t row, uint64_t total) {
-  const float u = a.uniform[row];
+__device__ __forceinline__ uint64_t target_of(float u, uint64_t total) {
   const uint64_t target = static_cast<uint64_t>((u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0) * static_cast<double>(total));
   return target < total ? target : total - 1;      // the largest weight is 2^40, so there is a total
 }
@@ -509,8 +521,8 @@ struct Few {
   unsigned long long total, kept;
 };
 
-__device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const Row& r, const uint64_t* list, int n,
-                                              const float* logits, Few& f) {
+__device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const Row& r, const uint64_t* list, int n, float u,
+                                              Few& f) {
   const int i = threadIdx.x % FEW, part = threadIdx.x / FEW;
   const bool mine = i < n;
   uint64_t order = 0, w = 0;
@@ -556,8 +568,9 @@ __device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const 
     if (static_cast<uint32_t>(f.order[j]) > static_cast<uint32_t>(order)) lower += f.weight[j];   // (complement of the index)
   if (mine && lower) atomicAdd(&f.by_index[i], static_cast<unsigned long long>(lower));
   __syncthreads();
-  const uint64_t target = target_of(a, row, f.kept);
-  if (part == 0 && keep && f.by_index[i] <= target && target < f.by_index[i] + w) answer(a, row, r, logits, index_of(order), f.kept);
+  const uint64_t target = target_of(u, f.kept);
+  if (part == 0 && keep && f.by_index[i] <= target && target < f.by_index[i] + w)
+    answer(a, row, r, index_of(order), logit_of(order), f.kept);
 }
 
 __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
@@ -570,8 +583,10 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   __shared__ uint64_t rest;
   const int64_t row = blockIdx.x;
   Cut cut = a.cuts[row];
+  const uint32_t listed = a.listed[row * LINE];
+  const float u = a.uniform[row];
   const uint64_t best = cut.best;
-  const Row r = row_of(a, row, logit_of(best));
+  const Row r = cut.row;
   if (best == 0 || r.greedy) {
     if (threadIdx.x == 0) {
       a.ids[row] = best ? index_of(best) : -1;
@@ -579,11 +594,10 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     }
     return;
   }
-  const uint32_t listed = a.listed[row * LINE];
   if (listed > static_cast<uint32_t>(a.cap)) cut.mode = FULL;   // (BOUND: the bin did not fit the list)
   const float* logits = a.logits + row * a.stride;
   if (cut.mode == PREFIX && listed <= FEW) {
-    choose_of_few(a, row, r, a.list + row * a.cap, static_cast<int>(listed), logits, few);
+    choose_of_few(a, row, r, a.list + row * a.cap, static_cast<int>(listed), u, few);
     return;
   }
   Tokens t{r, cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr, nullptr, logits,
@@ -652,8 +666,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     t.each([&](uint64_t o, auto w_of) { total += weight_left(o, w_of); });
   }
   total = block_sum<LAST>(total, lds);
-  const uint64_t target = target_of(a, row, total);
-  int id;
+  const uint64_t target = target_of(u, total);
   if (by_chunk) {
     if (threadIdx.x < 64) {
       const int lane = threadIdx.x;
@@ -679,14 +692,17 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
     // The chunk's tokens, 4 neighbours a thread, in index order.
     const int first = chosen_chunk * CHUNK + static_cast<int>(threadIdx.x) * 4;
     uint64_t w[4], s = 0;
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = first + i < a.vocab ? logits[first + i] : __builtin_nanf("");
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       w[i] = 0;
-      const uint64_t o = first + i < a.vocab ? order_of(logits[first + i], first + i) : 0;
+      const uint64_t o = order_of(x[i], first + i);
       if (o) {
-        const float x = logit_of(o);
-        const int bin = bin_of(r, x);
-        if (bin < cut.bin || (bin <= cut.last && stays(o))) w[i] = weight(depth(r, x));
+        const float l = logit_of(o);
+        const int bin = bin_of(r, l);
+        if (bin < cut.bin || (bin <= cut.last && stays(o))) w[i] = weight(depth(r, l));
       }
       s += w[i];
     }
@@ -705,16 +721,14 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
       uint64_t at = run - s;
       int i = 0;
       while (i < 3 && !(at + w[i] > rest)) at += w[i++];
-      digits.digit = first + i;
+      answer(a, row, r, first + i, finite(x[i]), total);
     }
-    __syncthreads();
-    id = digits.digit;
   } else {
     // Smaller indices first: the complement of the index orders them so, in 24 bits.
     const uint64_t v = walk(t, digits, target, [](uint64_t o) { return o & 0xFFFFFFu; }, weight_left);
-    id = static_cast<int>(~static_cast<uint32_t>(v) & 0xFFFFFFu);
+    const int id = static_cast<int>(~static_cast<uint32_t>(v) & 0xFFFFFFu);
+    if (threadIdx.x == 0) answer(a, row, r, id, finite(logits[id]), total);
   }
-  if (threadIdx.x == 0) answer(a, row, r, logits, id, total);
 }
 
 constexpr int BAD = static_cast<int>(hipErrorInvalidValue);
