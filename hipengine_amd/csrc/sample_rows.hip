@@ -40,6 +40,10 @@ constexpr int FEW = 128;
 constexpr int NOTHING = 8 * 42;          // from this bin on a weight is less than 2^-40
 constexpr int CACHED = 2048;             // tokens of a list that pass 4 keeps in LDS
 constexpr int LINE = 32;
+// rows * chunks^2 up to which pass 3's workgroups each find their row's borders (and read all its sums): one launch less
+// (8 rows of 32003: 25.3 us against 27.2, 1 of 151936: 25.9 against 27.3, 4 of 151936: no difference, 16 of 151936: 33
+// against 30, 1 of 10^6: 38 against 35).
+constexpr int64_t SHARED_CUTS = 4096;
 constexpr int64_t MAX_VOCAB = 1 << 22;   // 1024 chunks; 2^22 weights of 2^40 stay under 2^63
 constexpr int MAX_CHUNKS = static_cast<int>(MAX_VOCAB / CHUNK);
 
@@ -271,12 +275,18 @@ __device__ __forceinline__ uint64_t border(double p, uint64_t total) {   // smal
   return static_cast<uint64_t>(ceil(p * static_cast<double>(total)));
 }
 
-// Between passes 2 and 3: one workgroup a row adds up the chunks, two neighbouring bins a thread and every fourth chunk;
-// then one wave looks for the borders, 8 bins a lane.
-__global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
-  constexpr int PARTS = LAST / (BINS / 2);
-  __shared__ uint64_t before[PARTS][BINS];
-  const int64_t row = blockIdx.x;
+// Between passes 2 and 3 a workgroup of N threads adds up the row's chunks, two neighbouring bins a thread; then one wave
+// looks for the borders, 8 bins a lane.
+template <int N>
+struct CutLds {
+  static constexpr int PARTS = N / (BINS / 2);
+  uint64_t before[PARTS][BINS];
+  Cut cut;
+};
+template <int N>
+__device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& lds) {
+  constexpr int PARTS = CutLds<N>::PARTS;
+  auto& before = lds.before;
   const int lane = threadIdx.x & 63;
   const Given g = given(a, row);
   uint64_t best = 0, sum[2] = {0, 0};
@@ -305,13 +315,15 @@ __global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
     before[part][pair] = sum[0];
     before[part][pair + 1] = sum[1];
     __syncthreads();
-    if (threadIdx.x < BINS) {
-      uint64_t all = 0;
+    if constexpr (PARTS > 1) {
+      if (threadIdx.x < BINS) {
+        uint64_t all = 0;
 #pragma unroll
-      for (int p = 0; p < PARTS; ++p) all += before[p][threadIdx.x];
-      before[0][threadIdx.x] = all;
+        for (int p = 0; p < PARTS; ++p) all += before[p][threadIdx.x];
+        before[0][threadIdx.x] = all;
+      }
+      __syncthreads();
     }
-    __syncthreads();
     if (threadIdx.x >= 64) return;
     // (Nothing in the last bin counts: it has no weight, and top-k is taken to end in it where it is not reached before.)
     auto up_to = [&](int bin) { return before[0][min(bin + 1, BINS - 1)]; };
@@ -343,18 +355,31 @@ __global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
     }
     if (cut.mode == ALL) cut.bin = cut.last = BINS;
   }
-  if (threadIdx.x == 0) a.cuts[row] = cut;
+  if (threadIdx.x == 0) lds.cut = cut;
 }
 
-// Pass 3.
+__global__ void __launch_bounds__(LAST) sample_cut_kernel(Args a) {
+  __shared__ CutLds<LAST> cut_lds;
+  find_cut(a, blockIdx.x, cut_lds);
+  if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut_lds.cut;
+}
+
+// Pass 3; with CUT every workgroup finds the borders for itself.
+template <bool CUT>
 __global__ void __launch_bounds__(THREADS) sample_collect_kernel(Args a) {
   __shared__ uint64_t lds[THREADS / 64];
+  __shared__ CutLds<CUT ? THREADS : BINS / 2> cut_lds;
   __shared__ uint32_t here, base;
   const int64_t row = blockIdx.y;
   const int chunk = blockIdx.x;
   float l[16];
   load_chunk(a, row, chunk, l);
-  const Cut cut = a.cuts[row];
+  if constexpr (CUT) {
+    find_cut(a, row, cut_lds);
+    __syncthreads();
+    if (chunk == 0 && threadIdx.x == 0) a.cuts[row] = cut_lds.cut;
+  }
+  const Cut cut = CUT ? cut_lds.cut : a.cuts[row];
   const Row r = cut.row;
   if (cut.best == 0 || r.greedy || cut.mode == FULL) return;
   if (threadIdx.x == 0) here = 0;
@@ -521,14 +546,13 @@ struct Few {
   unsigned long long total, kept;
 };
 
-__device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const Row& r, const uint64_t* list, int n, float u,
-                                              Few& f) {
+__device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const Row& r, uint64_t order, int n, float u, Few& f) {
   const int i = threadIdx.x % FEW, part = threadIdx.x / FEW;
   const bool mine = i < n;
-  uint64_t order = 0, w = 0;
+  uint64_t w = 0;
   double y = 0.0;
+  if (!mine) order = 0;
   if (mine) {
-    order = list[i];
     y = depth(r, logit_of(order));
     w = weight(y);
   }
@@ -585,6 +609,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   Cut cut = a.cuts[row];
   const uint32_t listed = a.listed[row * LINE];
   const float u = a.uniform[row];
+  const uint64_t order = a.list[row * a.cap + min(static_cast<int>(threadIdx.x) % FEW, a.cap - 1)];   // (for choose_of_few)
   const uint64_t best = cut.best;
   const Row r = cut.row;
   if (best == 0 || r.greedy) {
@@ -597,7 +622,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
   if (listed > static_cast<uint32_t>(a.cap)) cut.mode = FULL;   // (BOUND: the bin did not fit the list)
   const float* logits = a.logits + row * a.stride;
   if (cut.mode == PREFIX && listed <= FEW) {
-    choose_of_few(a, row, r, a.list + row * a.cap, static_cast<int>(listed), u, few);
+    choose_of_few(a, row, r, order, static_cast<int>(listed), u, few);
     return;
   }
   Tokens t{r, cut.mode == BOUND || cut.mode == PREFIX ? a.list + row * a.cap : nullptr, nullptr, logits,
@@ -774,9 +799,13 @@ extern "C" int hipengine_gfx950_sample_f32_rows_i32(const float* logits, int64_t
   if (err != hipSuccess) return static_cast<int>(err);
   hipLaunchKernelGGL(sample_histogram_kernel, grid, threads, 0, stream, a);
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
-  hipLaunchKernelGGL(sample_cut_kernel, dim3(static_cast<unsigned>(rows)), dim3(LAST), 0, stream, a);
-  if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
-  hipLaunchKernelGGL(sample_collect_kernel, grid, threads, 0, stream, a);
+  if (rows * chunks * chunks <= SHARED_CUTS) {
+    hipLaunchKernelGGL(sample_collect_kernel<true>, grid, threads, 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(sample_cut_kernel, dim3(static_cast<unsigned>(rows)), dim3(LAST), 0, stream, a);
+    if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
+    hipLaunchKernelGGL(sample_collect_kernel<false>, grid, threads, 0, stream, a);
+  }
   if ((err = hipGetLastError()) != hipSuccess) return static_cast<int>(err);
   hipLaunchKernelGGL(sample_choose_kernel, dim3(static_cast<unsigned>(rows)), dim3(LAST), 0, stream, a);
   return static_cast<int>(hipGetLastError());
