@@ -144,13 +144,45 @@ __device__ __forceinline__ uint64_t weight(double y) {   // 2^-y * 2^40, downwar
   return (static_cast<uint64_t>(m) << 18) >> min(static_cast<int>(n) + 128 - static_cast<int>(e >> 23), 63);
 }
 
+// 64-bit values of a wave joined, or summed up to each lane, by moves between registers: through LDS every step would wait
+// some hundred clocks, and a short call consists of such steps. All lanes have to be active.
+__device__ __forceinline__ uint64_t whole(uint32_t lo, uint32_t hi) { return (static_cast<uint64_t>(hi) << 32) | lo; }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {      // 0 where nothing comes from
+  const int lo = static_cast<int>(v), hi = static_cast<int>(v >> 32);
+  return whole(__builtin_amdgcn_update_dpp(0, lo, CTRL, ROWS, 0xf, false), __builtin_amdgcn_update_dpp(0, hi, CTRL, ROWS, 0xf, false));
+}
+template <typename F>
+__device__ __forceinline__ uint64_t wave_join(uint64_t v, F f) {
+  v = f(v, moved<DPP_QUAD_XOR1, 0xf>(v));
+  v = f(v, moved<DPP_QUAD_XOR2, 0xf>(v));
+  v = f(v, moved<DPP_ROW_HALF_MIRROR, 0xf>(v));
+  v = f(v, moved<0x140, 0xf>(v));                            // row_mirror
+  const uint32_t lo = static_cast<uint32_t>(v), hi = static_cast<uint32_t>(v >> 32);
+  const auto l = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), h = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+  v = f(whole(l[0], h[0]), whole(l[1], h[1]));
+  const uint32_t lo2 = static_cast<uint32_t>(v), hi2 = static_cast<uint32_t>(v >> 32);
+  const auto l2 = __builtin_amdgcn_permlane32_swap(lo2, lo2, false, false), h2 = __builtin_amdgcn_permlane32_swap(hi2, hi2, false, false);
+  return f(whole(l2[0], h2[0]), whole(l2[1], h2[1]));
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+  return wave_join(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
+  return wave_join(v, [](uint64_t a, uint64_t b) { return a + b; });
+}
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {  // with the lane's own
+  v += moved<0x111, 0xf>(v);                                 // row_shr 1, 2, 4, 8
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);                                 // lane 15 of rows 0 and 2 to rows 1 and 3
+  return v + moved<0x143, 0xc>(v);                           // lane 31 to rows 2 and 3
+}
+
 template <int N>
 __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* lds) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(v), off);
-    v = o > v ? o : v;
-  }
+  v = wave_max(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -160,8 +192,7 @@ __device__ __forceinline__ uint64_t block_max(uint64_t v, uint64_t* lds) {
 }
 template <int N>
 __device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* lds) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(static_cast<unsigned long long>(v), off);
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -244,12 +275,7 @@ __global__ void __launch_bounds__(THREADS) sample_histogram_kernel(Args a) {
   // Sums over the bins, as the next kernel needs them for the row (it adds the chunks') and pass 4 for the chunk.
   const int b = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint64_t first = weights[b], own = first + weights[b + 1];
-  uint64_t run = own;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
-    if (lane >= off) run += o;
-  }
+  uint64_t run = wave_scan(own);
   if (lane == 63) lds[wave] = run;
   __syncthreads();
   run -= own;
@@ -304,11 +330,7 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
     const uint64_t o = a.best[row * a.chunks + c];
     best = o > best ? o : best;
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_xor(static_cast<unsigned long long>(best), off);
-    best = o > best ? o : best;
-  }
+  best = wave_max(best);
   const Row r = row_of(a, g, logit_of(best));
   Cut cut{r, best, 0, 0, ALL, BINS, BINS, 0};
   if (best != 0 && !r.greedy && cuts(r)) {
@@ -453,11 +475,8 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t be
     some |= v;
     all &= v;
   });
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    some |= __shfl_xor(static_cast<unsigned long long>(some), off);
-    all &= __shfl_xor(static_cast<unsigned long long>(all), off);
-  }
+  some = wave_join(some, [](uint64_t x, uint64_t y) { return x | y; });
+  all = wave_join(all, [](uint64_t x, uint64_t y) { return x & y; });
   if (threadIdx.x == 0) { d.some = 0; d.all = ~0ull; }
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {
@@ -490,12 +509,7 @@ __device__ __forceinline__ uint64_t walk(const Tokens& t, Digits& d, uint64_t be
       uint64_t w[4], s = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) { w[i] = d.weights[255 - 4 * lane - i]; s += w[i]; }
-      uint64_t run = s;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
-        if (lane >= off) run += o;
-      }
+      uint64_t run = wave_scan(s);
       const unsigned long long over = __ballot(run > before);
       const int owner = over ? __builtin_ctzll(over) : 63;
       if (lane == owner) {
@@ -577,14 +591,18 @@ __device__ __forceinline__ void choose_of_few(const Args& a, int64_t row, const 
   }
   __syncthreads();
   bool keep = mine && f.rank[i] < static_cast<uint32_t>(r.k);
-  if (part == 0 && keep) atomicAdd(&f.total, static_cast<unsigned long long>(w));
+  if (part == 0) {
+    const uint64_t sum = wave_sum(keep ? w : 0);
+    if ((threadIdx.x & 63) == 0) atomicAdd(&f.total, static_cast<unsigned long long>(sum));
+  }
   __syncthreads();
   const uint64_t need = r.p < 1.0 ? border(r.p, f.total) : ~uint64_t{0};
   keep = keep && (f.before[i] < need || f.rank[i] == 0) && y <= r.octaves;
   __syncthreads();
   if (part == 0) {
     if (!keep) f.weight[i] = 0;
-    else atomicAdd(&f.kept, static_cast<unsigned long long>(w));
+    const uint64_t sum = wave_sum(keep ? w : 0);
+    if ((threadIdx.x & 63) == 0) atomicAdd(&f.kept, static_cast<unsigned long long>(sum));
   }
   __syncthreads();
   uint64_t lower = 0;
@@ -698,12 +716,7 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
       uint64_t passed = 0;
       for (int c0 = 0; c0 < a.chunks; c0 += 64) {
         const uint64_t s = c0 + lane < a.chunks ? chunk_sum[c0 + lane] : 0;
-        uint64_t run = s;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
-          if (lane >= off) run += o;
-        }
+        const uint64_t run = wave_scan(s);
         const unsigned long long over = __ballot(passed + run > target);
         if (over) {
           const int owner = __builtin_ctzll(over);
@@ -731,13 +744,8 @@ __global__ void __launch_bounds__(LAST) sample_choose_kernel(Args a) {
       }
       s += w[i];
     }
-    uint64_t run = s;
+    uint64_t run = wave_scan(s);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint64_t o = __shfl_up(static_cast<unsigned long long>(run), off);
-      if (lane >= off) run += o;
-    }
     __syncthreads();
     if (lane == 63) lds[wave] = run;
     __syncthreads();
