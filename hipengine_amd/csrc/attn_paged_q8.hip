@@ -585,9 +585,9 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
 }
 
 // Joins the chunks of output rows: grid (rows a sequence / (4 / TEAM), batch); TEAM waves have a row and take its chunks in
-// turn, D / 64 dims a lane.  What bounds it is the time that a load takes: eight are on their way at once.  With more than
-// 8 chunks four waves join a row (40 rows of 64 chunks, one token behind 32768 others: 11.2 us with one wave a row, 5.4 with
-// four), else one (24576 rows of D 256 and 2 chunks: 13.2 us, with four 38.9).
+// turn, D / 64 dims a lane.  What bounds it is the time that a load takes, so for few rows, or many chunks, a row has four
+// waves: 40 rows of 64 chunks 4.0 us, 320 of up to 8 chunks 4.9 us, with a wave a row 11 and 5.8.  Many rows of few chunks
+// have enough loads on their way: 2560 rows of 2 or 3 chunks 5.2 us, 24576 of D 256 14.4 us, with four waves 9.9 and 39.
 template <int D, int KIND, int TEAM>
 __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   constexpr int V = D / 64;
@@ -618,12 +618,22 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
       l += a.part_ml[i + 1] * f;
     }
     const int n = min(splits - s0, 64);
-#pragma unroll 8
-    for (int k = wave % TEAM; k < n; k += TEAM) {
-      const float w = read_lane_f(f, k);
-      const float* src = a.part_acc + ((s0 + k) * pitch + at) * D + lane * V;
+    // A team's last chunks are asked for at once too (those behind the end are the last one again, at no weight); a wave that
+    // is one of thousands does better without.
+    constexpr int AHEAD = TEAM == 1 ? 1 : 8;
+#pragma unroll(TEAM == 1 ? 8 : 1)
+    for (int k0 = wave % TEAM; k0 < n; k0 += AHEAD * TEAM) {
+      float x[AHEAD][V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) o[v] = fmaf(src[v], w, o[v]);
+      for (int i = 0; i < AHEAD; ++i)
+        __builtin_memcpy(x[i], __builtin_assume_aligned(a.part_acc + ((s0 + min(k0 + i * TEAM, n - 1)) * pitch + at) * D + lane * V, 4 * V), 4 * V);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const bool there = k0 + i * TEAM < n;
+        const float w = there ? read_lane_f(f, k0 + i * TEAM) : 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = fmaf(there ? x[i][v] : 0.0f, w, o[v]);
+      }
     }
   }
 #pragma unroll
@@ -732,7 +742,7 @@ int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
   const int64_t out_rows = max_q * a.q_heads;
-  if (p.splits > 8)
+  if (p.splits > 8 || batch * out_rows <= 2048)
     hipLaunchKernelGGL((join_kernel<D, KIND, 4>), dim3(static_cast<unsigned>(out_rows), static_cast<unsigned>(batch)), dim3(256), 0, stream, a, p.tile_rows);
   else
     hipLaunchKernelGGL((join_kernel<D, KIND, 1>), dim3(static_cast<unsigned>((out_rows + 3) / 4), static_cast<unsigned>(batch)), dim3(256), 0, stream, a, p.tile_rows);

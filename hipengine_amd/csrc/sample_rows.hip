@@ -316,14 +316,20 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
   const int lane = threadIdx.x & 63;
   const Given g = given(a, row);
   uint64_t best = 0, sum[2] = {0, 0};
-  const int pair = 2 * (threadIdx.x % (BINS / 2)), part = threadIdx.x / (BINS / 2);
+  const int pair = 2 * (threadIdx.x % (BINS / 2)), part = __builtin_amdgcn_readfirstlane(threadIdx.x / (BINS / 2));
   if (g.t > 0.0f) {                                    // (what no histogram was written for is not used)
-#pragma unroll 8
-    for (int c = part; c < a.chunks; c += PARTS) {
-      uint64_t v[2];
-      __builtin_memcpy(v, __builtin_assume_aligned(a.before + (row * a.chunks + c) * BINS + pair, 8), 16);
-      sum[0] += v[0];
-      sum[1] += v[1];
+    constexpr int AHEAD = 16;                          // loads on their way, the last few too: not a loop over the rest
+    for (int c0 = part; c0 < a.chunks; c0 += AHEAD * PARTS) {
+      uint64_t v[AHEAD][2] = {};
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (c0 + i * PARTS < a.chunks)
+          __builtin_memcpy(v[i], __builtin_assume_aligned(a.before + (row * a.chunks + c0 + i * PARTS) * BINS + pair, 8), 16);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        sum[0] += v[i][0];
+        sum[1] += v[i][1];
+      }
     }
   }
   for (int c = lane; c < a.chunks; c += 64) {
