@@ -346,7 +346,7 @@ extern "C" int hipengine_gfx950_kv_append_q8(const void* k, const void* v, int32
                 head_dim))
     return BAD;
   if (!k || !v || in_kind < KIND_F32 || in_kind > KIND_F16 || tokens <= 0 || tokens > 0x7FFFFFFF || batch <= 0 ||
-      batch > MAX_UNITS / 2 || max_q_len <= 0 || !(eps >= 0.0f))
+      batch > 65535 || max_q_len <= 0 || !(eps >= 0.0f))
     return BAD;
   if (inv_freq ? (rotary_dim < 16 || rotary_dim > head_dim || rotary_dim % 16 != 0) : rotary_dim != 0) return BAD;
   const int64_t width = kv_heads * head_dim;
@@ -377,7 +377,7 @@ extern "C" int hipengine_gfx950_kv_read_q8(const uint8_t* k_cache, const uint8_t
                 head_dim))
     return BAD;
   if ((!k_out && !v_out) || out_kind < KIND_F32 || out_kind > KIND_F16 || tokens <= 0 || tokens > 0x7FFFFFFF || batch <= 0 ||
-      batch > MAX_UNITS / 2)
+      batch > 65535)
     return BAD;
   const int64_t width = kv_heads * head_dim;
   if (k_out_stride == 0) k_out_stride = width;

@@ -317,7 +317,7 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
   const Given g = given(a, row);
   uint64_t best = 0, sum[2] = {0, 0};
   const int pair = 2 * (threadIdx.x % (BINS / 2)), part = __builtin_amdgcn_readfirstlane(threadIdx.x / (BINS / 2));
-  if (g.t > 0.0f) {                                    // (what no histogram was written for is not used)
+  if (g.t > 0.0f && (g.k > 0 || g.p < 1.0f || g.m > 0.0f)) {   // (what no histogram was written for is not used)
     constexpr int AHEAD = 16;                          // loads on their way, the last few too: not a loop over the rest
     for (int c0 = part; c0 < a.chunks; c0 += AHEAD * PARTS) {
       uint64_t v[AHEAD][2] = {};

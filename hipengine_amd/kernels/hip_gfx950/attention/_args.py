@@ -32,6 +32,11 @@ def check_positive(**values: int) -> None:
             raise ValueError(f"{name} must be positive")
 
 
+def check_batch(batch: int) -> None:
+    if batch > 65535:
+        raise ValueError("batch must be at most 65535")
+
+
 def check_head_dim(head_dim: int) -> None:
     if head_dim not in HEAD_DIMS:
         raise ValueError("head_dim must be 64, 128 or 256")

@@ -25,6 +25,7 @@ from hipengine_amd.kernels.hip_gfx950.attention._args import (
     HEAD_DIMS,
     KINDS,
     are_pointers,
+    check_batch,
     check_head_dim,
     check_positive,
     check_rotation,
@@ -87,15 +88,16 @@ def kv_append_q8(cache: KVCacheQ8, k_ptr: int, v_ptr: int, page_table_ptr: int, 
     ``k_weight_ptr`` (float32 ``[head_dim]``) norms every key head, ``inv_freq_ptr`` rotates it at ``positions_ptr``
     (int64 ``[tokens]``; None: a token's place in its sequence). A block's scale grows to hold the new tokens, and its
     earlier tokens are rescaled then; a block whose first token is appended starts anew; bytes behind the new tokens
-    stay. A NaN or infinity makes its block's scale NaN until the block starts anew. No two sequences may append to the
-    same block in one call."""
+    stay. A NaN or infinity makes its block's scale NaN until the block starts anew. No block may be appended to under two
+    names in one call (two sequences, or a page twice in one table)."""
     width = cache.kv_heads * cache.head_dim
     if _launch.VALIDATE and not (
-            tokens > 0 and batch > 0 and max_q_len > 0 and table_stride > 0 and in_kind in KINDS and eps >= 0.0
+            tokens > 0 and 0 < batch <= 65535 and max_q_len > 0 and table_stride > 0 and in_kind in KINDS and eps >= 0.0
             and (k_stride == 0 or k_stride >= width) and (v_stride == 0 or v_stride >= width)
             and (16 <= rotary_dim <= cache.head_dim and rotary_dim & 15 == 0 if inv_freq_ptr else rotary_dim == 0)
             and are_pointers(k_ptr, v_ptr, page_table_ptr, q_start_ptr, kv_lens_ptr)):
         check_positive(tokens=tokens, batch=batch, max_q_len=max_q_len, table_stride=table_stride)
+        check_batch(batch)
         kind_of(in_kind, "in_kind")
         check_rotation(inv_freq_ptr, rotary_dim, cache.head_dim)
         check_stride("k_stride", k_stride, width)
@@ -120,10 +122,11 @@ def kv_read_q8(cache: KVCacheQ8, k_out_ptr: int | None, v_out_ptr: int | None, p
     cache read as zeros."""
     width = cache.kv_heads * cache.head_dim
     if _launch.VALIDATE and not (
-            tokens > 0 and batch > 0 and table_stride > 0 and out_kind in KINDS and (k_out_ptr or v_out_ptr)
+            tokens > 0 and 0 < batch <= 65535 and table_stride > 0 and out_kind in KINDS and (k_out_ptr or v_out_ptr)
             and (k_out_stride == 0 or k_out_stride >= width) and (v_out_stride == 0 or v_out_stride >= width)
             and are_pointers(page_table_ptr, row_start_ptr, kv_lens_ptr)):
         check_positive(tokens=tokens, batch=batch, table_stride=table_stride)
+        check_batch(batch)
         kind_of(out_kind, "out_kind")
         check_stride("k_out_stride", k_out_stride, width)
         check_stride("v_out_stride", v_out_stride, width)

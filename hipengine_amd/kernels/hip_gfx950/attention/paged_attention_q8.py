@@ -18,6 +18,7 @@ from hipengine_amd.kernels.hip_gfx950.attention._args import (
     F32,
     KINDS,
     are_pointers,
+    check_batch,
     check_head_dim,
     check_positive,
     check_stride,
@@ -32,8 +33,9 @@ _WORKSPACE_ARGS = [I64] * 7 + [ctypes.POINTER(I64)]
 
 def _check_shape(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int) -> None:
     check_positive(tokens=tokens, batch=batch, max_q_len=max_q_len, q_heads=q_heads, kv_heads=kv_heads)
-    if tokens > 1 << 26 or batch > 65535:
-        raise ValueError("tokens must be at most 2^26 and batch at most 65535")
+    check_batch(batch)
+    if tokens > 1 << 26:
+        raise ValueError("tokens must be at most 2^26")
     if max_kv_len < 0 or max_kv_len > 1 << 30:
         raise ValueError("max_kv_len must be 0 .. 2^30")
     if q_heads % kv_heads != 0 or q_heads > 4096:

@@ -898,6 +898,7 @@ int hipengine_gfx950_moe_tile_map(const int64_t* expert_start_compact, int64_t* 
  *   page_table      int32 [batch, table_stride] page numbers.  A number outside 0 .. pages - 1 is no page: tokens on it are
  *                   not written, read as zeros and not attended to.  Entries behind a sequence's end are not looked at.
  *   q_start         int32 [batch + 1]: sequence b's rows are q_start[b] .. q_start[b + 1] - 1
+ *   batch           at most 65535
  *   kv_lens         int32 [batch]: tokens in sequence b's cache, its rows of this call (the last ones) included.
  *                   A sequence may have no rows, and no tokens.
  *   max_q_len, max_kv_len  at least the longest sequence's rows / cached tokens (any larger value is right, too)
@@ -917,8 +918,8 @@ int hipengine_gfx950_qk_norm_rope(const void* q, const void* k, const float* q_w
  * sequence) and v to the cache, at places kv_lens[b] - rows .. kv_lens[b] - 1 of sequence b.  A block's scale grows to hold
  * the new tokens and its earlier tokens are rescaled then; a block whose first token is appended starts anew; bytes behind
  * the new tokens stay as they were.  Rows at negative places (more rows than kv_lens[b]) are left out.  A NaN or infinity
- * makes its block's scale NaN until the block starts anew.  Within one call no two sequences may append to the same
- * block: which one's tokens it then holds is not defined. */
+ * makes its block's scale NaN until the block starts anew.  Within one call no block may be appended to under two
+ * names (two sequences, or a page twice in one table): whose tokens it then holds is not defined. */
 int hipengine_gfx950_kv_append_q8(const void* k, const void* v, int32_t in_kind, int64_t k_stride, int64_t v_stride,
                                   const float* k_weight, const int64_t* positions, const float* inv_freq,
                                   int64_t rotary_dim, int32_t interleaved, float eps, float rope_scale, uint8_t* k_cache,

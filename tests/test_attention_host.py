@@ -65,7 +65,7 @@ APPEND = dict(k_ptr=16, v_ptr=16, page_table_ptr=16, table_stride=2, q_start_ptr
 @pytest.mark.parametrize("over", [
     {"tokens": 0}, {"batch": 0}, {"max_q_len": 0}, {"table_stride": 0}, {"k_ptr": 0}, {"v_ptr": None}, {"page_table_ptr": 0},
     {"q_start_ptr": 0}, {"kv_lens_ptr": 0}, {"in_kind": "int8"}, {"rotary_dim": 16}, {"inv_freq_ptr": 16, "rotary_dim": 8},
-    {"inv_freq_ptr": 16, "rotary_dim": 256}, {"k_stride": 100}, {"v_stride": -4}, {"eps": -1e-6},
+    {"inv_freq_ptr": 16, "rotary_dim": 256}, {"k_stride": 100}, {"v_stride": -4}, {"eps": -1e-6}, {"batch": 65536},
 ])
 def test_append_refusals(over):
     with pytest.raises(ValueError):
@@ -76,7 +76,7 @@ READ = dict(k_out_ptr=16, v_out_ptr=16, page_table_ptr=16, table_stride=2, row_s
 
 
 @pytest.mark.parametrize("over", [{"tokens": 0}, {"batch": 0}, {"table_stride": 0}, {"k_out_ptr": None, "v_out_ptr": 0},
-                                  {"out_kind": ""}, {"k_out_stride": 255}, {"row_start_ptr": 0}, {"kv_lens_ptr": None}])
+                                  {"out_kind": ""}, {"k_out_stride": 255}, {"batch": 65536}, {"row_start_ptr": 0}, {"kv_lens_ptr": None}])
 def test_read_refusals(over):
     with pytest.raises(ValueError):
         C.kv_read_q8(cache(), **(READ | over), library=Never())
@@ -138,7 +138,7 @@ def _append(**over):
 @pytest.mark.parametrize("over", [
     {"k": None}, {"v": None}, {"kind": 3}, {"ks": 10}, {"vs": -1}, {"rot": 32}, {"freq": 16, "rot": 8}, {"eps": -1.0}, {"kc": None},
     {"vc": 8193}, {"ksc": None}, {"vsc": None}, {"table": None}, {"ts": 0}, {"qs": None}, {"lens": None}, {"tokens": 0}, {"batch": 0},
-    {"batch": 1 << 40}, {"maxq": 0}, {"pages": 0}, {"pages": 1 << 31}, {"size": 48}, {"size": 16}, {"size": 1 << 21}, {"heads": 0},
+    {"batch": 65536}, {"batch": 1 << 40}, {"maxq": 0}, {"pages": 0}, {"pages": 1 << 31}, {"size": 48}, {"size": 16}, {"size": 1 << 21}, {"heads": 0},
     {"heads": 65536}, {"dim": 127}, {"tokens": 1 << 31}])
 def test_c_append_refuses(over):
     assert _append(**over) == 1
@@ -152,7 +152,7 @@ def _read(**over):
     return fn(*a.values())
 
 
-@pytest.mark.parametrize("over", [{"k": None, "v": None}, {"kind": 9}, {"ks": 255}, {"vs": 1}, {"tokens": 0}, {"batch": -1}, {"rs": None},
+@pytest.mark.parametrize("over", [{"k": None, "v": None}, {"kind": 9}, {"ks": 255}, {"vs": 1}, {"tokens": 0}, {"batch": -1}, {"batch": 65536}, {"rs": None},
                                   {"kc": 4104}, {"dim": 32}, {"size": 33}])
 def test_c_read_refuses(over):
     assert _read(**over) == 1
