@@ -131,12 +131,18 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// The first of the pairs that the head dims 8 * slot .. + 7 belong to (8 pairs, or 4 where interleaved).
+__device__ __forceinline__ int first_pair(int slot, int rotary_dim, bool interleaved) {
+  const int d0 = 8 * slot, pairs = rotary_dim >> 1;
+  return interleaved ? d0 >> 1 : d0 < pairs ? d0 : d0 - pairs;
+}
+
 // One head's RMS norm and rotation by the D / 8 neighbouring lanes that hold it, 8 values a lane (x: head dims 8 * slot ..).
-// `turn` holds (cos, sin) of the rotary_dim / 2 pairs.  rotary_dim is a multiple of 16, so a lane's 8 values lie on one
+// turn(i) gives (cos, sin) of the i-th pair from first_pair on.  rotary_dim is a multiple of 16, so a lane's 8 values lie on one
 // side of every border and their partners all in one other lane.
-template <int D>
-__device__ __forceinline__ void norm_rotate8(float (&x)[8], int slot, const float* __restrict__ weight, float eps,
-                                             const float2* turn, int rotary_dim, bool interleaved) {
+template <int D, typename Turn>
+__device__ __forceinline__ void norm_rotate8(float (&x)[8], int slot, const float* __restrict__ weight, float eps, Turn turn,
+                                             int rotary_dim, bool interleaved) {
   constexpr int LANES = D / 8;
   const int d0 = 8 * slot, pairs = rotary_dim >> 1;
   if (weight) {
@@ -153,7 +159,7 @@ __device__ __forceinline__ void norm_rotate8(float (&x)[8], int slot, const floa
   if (interleaved) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 cs = turn[(d0 >> 1) + i];
+      const float2 cs = turn(i);
       const float a = x[2 * i], b = x[2 * i + 1];
       x[2 * i] = fmaf(a, cs.x, -b * cs.y);
       x[2 * i + 1] = fmaf(b, cs.x, a * cs.y);
@@ -161,12 +167,14 @@ __device__ __forceinline__ void norm_rotate8(float (&x)[8], int slot, const floa
   } else {
     const bool low = d0 < pairs;
     const int other = low ? d0 + pairs : d0 - pairs, lane = (static_cast<int>(threadIdx.x) & 63 & ~(LANES - 1)) + (other >> 3);
-    const float2* cs = turn + (low ? d0 : other);
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], lane);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i].x, (low ? -y[i] : y[i]) * cs[i].y);
+    for (int i = 0; i < 8; ++i) {
+      const float2 cs = turn(i);
+      x[i] = fmaf(x[i], cs.x, (low ? -y[i] : y[i]) * cs.y);
+    }
   }
 }
 

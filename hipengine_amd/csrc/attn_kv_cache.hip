@@ -107,121 +107,155 @@ __device__ __forceinline__ uint32_t requantize(uint32_t byte, float ratio) {
   return static_cast<uint32_t>(static_cast<int>(rintf(static_cast<float>(static_cast<int>(byte) - 128) * ratio)) + 128);
 }
 
+// The largest of a wave.
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t u) {
+  u = max(u, static_cast<uint32_t>(dpp_i<DPP_QUAD_XOR1>(static_cast<int>(u))));
+  u = max(u, static_cast<uint32_t>(dpp_i<DPP_QUAD_XOR2>(static_cast<int>(u))));
+  u = max(u, static_cast<uint32_t>(dpp_i<DPP_ROW_HALF_MIRROR>(static_cast<int>(u))));
+  u = max(u, static_cast<uint32_t>(dpp_i<0x140>(static_cast<int>(u))));     // row_mirror
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = max(r[0], r[1]);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return max(h[0], h[1]);
+}
+
+constexpr int V_ROW = KV_BLOCK + 4;      // bytes of a V block's row in LDS: 8 lanes work on rows 8 apart
+
 template <int D>
 struct AppendLds {
-  static constexpr int ROWS = THREADS / (D / 8), PAD = D + 4;
-  float x[KV_BLOCK * PAD];
-  float2 turn[ROWS][D / 2];
-  int64_t position[KV_BLOCK];
-  double freq[D / 2];
+  __align__(16) uint8_t v[D * V_ROW];
   uint32_t amax_of[THREADS / 64];
+  float old;
 };
 
+// The new tokens stay in registers, 8 values of a token a lane, from their loads to their bytes: normed and rotated (angles
+// are computed by every lane for itself), their largest magnitude joined through LDS, quantized.  A token's bytes of K lie
+// together and go straight to the cache; those of V pass through LDS as bytes, to leave as the rows of the V block.
 template <int KIND, int D, bool is_v>
 __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& lds) {
-  constexpr int LANES = D / 8, ROWS = AppendLds<D>::ROWS, PAD = AppendLds<D>::PAD;
-  float* x = lds.x;
-  auto& turn = lds.turn;
-  auto& amax_of = lds.amax_of;
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES, PASSES = KV_BLOCK / ROWS, ITEMS = (2 * D + THREADS - 1) / THREADS;
   const int head = blockIdx.y;
   Piece p;
   if (!find_piece(a.q_start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, p)) return;
   const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
   if (block < 0) return;
+  const bool whole = p.first == 0 && p.last == KV_BLOCK;
+  uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
+  float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
 
-  // The new tokens, normed and rotated, in float32 in LDS; their largest magnitude on the way.
+  // Everything that is to be read is asked for at once.
   const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const void* src = is_v ? a.v : a.k;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
-  constexpr int PASSES = KV_BLOCK / ROWS;
   float y[PASSES][8];
-  uint32_t amax_bits = 0;         // magnitudes order like their bits, infinity and NaN above all numbers
-  // All rows are asked for at once; the angles are computed while they are on their way.
-  auto row_at = [&](int t) { return (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D; };
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int t = p.first + i * ROWS + sub;
-    if (t < p.last) load8_f32<KIND>(src, row_at(t) + 8 * slot, y[i]);
+    if (t < p.last) load8_f32<KIND>(src, (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D + 8 * slot, y[i]);
   }
-  const int pairs = a.rotary_dim / 2;
-  if (!is_v && pairs > 0) {
-    if (threadIdx.x < static_cast<unsigned>(pairs)) lds.freq[threadIdx.x] = turns_of(a.inv_freq[threadIdx.x]);
-    const int t = p.first + static_cast<int>(threadIdx.x) - THREADS / 2;      // (other threads than those)
-    if (t >= p.first && t < p.last)
-      lds.position[t] = a.positions ? a.positions[p.row + (t - p.first)] : (p.block << 5) + t;
-    __syncthreads();
+  float old = 0.0f;
+  if (threadIdx.x == 0 && p.first > 0) old = *scale_at;      // by the thread that will write it
+  uint4 kept[ITEMS];
+  if (is_v && !whole) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int item = threadIdx.x + i * THREADS;
+      if (item < 2 * D) kept[i] = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
+    }
+  }
+  uint32_t amax_bits = 0;         // magnitudes order like their bits, infinity and NaN above all numbers
+  const bool turns = !is_v && 8 * slot < a.rotary_dim, interleaved = a.interleaved != 0;
+  double freq[8];
+  if (turns) {
+    const float* from = a.inv_freq + first_pair(slot, a.rotary_dim, interleaved);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < 4 || !interleaved) freq[k] = turns_of(from[k]);
   }
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int t0 = p.first + i * ROWS, t = t0 + sub;
-    if (t0 >= p.last) break;
-    if (!is_v && pairs > 0) {
-      if (i > 0) __syncthreads();
-      for (int k = threadIdx.x; k < ROWS * pairs; k += THREADS) {
-        const int r = k / pairs, j = k - r * pairs;
-        if (t0 + r < p.last) turn[r][j] = rotation(lds.position[t0 + r], lds.freq[j], a.rope_scale);
-      }
-      __syncthreads();
-    }
-    if (t < p.last) {
-      if (!is_v)
-        norm_rotate8<D>(y[i], slot, a.k_weight, a.eps, turn[sub], a.rotary_dim, a.interleaved != 0);
+    const int t = p.first + i * ROWS + sub;
+    if (t >= p.last) break;
+    if constexpr (!is_v) {
+      float2 cs[8];
+      if (turns) {
+        const int64_t position = a.positions ? a.positions[p.row + (t - p.first)] : (p.block << 5) + t;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        x[t * PAD + 8 * slot + k] = y[i][k];
-        amax_bits = max(amax_bits, float_to_bits(y[i][k]) & 0x7FFFFFFFu);
+        for (int k = 0; k < 8; ++k)
+          if (k < 4 || !interleaved) cs[k] = rotation(position, freq[k], a.rope_scale);
       }
+      norm_rotate8<D>(y[i], slot, a.k_weight, a.eps, [&](int k) { return cs[k]; }, a.rotary_dim, interleaved);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax_bits = max(amax_bits, float_to_bits(y[i][k]) & 0x7FFFFFFFu);
+  }
+  amax_bits = wave_max_u32(amax_bits);
+  if ((threadIdx.x & 63) == 0) lds.amax_of[threadIdx.x >> 6] = amax_bits;
+  if (threadIdx.x == 0) lds.old = old;
+  __syncthreads();
+  amax_bits = max(max(lds.amax_of[0], lds.amax_of[1]), max(lds.amax_of[2], lds.amax_of[3]));
+  old = lds.old;
+  const bool poisoned = amax_bits >= 0x7F800000u || old != old;
+  const float scale = fmaxf(fmaxf(old, bits_to_float(amax_bits) / 127.0f), KV_SCALE_FLOOR);
+  const float ratio = old / scale, reciprocal = 1.0f / scale;      // ratio: 1 where the scale stays
+  if (threadIdx.x == 0) *scale_at = poisoned ? __builtin_nanf("") : scale;
+  const bool grown = ratio != 1.0f && !poisoned;
+
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int t = p.first + i * ROWS + sub;
+    if (t >= p.last) break;
+    uint32_t q[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) q[k] = poisoned ? 128u : quantize(y[i][k], scale, reciprocal);
+    if constexpr (is_v) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) lds.v[(8 * slot + k) * V_ROW + v_place(t)] = static_cast<uint8_t>(q[k]);
+    } else {
+      *reinterpret_cast<uint2*>(bytes + ((slot >> 1) * KV_BLOCK + t) * 16 + 8 * (slot & 1)) =
+          make_uint2(pack_bytes(q[0], q[1], q[2], q[3]), pack_bytes(q[4], q[5], q[6], q[7]));
     }
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) amax_bits = max(amax_bits, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax_bits), off)));
-  if ((threadIdx.x & 63) == 0) amax_of[threadIdx.x >> 6] = amax_bits;
-  __syncthreads();
-  amax_bits = max(max(amax_of[0], amax_of[1]), max(amax_of[2], amax_of[3]));
-  const float amax = bits_to_float(amax_bits);
-
-  float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
-  const float old = p.first > 0 ? *scale_at : 0.0f;
-  const bool poisoned = amax_bits >= 0x7F800000u || old != old;
-  const float scale = fmaxf(fmaxf(old, amax / 127.0f), KV_SCALE_FLOOR);
-  const float ratio = old / scale, reciprocal = 1.0f / scale;      // ratio: 1 where the scale stays
-  uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
-  __syncthreads();                                     // every thread has read the old scale
-  if (threadIdx.x == 0) *scale_at = poisoned ? __builtin_nanf("") : scale;
-
-  const bool grown = ratio != 1.0f && !poisoned, whole = p.first == 0 && p.last == KV_BLOCK && !poisoned;
-  for (int item = threadIdx.x; item < 2 * D; item += THREADS) {
-    // 16 bytes: of K one token's 16 dims, of V one dim's 16 tokens.
-    const int t_k = item & 31, d_k = (item >> 5) * 16;
-    const int d_v = item >> 1, place0 = (item & 1) * 16;
-    auto at = [&](int k) { return is_v ? v_token(place0 + k) * PAD + d_v : t_k * PAD + d_k + k; };
-    uint32_t w[4];
-    if (whole) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = pack_bytes(quantize(x[at(4 * i)], scale, reciprocal), quantize(x[at(4 * i + 1)], scale, reciprocal),
-                          quantize(x[at(4 * i + 2)], scale, reciprocal), quantize(x[at(4 * i + 3)], scale, reciprocal));
-    } else {
-      const bool keeps = is_v || t_k < p.first, takes = is_v || (t_k >= p.first && t_k < p.last);
-      if (!takes && !(keeps && grown)) continue;
-      uint4 u = make_uint4(0, 0, 0, 0);
-      if (keeps) u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  if constexpr (!is_v) {
+    if (!grown || p.first == 0) return;
+    for (int item = threadIdx.x; item < 2 * D; item += THREADS) {      // 16 dims of one of the earlier tokens
+      if ((item & 31) >= p.first) continue;
+      uint4 u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
+      uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t r = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = is_v ? v_token(place0 + 4 * i + j) : t_k;
-          uint32_t b = (w[i] >> (8 * j)) & 0xFFu;
-          if (t >= p.first && t < p.last) b = poisoned ? 128u : quantize(x[at(4 * i + j)], scale, reciprocal) & 0xFFu;
-          else if (t < p.first && grown) b = requantize(b, ratio);
-          r |= b << (8 * j);
-        }
+        for (int j = 0; j < 4; ++j) r |= requantize((w[i] >> (8 * j)) & 0xFFu, ratio) << (8 * j);
         w[i] = r;
       }
+      *reinterpret_cast<uint4*>(bytes + item_offset(item)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(bytes + item_offset(item)) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {      // 16 tokens of a dim
+      const int item = threadIdx.x + i * THREADS;
+      if (item >= 2 * D) break;
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(lds.v + (item >> 1) * V_ROW + (item & 1) * 16);
+      uint32_t w[4] = {from[0], from[1], from[2], from[3]};
+      if (!whole) {
+        const uint32_t there[4] = {kept[i].x, kept[i].y, kept[i].z, kept[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t r = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int t = v_token((item & 1) * 16 + 4 * j + b);
+            uint32_t byte = ((t >= p.first && t < p.last ? w[j] : there[j]) >> (8 * b)) & 0xFFu;
+            if (t < p.first && grown) byte = requantize(byte, ratio);
+            r |= byte << (8 * b);
+          }
+          w[j] = r;
+        }
+      }
+      *reinterpret_cast<uint4*>(bytes + item_offset(item)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
@@ -248,7 +282,7 @@ struct ReadArgs {
 // that is not in the cache (a bad page) yields zeros.
 template <int KIND, int D>
 __global__ void __launch_bounds__(THREADS) kv_read_kernel(ReadArgs a) {
-  constexpr int LANES = D / 8, ROWS = THREADS / LANES, V_ROW = KV_BLOCK + 4;   // V rows padded: 8 lanes read 8 dims apart
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES;
   __shared__ __align__(16) uint8_t lds[D * V_ROW];
   const bool is_v = blockIdx.z != 0;
   void* dst = is_v ? a.v : a.k;

@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_kernel(QkArgs a) {
       load(last ? next : t, last ? first : head + per_pass, ahead);
       if (head < heads) {
         const bool is_q = head < a.q_heads;
-        norm_rotate8<D>(x, slot, is_q ? a.q_weight : a.k_weight, a.eps, turn[buffer], a.rotary_dim, a.interleaved != 0);
+        const float2* from = turn[buffer] + first_pair(slot, a.rotary_dim, a.interleaved != 0);
+        norm_rotate8<D>(x, slot, is_q ? a.q_weight : a.k_weight, a.eps, [&](int i) { return from[i]; }, a.rotary_dim, a.interleaved != 0);
         const int64_t at = is_q ? t * a.q_out_stride + static_cast<int64_t>(head) * D
                                 : t * a.k_out_stride + static_cast<int64_t>(head - a.q_heads) * D;
         store8_f32<OUT>(is_q ? a.q_out : a.k_out, at + 8 * slot, x);
