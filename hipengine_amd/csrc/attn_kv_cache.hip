@@ -137,13 +137,7 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
   const int head = blockIdx.y;
   Piece p;
   if (!find_piece(a.q_start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, p)) return;
-  const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
-  if (block < 0) return;
-  const bool whole = p.first == 0 && p.last == KV_BLOCK;
-  uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
-  float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
-
-  // Everything that is to be read is asked for at once.
+  // Everything that is to be read is asked for as early as it can be: the rows before the page is known.
   const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const void* src = is_v ? a.v : a.k;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
@@ -153,6 +147,11 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
     const int t = p.first + i * ROWS + sub;
     if (t < p.last) load8_f32<KIND>(src, (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D + 8 * slot, y[i]);
   }
+  const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
+  if (block < 0) return;
+  const bool whole = p.first == 0 && p.last == KV_BLOCK;
+  uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
+  float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
   float old = 0.0f;
   if (threadIdx.x == 0 && p.first > 0) old = *scale_at;      // by the thread that will write it
   uint4 kept[ITEMS];
