@@ -445,6 +445,10 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
   constexpr int TILE = 32 * W;
   constexpr int KC = D / 32, PIECES = 2 * KC;          // operand pieces of K, and of V; a 16-byte load gives two of them
   constexpr int LOADS = 2 * KC, MINE = LOADS / W;      // of a block: K's, then V's
+  // Operands that are on their way from LDS while others are multiplied, V's first ones during the softmax; the order is
+  // pinned, the compiler would ask for two and wait for them (8192 tokens 712 us and 699 in this order, 2048 tokens 74 and 71). More cost
+  // more registers than there are.
+  constexpr int K_AHEAD = D == 256 ? 3 : 4, V_AHEAD = D == 256 ? 1 : 2;
   __shared__ h8 lds_k[2][PIECES][64];
   __shared__ h8 lds_v[2][PIECES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -527,8 +531,22 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
       lds_barrier();               // block j is in LDS, and nobody reads the other buffer any more
       const Scales b = s1;
       f16v s = f16v{0};
+      {
+        h8 o[K_AHEAD];
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_k[here][i][lane], k.q[i], s, 0, 0, 0);
+        for (int i = 0; i < K_AHEAD; ++i) o[i] = lds_k[here][i][lane];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(o[i % K_AHEAD], k.q[i], s, 0, 0, 0);
+          if (i + K_AHEAD < PIECES) o[i % K_AHEAD] = lds_k[here][i + K_AHEAD][lane];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      auto v_piece = [&](int i) { return lds_v[here][2 * (i % KC) + i / KC][lane]; };
+      h8 vo[V_AHEAD];
+#pragma unroll
+      for (int i = 0; i < V_AHEAD; ++i) vo[i] = v_piece(i);
       const int key0 = j * KV_BLOCK;
       float c = b.ks * k.c;
       c = c < 1e-37f ? 1e-37f : c;   // (a NaN stays)
@@ -573,9 +591,11 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
         l = fmaf(sum, b.iv, l);
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int t = 0; t < KC; ++t) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_v[here][2 * t + h][lane], p[h], acc[t], 0, 0, 0);
+      for (int i = 0; i < PIECES; ++i) {
+        acc[i % KC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vo[i % V_AHEAD], p[i / KC], acc[i % KC], 0, 0, 0);
+        if (i + V_AHEAD < PIECES) vo[i % V_AHEAD] = v_piece(i + V_AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       convert(here ^ 1);
       fetch(j + 2);
     }
