@@ -138,8 +138,8 @@ __device__ __forceinline__ int first_pair(int slot, int rotary_dim, bool interle
 }
 
 // One head's RMS norm and rotation by the D / 8 neighbouring lanes that hold it, 8 values a lane (x: head dims 8 * slot ..).
-// turn(i) gives (cos, sin) of the i-th pair from first_pair on.  rotary_dim is a multiple of 16, so a lane's 8 values lie on one
-// side of every border and their partners all in one other lane.
+// turn(i) gives (cos, sin) of the i-th pair from first_pair on.  rotary_dim is a multiple of 16, so a lane's 8 values lie on
+// one side of every border and their partners all in one other lane.
 template <int D, typename Turn>
 __device__ __forceinline__ void norm_rotate8(float (&x)[8], int slot, const float* __restrict__ weight, float eps, Turn turn,
                                              int rotary_dim, bool interleaved) {

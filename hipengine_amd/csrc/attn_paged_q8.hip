@@ -435,19 +435,21 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 // grown out of its range is the maximum looked for, the reference moved and P taken again.
 //
 // What bounds it: 8192 tokens, 40 / 8 heads of 128, 695 us (0.99 PFLOP/s; a large bf16 product: 1.37): vector instructions
-// 60 % and matrix instructions 45 % of the cycles, at 2.1 GHz.  Of D 256 it is the occupancy, two waves a SIMD, which wait
-// for each other at the barrier: 0.6 PFLOP/s.  Four waves, three such workgroups a CU, let one wave's softmax run in another's products.  Measured
-// and not taken: eight waves (half the conversions a wave, but two waves a SIMD) 735 us; products of the next block behind
-// the softmax of this one (250 registers, two waves a SIMD) 765 to 780 us; 64 rows a wave 1053 us; K and V converted by
-// every wave from registers 899 us; wave priorities around the products or the softmax, no difference.
+// 63 % and matrix instructions 51 % of the cycles, at 2.05 GHz.  Of D 256 it is the occupancy, two waves a SIMD, which wait
+// for each other at the barrier: 0.6 PFLOP/s.
+// Four waves, three such workgroups a CU, let one wave's softmax run in another's products.  Measured and not taken: eight
+// waves (half the conversions a wave, but two waves a SIMD) 717 to 735 us, with half of them half a step behind the others
+// 786 to 802; products of the next block behind the softmax of this one (250 registers, two waves a SIMD) 765 to 780; 64
+// rows a wave 1053; K and V converted by every wave from registers 899; a running maximum looked for ahead of the
+// exponentials 716; wave priorities around the products or the softmax, no difference.
 template <int D, int KIND, int W>
 __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kernel(AttnArgs a) {
   constexpr int TILE = 32 * W;
   constexpr int KC = D / 32, PIECES = 2 * KC;          // operand pieces of K, and of V; a 16-byte load gives two of them
   constexpr int LOADS = 2 * KC, MINE = LOADS / W;      // of a block: K's, then V's
   // Operands that are on their way from LDS while others are multiplied, V's first ones during the softmax; the order is
-  // pinned, the compiler would ask for two and wait for them (8192 tokens 712 us and 699 in this order, 2048 tokens 74 and 71). More cost
-  // more registers than there are.
+  // pinned, the compiler would ask for two and wait for them (8192 tokens 712 us and in this order 699, 2048 tokens 74 and
+  // 71).  More would take more registers than there are.
   constexpr int K_AHEAD = D == 256 ? 3 : 4, V_AHEAD = D == 256 ? 1 : 2;
   __shared__ h8 lds_k[2][PIECES][64];
   __shared__ h8 lds_v[2][PIECES][64];

@@ -16,8 +16,8 @@
 // holds the token by the chunks' weights up to B, and the token in it.
 // A list that would not fit (a row so flat that one bin holds over 16384 tokens) is replaced by the row itself.
 //
-// What bounds it.  One row of 151936 with top-k 50: five launches of 4 to 8 us, each a few loads that wait for each other.
-// 64 rows with top-p 0.9 (39 MB): 11 + 18 + 5 + 15 + 18 us; the passes over the logits stand at what such a launch takes to
+// What bounds it.  One row of 151936 with top-k 50: four launches of 4 to 8 us, each a few steps that wait for each other.
+// 64 rows with top-p 0.9 (39 MB): 11 + 16 + 5 + 15 + 16 us; the passes over the logits stand at what such a launch takes to
 // read them (11) plus 4 us for 10^7 weights in the second, and pass 4 at its barriers.  Sums of bins through global
 // atomics, and a counter beside the neighbouring rows', cost 15 us more: additions to one line wait for each other.
 
