@@ -62,6 +62,11 @@ struct AttnArgs {
   int window;
   int splits;             // most chunks of keys
   int chunk;              // fewest blocks of 32 keys in a chunk
+  // Of several prompts in parts:
+  int32_t* parts;         // [batch] chunks of each sequence; else null
+  int items, tiles;       // workgroups for a KV head, and for a sequence's rows at most
+  int batch;
+  int least;              // blocks that a part has if there are as many
   float* part_acc;        // [splits][tokens * q_heads][D]
   float* part_ml;         // [splits][tokens * q_heads][2]
 };
@@ -106,7 +111,79 @@ struct Sight {
 
 // Blocks in each of a tile's chunks, from the blocks that it sees: the announced lengths only say how many chunks there may
 // be, so that a call captured for the longest cache cuts a short one as finely.
-__device__ __forceinline__ int chunk_of(const AttnArgs& a, int blocks) { return max((blocks + a.splits - 1) / a.splits, a.chunk); }
+__device__ __forceinline__ int chunk_of(const AttnArgs& a, int parts, int blocks) { return max((blocks + parts - 1) / parts, a.chunk); }
+
+// Which part of which tile a workgroup works on.
+struct Share {
+  int seq, tile, split, parts;   // seq < 0: none
+};
+
+// Several prompts differ in rows and keys, so each is cut into parts of its own: all parts have about c blocks, with the least c
+// that needs no more workgroups than there are: 3 chunks of about 400 tokens of D 256 behind 2000 to 6000 others, 242
+// workgroups of up to 47 blocks, take 110 us; 160 of up to 63, by a chunk from the announced length, 132 us.  Every wave
+// computes it for itself, a sequence a lane, up to four times 64.
+template <int TILE>
+__device__ Share share_of(const AttnArgs& a, int item) {
+  constexpr int MORE = 4;
+  const int lane = threadIdx.x & 63;
+  int tiles[MORE], blocks[MORE], longest = 0;
+  float work = 0.0f;
+#pragma unroll
+  for (int i = 0; i < MORE; ++i) {
+    const int b = lane + 64 * i;
+    tiles[i] = blocks[i] = 0;
+    if (64 * i >= a.batch) continue;
+    if (b < a.batch) {
+      tiles[i] = static_cast<int>(min((seq_rows(a.q_start, b, a.tokens).count * a.group + TILE - 1) / TILE, static_cast<int64_t>(a.tiles)));
+      blocks[i] = (min(max(a.kv_lens[b], 0), MAX_KV) + 31) >> 5;
+      if (a.window > 0) blocks[i] = min(blocks[i], ((a.window + TILE / a.group + 1) >> 5) + 2);
+    }
+    work += static_cast<float>(tiles[i]) * static_cast<float>(blocks[i]);
+    if (tiles[i] > 0) longest = max(longest, blocks[i]);
+  }
+  auto sum = [](auto v) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v += __shfl_xor(v, off);
+    return v;
+  };
+  work = sum(work);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) longest = max(longest, __shfl_xor(longest, off));
+  int c = max(max(static_cast<int>(work / static_cast<float>(a.items)), a.least), (longest + a.splits - 1) / a.splits);
+  int parts[MORE];
+  for (;; c += (c >> 4) + 1) {       // ends: with c = longest there are no more than a.tiles * a.batch <= a.items
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < MORE; ++i) {
+      if (64 * i >= a.batch) continue;
+      parts[i] = max((blocks[i] + c - 1) / c, 1);
+      all += tiles[i] * parts[i];
+    }
+    if (c >= longest || sum(all) <= a.items) break;
+  }
+  Share r{-1, 0, 0, 1};
+#pragma unroll
+  for (int i = 0; i < MORE; ++i) {
+    if (64 * i >= a.batch) continue;
+    const int own = tiles[i] * parts[i];
+    int up_to = own;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(up_to, off);
+      if (lane >= off) up_to += o;
+    }
+    const unsigned long long here = __ballot(item >= up_to - own && item < up_to);
+    if (r.seq < 0 && here) {
+      const int l = __builtin_ctzll(here), n = __builtin_amdgcn_readlane(tiles[i], l);
+      const int at = item - __builtin_amdgcn_readlane(up_to - own, l);
+      r = {l + 64 * i, n - 1 - at % n, at / n, __builtin_amdgcn_readlane(parts[i], l)};
+    }
+    item -= __builtin_amdgcn_readlane(up_to, 63);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && lane + 64 * i < a.batch) a.parts[lane + 64 * i] = parts[i];
+  }
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  return {uniform(r.seq), uniform(r.tile), uniform(r.split), uniform(r.parts)};
+}
 
 // One column: a row of queries as the matrix instruction's second operand (lane (column, half) holds dims 32 i + 16 half +
 // 8 b .. + 7 of piece 2 i + b), and what goes with it.
@@ -270,11 +347,11 @@ __device__ __forceinline__ float opaque_one() {
 // A column's result: to the output, or with splits to the workspace.
 template <int D, int KIND>
 __device__ __forceinline__ void store_column(const AttnArgs& a, const SeqRows& rows, int r, int n_rows, int head, int split,
-                                             float m, float l, const f16v (&acc)[D / 32]) {
+                                             int parts, float m, float l, const f16v (&acc)[D / 32]) {
   if (r >= n_rows) return;
   const int half = (threadIdx.x & 63) >> 5, query = r / a.group;
   const int64_t q_head = head * a.group + (r - query * a.group), row = rows.first + query;
-  if (a.splits > 1) {
+  if (parts > 1) {
     const int64_t at = (static_cast<int64_t>(split) * a.tokens + row) * a.q_heads + q_head;
     if (half == 0) {
       a.part_ml[2 * at] = m;
@@ -322,7 +399,7 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
   const int lim_first = sight.limit(first_q), lo_last = sight.lower(last_q);
   int blk = sight.lower(first_q) >> 5, blk_end = (sight.limit(last_q) + 31) >> 5;
   if (a.splits > 1) {
-    const int chunk = chunk_of(a, blk_end - blk);
+    const int chunk = chunk_of(a, a.splits, blk_end - blk);
     blk += split * chunk;
     blk_end = min(blk_end, blk + chunk);
   }
@@ -420,7 +497,7 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
       __syncthreads();
     }
   }
-  if (wave == 0) store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, split, m, l, acc);
+  if (wave == 0) store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, split, a.splits, m, l, acc);
 }
 
 // ---- many rows: the waves of a workgroup have 32 rows each and walk over the keys together --------------------------
@@ -455,18 +532,22 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
   __shared__ h8 lds_v[2][PIECES][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.x;
-  const int seq = blockIdx.z / a.splits, split = blockIdx.z - seq * a.splits;
+  Share share{static_cast<int>(blockIdx.z / a.splits), static_cast<int>(gridDim.y - 1 - blockIdx.y),
+              static_cast<int>(blockIdx.z % a.splits), a.splits};
+  if (a.parts) share = share_of<TILE>(a, blockIdx.y);
+  if (share.seq < 0) return;
+  const int seq = share.seq;
   const SeqRows rows = seq_rows(a.q_start, seq, a.tokens);
   const int n_rows = static_cast<int>(rows.count) * a.group;
-  const int tile0 = (gridDim.y - 1 - blockIdx.y) * TILE, row0 = tile0 + wave * 32;
+  const int tile0 = share.tile * TILE, row0 = tile0 + wave * 32;
   if (tile0 >= n_rows) return;
   const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
   // Blocks that the tile sees; a wave's own rows may see fewer, it masks the rest.
   int blk = sight.lower(tile0 / a.group) >> 5;
   int blk_end = (sight.limit((min(tile0 + TILE, n_rows) - 1) / a.group) + 31) >> 5;
-  if (a.splits > 1) {
-    const int chunk = chunk_of(a, blk_end - blk);
-    blk += split * chunk;
+  if (share.parts > 1) {
+    const int chunk = chunk_of(a, share.parts, blk_end - blk);
+    blk += share.split * chunk;
     blk_end = min(blk_end, blk + chunk);
   }
   const int lim_first = sight.limit(min(row0, n_rows - 1) / a.group);
@@ -603,7 +684,7 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
     }
   }
   l += other_half(l);
-  store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, split, m, l, acc);
+  store_column<D, KIND>(a, rows, row0 + (lane & 31), n_rows, head, share.split, share.parts, m, l, acc);
 }
 
 // Joins the chunks of output rows: grid (rows a sequence / (4 / TEAM), batch); TEAM waves have a row and take its chunks in
@@ -615,6 +696,8 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   constexpr int V = D / 64;
   __shared__ float part[4][D];
   const int seq = blockIdx.y, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int parts = a.parts ? a.parts[seq] : a.splits;
+  if (parts <= 1) return;
   const SeqRows rows = seq_rows(a.q_start, seq, a.tokens);
   const int64_t r = static_cast<int64_t>(blockIdx.x) * (4 / TEAM) + wave / TEAM;
   if (r >= rows.count * a.q_heads) return;             // (of a team all waves or none: the barrier below is for TEAM 4)
@@ -623,7 +706,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
   const int row = query * a.group + q_head % a.group;
   const int tile0 = row / tile_rows * tile_rows, last_q = (min(tile0 + tile_rows, static_cast<int>(rows.count) * a.group) - 1) / a.group;
-  const int first = sight.lower(tile0 / a.group) >> 5, chunk = chunk_of(a, ((sight.limit(last_q) + 31) >> 5) - first);
+  const int first = sight.lower(tile0 / a.group) >> 5, chunk = chunk_of(a, parts, ((sight.limit(last_q) + 31) >> 5) - first);
   const int blocks = max(((sight.limit(query) + 31) >> 5) - first, 0), splits = (blocks + chunk - 1) / chunk;
   const int64_t at = (rows.first + query) * a.q_heads + q_head, pitch = a.tokens * a.q_heads;
   float m = NEVER;
@@ -685,23 +768,29 @@ struct Plan {
   int waves;
   int tile_rows;
   int64_t tiles;
+  int splits;         // most parts of a tile's keys
   int most_splits;    // what the workspace is sized for: no fewer for fewer keys
-  int splits, chunk;
+  int typical;        // parts where all sequences are as long as announced
+  int chunk, least;   // fewest blocks in a part of a sequence by itself, and where sequences share workgroups
+  bool shares;        // several prompts in parts
+  int64_t items;      // their workgroups a KV head
 };
 
 constexpr int CUS = 256;
 
 // What rows are cut into, and keys where the rows alone are too few.
-void cut(Plan& p, int64_t rows, int64_t blocks, int64_t heads, int64_t slots, int64_t least) {
+void cut(Plan& p, int64_t rows, int64_t blocks, int64_t batch, int64_t kv_heads, int64_t slots, int64_t least) {
   p.tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-  const int64_t groups = heads * p.tiles, most = (blocks + least - 1) / least;
-  int64_t splits = !p.keys && groups >= CUS ? 1 : (slots + groups - 1) / groups;
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  p.most_splits = static_cast<int>(splits);
-  p.chunk = static_cast<int>((blocks + splits - 1) / splits);
-  p.splits = p.chunk > 0 ? static_cast<int>((blocks + p.chunk - 1) / p.chunk) : 1;
-  if (p.keys) p.chunk = static_cast<int>(least);
+  const int64_t groups = batch * kv_heads * p.tiles, most = blocks > least ? (blocks + least - 1) / least : 1;
+  const int64_t splits = !p.keys && groups >= CUS ? 1 : (slots + groups - 1) / groups;
+  // Of prompts that differ in length the longer ones get more parts than that.
+  const int64_t up_to = p.keys || batch == 1 || splits == 1 ? splits : 2 * splits;
+  p.typical = static_cast<int>(splits < most ? splits : most);
+  p.splits = p.most_splits = static_cast<int>(up_to < most ? up_to : most);
+  p.shares = !p.keys && batch > 1 && p.splits > 1;
+  p.least = static_cast<int>(least);
+  p.chunk = p.shares ? 1 : p.keys ? p.least : static_cast<int>((blocks + p.splits - 1) / p.splits);
+  p.items = slots / kv_heads > batch * p.tiles ? slots / kv_heads : batch * p.tiles;
 }
 
 Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t window) {
@@ -718,10 +807,10 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   // LEAST_ROWS and one of few rows, whose keys four waves share, at least LEAST_KEYS: a single token behind 600 others (19
   // blocks of 128) takes 14.4 us undivided and 17.3 us in two parts and the joining of them, behind 32768 others 22 us in
   // 32 parts and 26 us in 64; 512 tokens of D 128 (16 blocks) 23 us undivided and 35 us in two, of D 256 40 and 38 us.
-  const int64_t heads = batch * kv_heads, LEAST_KEYS = 4096 / dim, LEAST_ROWS = 2048 / dim;
+  const int64_t LEAST_KEYS = 4096 / dim, LEAST_ROWS = 2048 / dim;
   p.waves = WAVES;
   p.tile_rows = p.keys ? 32 : 32 * WAVES;
-  cut(p, rows, blocks, heads, 2 * CUS, p.keys ? LEAST_KEYS : LEAST_ROWS);
+  cut(p, rows, blocks, batch, kv_heads, 2 * CUS, p.keys ? LEAST_KEYS : LEAST_ROWS);
   if (!p.keys && dim == 256) {
     // Eight waves convert a block for twice the rows. Of D 256 a CU holds as many of them either way (of smaller D not: 3
     // workgroups of four), and they win once there is nearly a workgroup for every CU: 3 chunks of 512 tokens 129 us
@@ -729,9 +818,9 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
     Plan wide = p;
     wide.waves = 2 * WAVES;
     wide.tile_rows = 64 * WAVES;
-    cut(wide, rows, blocks, heads, CUS, LEAST_ROWS);
+    cut(wide, rows, blocks, batch, kv_heads, CUS, LEAST_ROWS);
     const int most = p.most_splits > wide.most_splits ? p.most_splits : wide.most_splits;   // (a window may decide otherwise)
-    if (heads * wide.tiles * wide.splits >= CUS * 3 / 4) p = wide;
+    if (batch * kv_heads * wide.tiles * wide.typical >= CUS * 3 / 4) p = wide;
     p.most_splits = most;
   }
   return p;
@@ -747,13 +836,14 @@ bool shape_ok(int64_t tokens, int64_t batch, int64_t max_q, int64_t max_kv, int6
          max_q * (q_heads / kv_heads) <= (1 << 30);
 }
 
-int64_t workspace_of(int splits, int64_t tokens, int64_t q_heads, int64_t dim) {
-  return splits > 1 ? static_cast<int64_t>(splits) * tokens * q_heads * (dim + 2) * 4 : 0;
+int64_t workspace_of(bool keys, int splits, int64_t tokens, int64_t batch, int64_t q_heads, int64_t dim) {
+  return splits > 1 ? static_cast<int64_t>(splits) * tokens * q_heads * (dim + 2) * 4 + (keys || batch == 1 ? 0 : 4 * batch) : 0;
 }
 
 template <int D, int KIND>
 int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64_t kv_heads, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.tiles), static_cast<unsigned>(batch * p.splits));
+  const dim3 grid(static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.shares ? p.items : p.tiles),
+                  static_cast<unsigned>(p.shares ? 1 : batch * p.splits));
   if (p.keys) {
     hipLaunchKernelGGL((attention_keys_kernel<D, KIND>), grid, dim3(WAVES * 64), 0, stream, a);
   } else if (p.waves == WAVES) {
@@ -764,10 +854,11 @@ int launch(const AttnArgs& a, const Plan& p, int64_t batch, int64_t max_q, int64
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess || p.splits == 1) return static_cast<int>(err);
   const int64_t out_rows = max_q * a.q_heads;
-  if (p.splits > 8 || batch * out_rows <= 2048)
-    hipLaunchKernelGGL((join_kernel<D, KIND, 4>), dim3(static_cast<unsigned>(out_rows), static_cast<unsigned>(batch)), dim3(256), 0, stream, a, p.tile_rows);
+  const unsigned each = static_cast<unsigned>(out_rows), of_four = static_cast<unsigned>((out_rows + 3) / 4), b = static_cast<unsigned>(batch);
+  if (p.typical > 8 || batch * out_rows <= 2048)
+    hipLaunchKernelGGL((join_kernel<D, KIND, 4>), dim3(each, b), dim3(256), 0, stream, a, p.tile_rows);
   else
-    hipLaunchKernelGGL((join_kernel<D, KIND, 1>), dim3(static_cast<unsigned>((out_rows + 3) / 4), static_cast<unsigned>(batch)), dim3(256), 0, stream, a, p.tile_rows);
+    hipLaunchKernelGGL((join_kernel<D, KIND, 1>), dim3(of_four, b), dim3(256), 0, stream, a, p.tile_rows);
   return static_cast<int>(hipGetLastError());
 }
 
@@ -778,7 +869,8 @@ extern "C" int hipengine_gfx950_paged_attention_q8_workspace_bytes(int64_t token
                                                                    int64_t head_dim, int64_t* bytes) {
   if (!bytes || !shape_ok(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim, 0)) return BAD;
   const int64_t longest = max_q_len < tokens ? max_q_len : tokens;
-  *bytes = workspace_of(plan_of(batch, longest, max_kv_len, q_heads, kv_heads, head_dim, 0).most_splits, tokens, q_heads, head_dim);
+  const Plan p = plan_of(batch, longest, max_kv_len, q_heads, kv_heads, head_dim, 0);
+  *bytes = workspace_of(p.keys, p.most_splits, tokens, batch, q_heads, head_dim);
   return 0;
 }
 
@@ -803,16 +895,19 @@ extern "C" int hipengine_gfx950_paged_attention_q8(const void* q, void* out, int
   if (q_stride < width || out_stride < width) return BAD;
   const int64_t longest = max_q_len < tokens ? max_q_len : tokens;
   const Plan p = plan_of(batch, longest, max_kv_len, q_heads, kv_heads, head_dim, window);
-  const int64_t need = workspace_of(p.splits, tokens, q_heads, head_dim);
+  const int64_t need = workspace_of(p.keys, p.splits, tokens, batch, q_heads, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return BAD;
   if (p.tiles > 65535 || batch * p.splits > 65535) return BAD;
   const KvCacheQ8 cache{const_cast<uint8_t*>(k_cache), const_cast<uint8_t*>(v_cache), const_cast<float*>(k_scale),
                         const_cast<float*>(v_scale), page_table, table_stride, pages, static_cast<int>(kv_heads),
                         63 - __builtin_clzll(static_cast<unsigned long long>(page_size))};
-  float* acc = static_cast<float*>(workspace);
+  const int64_t out_rows = p.splits > 1 ? static_cast<int64_t>(p.splits) * tokens * q_heads : 0;
+  float* acc = p.splits > 1 ? static_cast<float*>(workspace) : nullptr;
+  float* ml = acc ? acc + out_rows * head_dim : nullptr;
+  int32_t* parts = p.shares ? reinterpret_cast<int32_t*>(ml + 2 * out_rows) : nullptr;
   const AttnArgs a{cache, q, out, q_stride, out_stride, q_start, kv_lens, tokens, softmax_scale * LOG2E,
                    static_cast<int>(q_heads / kv_heads), static_cast<int>(q_heads), static_cast<int>(window), p.splits,
-                   p.chunk, acc, acc ? acc + static_cast<int64_t>(p.splits) * tokens * q_heads * head_dim : nullptr};
+                   p.chunk, parts, static_cast<int>(p.items), static_cast<int>(p.tiles), static_cast<int>(batch), p.least, acc, ml};
   switch (head_dim * 4 + kind) {
     case 64 * 4 + KIND_BF16: return launch<64, KIND_BF16>(a, p, batch, longest, kv_heads, stream);
     case 64 * 4 + KIND_F16: return launch<64, KIND_F16>(a, p, batch, longest, kv_heads, stream);

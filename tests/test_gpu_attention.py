@@ -497,6 +497,26 @@ def test_attention_refuses_a_small_workspace(dev):
     c.free()
 
 
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("announced", [3000, 1 << 20])
+def test_prompts_that_share_the_chip(dev, window, announced):
+    """150 short prompts, some without rows, without keys, or with fewer keys than rows, a few behind thousands of keys: every
+    sequence is cut into a number of parts of its own."""
+    rng = np.random.default_rng(92)
+    dim, heads, group, batch = 64, 1, 4, 150
+    rows = [int(x) for x in rng.integers(0, 21, batch)]
+    lens = [int(n + x) for n, x in zip(rows, rng.integers(0, 90, batch))]
+    rows[3], lens[3], rows[70], lens[70], rows[71], lens[71], rows[149], lens[149] = 20, 3000, 17, 2500, 20, 0, 20, 2999
+    rows[5], lens[5], rows[64], lens[64] = 20, 7, 0, 1500
+    c = Cache(dev, rng, lens, 64, heads, dim)
+    start, kv = _ragged(rows), np.array(lens, np.int32)
+    q = O.round_to(rng.standard_normal((sum(rows), heads * group, dim)), "bf16")
+    want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5, window=window)
+    got = O.from_bits(run_attention(dev, c, q, start, kv, 20, announced, heads * group, "bf16", window=window), "bf16")
+    assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "bf16", 3000, dim, 127 * c.vs.max())).all()
+    c.free()
+
+
 @pytest.mark.parametrize("rows,lens", [([1, 2], [3000, 70]), ([3, 150], [40, 2100])])
 def test_attention_announced_for_a_longer_cache_than_there_is(dev, rows, lens):
     """As a graph does that was captured for the longest cache: the keys are cut into parts by the lengths that there are."""
