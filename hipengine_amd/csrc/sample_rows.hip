@@ -318,7 +318,7 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
   uint64_t best = 0, sum[2] = {0, 0};
   const int pair = 2 * (threadIdx.x % (BINS / 2)), part = __builtin_amdgcn_readfirstlane(threadIdx.x / (BINS / 2));
   if (g.t > 0.0f && (g.k > 0 || g.p < 1.0f || g.m > 0.0f)) {   // (what no histogram was written for is not used)
-    constexpr int AHEAD = 16;                          // loads on their way, the last few too: not a loop over the rest
+    constexpr int AHEAD = 20;                          // loads on their way, the last few too: not a loop over the rest
     for (int c0 = part; c0 < a.chunks; c0 += AHEAD * PARTS) {
       uint64_t v[AHEAD][2] = {};
 #pragma unroll
@@ -363,8 +363,8 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (up_to(lane * 8 + i) >= goal) reached = min(reached, lane * 8 + i);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) reached = min(reached, __shfl_xor(reached, off));
+    const unsigned long long some = __ballot(reached < BINS - 1);      // (sums only grow: the first lane has it)
+    reached = some ? __builtin_amdgcn_readlane(reached, __builtin_ctzll(some)) : BINS - 1;
     cut.need = need;
     if (r.k > 0) {
       // A border in the last bin cuts nothing (its weights are 0); what top-p and min-p then cut is not known by weight.
