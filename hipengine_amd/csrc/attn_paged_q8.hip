@@ -118,10 +118,10 @@ struct Share {
   int seq, tile, split, parts;   // seq < 0: none
 };
 
-// Several prompts differ in rows and keys, so each is cut into parts of its own: all parts have about c blocks, with the least c
-// that needs no more workgroups than there are: 3 chunks of about 400 tokens of D 256 behind 2000 to 6000 others, 242
-// workgroups of up to 47 blocks, take 110 us; 160 of up to 63, by a chunk from the announced length, 132 us.  Every wave
-// computes it for itself, a sequence a lane, up to four times 64.
+// Several prompts differ in rows and keys, so each is cut into parts of its own: all parts have about c blocks, with the
+// least c that needs no more workgroups than there are.  3 chunks of about 400 tokens of D 256 behind 2000 to 6000 others,
+// as 242 workgroups of up to 47 blocks, take 110 us; as 160 of up to 63, by a chunk from the announced length, 132 us.
+// Every wave computes it for itself, a sequence a lane, up to four times 64.
 template <int TILE>
 __device__ Share share_of(const AttnArgs& a, int item) {
   constexpr int MORE = 4;
