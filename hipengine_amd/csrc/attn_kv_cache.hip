@@ -11,8 +11,8 @@
 // scale and bytes, so there are no atomics and results do not depend on timing.
 //
 // What bounds it.  A single token waits for its chain of loads (row, page, scale, block): 8 sequences, append 4.6 and read
-// 4.4 us.  Of prompts, 8244 tokens of 8 heads of 128 (50 MB in and out), reading back takes 13 us (3.9 TB/s); appending
-// takes 21, not by its bytes but by its stages: rows, norm and rotation, the largest magnitude, and only then the bytes (K
+// 4.0 us.  Of prompts, 8244 tokens of 8 heads of 128 (50 MB in and out), reading back takes 11 us (4.6 TB/s, a large copy
+// 4.8; with K through LDS as well 13.9); appending takes 21, not by its bytes but by its stages: rows, norm and rotation, the largest magnitude, and only then the bytes (K
 // alone 18, V alone 11, both without the rotation 18; with the tokens in LDS as float32 and the angles shared, 26).
 
 #include <hip/hip_runtime.h>
@@ -277,13 +277,11 @@ struct ReadArgs {
   int batch, per_seq;
 };
 
-// grid (units, heads, 2).  The block passes through LDS as bytes, so that a row's values leave as whole lines.  A block
-// that is not in the cache (a bad page) yields zeros.
-template <int KIND, int D>
-__global__ void __launch_bounds__(THREADS) kv_read_kernel(ReadArgs a) {
-  constexpr int LANES = D / 8, ROWS = THREADS / LANES;
-  __shared__ __align__(16) uint8_t lds[D * V_ROW];
-  const bool is_v = blockIdx.z != 0;
+// 8 values of a token a lane, as in the append.  Those of K lie together; V's block passes through LDS as bytes, so that a
+// row's values leave as whole lines.  A block that is not in the cache (a bad page) yields zeros.
+template <int KIND, int D, bool is_v>
+__device__ __forceinline__ void read_piece(const ReadArgs& a, uint8_t* lds) {
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES, PASSES = KV_BLOCK / ROWS;
   void* dst = is_v ? a.v : a.k;
   if (!dst) return;
   const int head = blockIdx.y;
@@ -291,27 +289,44 @@ __global__ void __launch_bounds__(THREADS) kv_read_kernel(ReadArgs a) {
   if (!find_piece(a.start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, p)) return;
   const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
   const float scale = block < 0 ? 0.0f : (is_v ? a.cache.v_scale : a.cache.k_scale)[block];
-  if (block >= 0) {
-    const uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
+  const uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + max(block, int64_t{0}) * (D * KV_BLOCK);
+  const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  uint2 direct[PASSES];
+  if constexpr (is_v) {
     for (int item = threadIdx.x; item < 2 * D; item += THREADS) {
       const uint4 u = *reinterpret_cast<const uint4*>(bytes + item_offset(item));
-      uint32_t* to = reinterpret_cast<uint32_t*>(lds + (is_v ? (item >> 1) * V_ROW + (item & 1) * 16 : item_offset(item)));
+      uint32_t* to = reinterpret_cast<uint32_t*>(lds + (item >> 1) * V_ROW + (item & 1) * 16);
       to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
     }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int t = p.first + i * ROWS + sub;
+      if (t < p.last) direct[i] = *reinterpret_cast<const uint2*>(bytes + ((slot >> 1) * KV_BLOCK + t) * 16 + 8 * (slot & 1));
+    }
   }
-  __syncthreads();
-  const int slot = threadIdx.x % LANES;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
-  for (int t = p.first + static_cast<int>(threadIdx.x) / LANES; t < p.last; t += ROWS) {
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int t = p.first + i * ROWS + sub;
+    if (t >= p.last) break;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = 8 * slot + i;
-      const int at = is_v ? d * V_ROW + v_place(t) : ((d >> 4) * KV_BLOCK + t) * 16 + (d & 15);
-      y[i] = block < 0 ? 0.0f : static_cast<float>(static_cast<int>(lds[at]) - 128) * scale;
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t byte = is_v ? lds[(8 * slot + k) * V_ROW + v_place(t)] : ((k < 4 ? direct[i].x : direct[i].y) >> (8 * (k & 3))) & 0xFFu;
+      y[k] = block < 0 ? 0.0f : (static_cast<float>(byte) - 128.0f) * scale;
     }
     store8_f32<KIND>(dst, (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D + 8 * slot, y);
   }
+}
+
+// grid (units, heads, 2)
+template <int KIND, int D>
+__global__ void __launch_bounds__(THREADS) kv_read_kernel(ReadArgs a) {
+  __shared__ __align__(16) uint8_t lds[D * V_ROW];
+  if (blockIdx.z == 0) read_piece<KIND, D, false>(a, lds);
+  else read_piece<KIND, D, true>(a, lds);
 }
 
 // The cheaper of the two ways of cutting a batch into units (see Piece): `per_seq` blocks for every sequence where all
