@@ -12,8 +12,9 @@
 //
 // What bounds it.  A single token waits for its chain of loads (row, page, scale, block): 8 sequences, append 4.6 and read
 // 4.0 us.  Of prompts, 8244 tokens of 8 heads of 128 (50 MB in and out), reading back takes 11 us (4.6 TB/s, a large copy
-// 4.8; with K through LDS as well 13.9); appending takes 21, not by its bytes but by its stages: rows, norm and rotation, the largest magnitude, and only then the bytes (K
-// alone 18, V alone 11, both without the rotation 18; with the tokens in LDS as float32 and the angles shared, 26).
+// 4.8; with K through LDS as well 13.9); appending takes 21, not by its bytes but by its stages: rows, norm and rotation,
+// the largest magnitude, and only then the bytes (K alone 18, V alone 11, both without the rotation 18; with the tokens in
+// LDS as float32 and the angles shared, 26).
 
 #include <hip/hip_runtime.h>
 
@@ -141,11 +142,16 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
   const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   const void* src = is_v ? a.v : a.k;
   const int64_t stride = is_v ? a.v_stride : a.k_stride;
+  const bool turns = !is_v && 8 * slot < a.rotary_dim, interleaved = a.interleaved != 0;
   float y[PASSES][8];
+  int64_t position[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
     const int t = p.first + i * ROWS + sub;
-    if (t < p.last) load8_f32<KIND>(src, (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D + 8 * slot, y[i]);
+    if (t >= p.last) break;
+    load8_f32<KIND>(src, (p.row + (t - p.first)) * stride + static_cast<int64_t>(head) * D + 8 * slot, y[i]);
+    position[i] = (p.block << 5) + t;
+    if (turns && a.positions) position[i] = a.positions[p.row + (t - p.first)];
   }
   const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
   if (block < 0) return;
@@ -163,7 +169,6 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
     }
   }
   uint32_t amax_bits = 0;         // magnitudes order like their bits, infinity and NaN above all numbers
-  const bool turns = !is_v && 8 * slot < a.rotary_dim, interleaved = a.interleaved != 0;
   double freq[8];
   if (turns) {
     const float* from = a.inv_freq + first_pair(slot, a.rotary_dim, interleaved);
@@ -178,10 +183,9 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
     if constexpr (!is_v) {
       float2 cs[8];
       if (turns) {
-        const int64_t position = a.positions ? a.positions[p.row + (t - p.first)] : (p.block << 5) + t;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (k < 4 || !interleaved) cs[k] = rotation(position, freq[k], a.rope_scale);
+          if (k < 4 || !interleaved) cs[k] = rotation(position[i], freq[k], a.rope_scale);
       }
       norm_rotate8<D>(y[i], slot, a.k_weight, a.eps, [&](int k) { return cs[k]; }, a.rotary_dim, interleaved);
     }
