@@ -18,7 +18,8 @@
 // Scales.  K's block scale goes into the softmax's argument.  V's goes into P: with w = p * v_scale, w = exp2(s + log2
 // v_scale - m) for a maximum m over that sum, O = (sum w v_int) / (sum w / v_scale) - one more constant per block in an
 // addition that is there anyway, and P keeps its range whatever the scales are.  (Where scales lie far apart a block's w
-// can vanish while its p counts in the sum: `far` below.)
+// can vanish while its p counts in the sum: `far` below.  What fp16 holds to its 11 bits counts as rounded there too: with p
+// in its place a row whose weight lies on such a block was off by another 2^-11 of its value.)
 //
 // Splits.  Where rows are few, the keys of a sequence are cut into chunks for workgroups of their own, whose partial
 // maxima, sums and outputs go to a workspace and are joined by a second kernel in chunk order (no atomics).
@@ -46,6 +47,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEVER = -3e38f;        // a maximum before any key: finite, so that differences to it are no NaN
 constexpr float HEADROOM = 8.0f;       // attention_keys_kernel: log2 by which a row's maximum may pass its reference
 constexpr float RANGE = 32768.0f;      // attention_rows_kernel: sum of P above which it is moved (fp16 ends at 65504)
+constexpr _Float16 FULL = 6.103515625e-5f16;   // 2^-14: fp16 holds what is less to fewer than 11 bits
 constexpr float OFFSET = 7.0f;         // log2 of P at the reference: P <= 2^15, and fp16's least step is 2^-31 of it
 
 struct AttnArgs {
@@ -278,6 +280,13 @@ __device__ __forceinline__ Scales scales_of(const Blocks& b, int which, float& l
   return r;
 }
 
+__device__ __forceinline__ _Float16 least_of(const h8 (&w)[2]) {
+  const auto a = __builtin_elementwise_min(w[0], w[1]);
+  const auto b = __builtin_elementwise_min(__builtin_shufflevector(a, a, 0, 1, 2, 3), __builtin_shufflevector(a, a, 4, 5, 6, 7));
+  const h2 c = __builtin_elementwise_min(__builtin_shufflevector(b, b, 0, 1), __builtin_shufflevector(b, b, 2, 3));
+  return __builtin_elementwise_min(c.x, c.y);
+}
+
 // One block of the softmax of a column: raw products s of its 32 keys -> P, as the operand of O += V P, with the running
 // reference m and sum l.  rescale(f) multiplies O where the reference moves.
 template <int D, typename F>
@@ -307,35 +316,39 @@ __device__ __forceinline__ void softmax_block(f16v& s, const Column<D>& k, const
     l *= f;
     rescale(f);
   }
-  if (b.far) {
-    // w may be lost in fp16 although p counts in the sum, which then takes p itself, at the price of 16 more exponentials.
-    float e = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float p_i = __builtin_amdgcn_exp2f(fmaf(s[i], c, OFFSET - m));
-      e += !masked || sees(i) ? p_i : 0.0f;
-    }
-    l += e;
-  }
-  const float shift = b.lv - m + OFFSET;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift));
-  if (masked) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = sees(i) ? s[i] : 0.0f;
-  }
   // P is summed as rounded, its subnormals too (the dot product instruction would take those as 0): v_fma_mix_f32 with a
   // `one` that the compiler does not see through.
   float sum = 0.0f;
+  if (b.far) {
+    // Where w is lost in fp16 although p counts in the sum, that takes p itself; both from one exponential.
+    const float v = __builtin_amdgcn_exp2f(b.lv), shift = OFFSET - m;
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    const h2 r = __builtin_convertvector((f2v{s[i], s[i + 1]}), h2);
-    p[i >> 3][i & 7] = r.x;
-    p[i >> 3][(i & 7) + 1] = r.y;
-    sum = fmaf(static_cast<float>(r.x), one, sum);
-    sum = fmaf(static_cast<float>(r.y), one, sum);
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift));
+      if (masked) s[i] = sees(i) ? s[i] : 0.0f;
+      const _Float16 r = static_cast<_Float16>(s[i] * v);
+      p[i >> 3][i & 7] = r;
+      sum += r >= FULL ? static_cast<float>(r) * b.iv : s[i];      // (a NaN takes s, which is one too)
+    }
+    l += sum;
+  } else {
+    const float shift = b.lv - m + OFFSET;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, shift));
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = sees(i) ? s[i] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const h2 r = __builtin_convertvector((f2v{s[i], s[i + 1]}), h2);
+      p[i >> 3][i & 7] = r.x;
+      p[i >> 3][(i & 7) + 1] = r.y;
+      sum = fmaf(static_cast<float>(r.x), one, sum);
+      sum = fmaf(static_cast<float>(r.y), one, sum);
+    }
+    l = fmaf(sum, b.iv, l);
   }
-  l = fmaf(sum, b.far ? 0.0f : b.iv, l);
 }
 
 __device__ __forceinline__ float opaque_one() {
@@ -664,14 +677,18 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
         sum = weigh(s, c, lv - m + OFFSET, p);
       }
       lv_top = fmaxf(lv_top, b.lv);
-      if (b.lv < lv_top - 2.0f && b.lv > -__builtin_inff()) {
-        // V's scale is less than a quarter of the largest so far: w may be lost in fp16 although p counts in the sum, which
-        // then takes p itself, at the price of 16 more exponentials.
+      l = fmaf(sum, b.iv, l);
+      if (b.lv < lv_top - 2.0f && b.lv > -__builtin_inff() && (D == 256 || __any(least_of(p) < FULL))) {
+        // V's scale is less than a quarter of the largest so far, and some w may be lost in fp16 although p counts in the sum,
+        // which then takes p itself in their place, at the price of 16 more exponentials (8192 tokens whose scales lie up to
+        // 2^6 apart: 696 us against 671; looking first for such w costs D 256 more registers than there are).
         const float shift = none ? -__builtin_inff() : OFFSET - m;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) l += __builtin_amdgcn_exp2f(fmaf(s[i], c, shift));
-      } else {
-        l = fmaf(sum, b.iv, l);
+        for (int i = 0; i < 16; ++i) {
+          const _Float16 w = p[i >> 3][i & 7];
+          const float more = fmaf(-static_cast<float>(w), b.iv, __builtin_amdgcn_exp2f(fmaf(s[i], c, shift)));
+          l += w < FULL ? more : 0.0f;
+        }
       }
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {

@@ -586,3 +586,31 @@ def test_append_then_attend_as_a_request_runs(dev):
     assert (np.abs(values - keys.swapaxes(0, 1)) <= steps * 3.5).all()
     dev.free(*fixed)
     c.free()
+
+
+@pytest.mark.parametrize("dim,heads,group,rows,kv_len", [(64, 2, 4, 3, 200), (128, 1, 8, 60, 300), (256, 2, 8, 40, 200)])
+def test_weights_on_a_block_of_small_scale_are_counted_as_rounded(dev, dim, heads, group, rows, kv_len):
+    """Every query's weight lies nearly all on one key of block 4, whose V is small beside that of block 0: the output is that
+    key's value, and the rounding of its weight to fp16 leaves it there because the sum takes the weight as rounded. (With the
+    sum over unrounded weights it is off by up to 2^-11 of itself more than its own rounding.) A key of block 0 is there to set
+    the reference: at the reference a weight is a power of two."""
+    rng = np.random.default_rng(dim)
+    c = Cache(dev, rng, [kv_len], 32, heads, dim)
+    c.vs[c.table[0, 0]] *= 30
+    c.vs = c.vs.astype(np.float32).astype(np.float64)
+    dev.free(*c.bufs)
+    c.upload()
+    start, kv = np.array([0, rows], np.int32), np.array([kv_len], np.int32)
+    keys, _ = O.gather(c.k, c.ks, c.table[0], kv_len)
+    q = np.zeros((rows, heads * group, dim))
+    for i in range(rows):
+        for h in range(heads * group):
+            pair = keys[h // group][[128 + rng.integers(0, 32), rng.integers(0, 32)]]
+            logit = 45 + rng.uniform(0, 8)                 # in log2; the other's w is 1 to 6 octaves less
+            other = logit - np.log2(c.vs[c.table[0, 0], h // group, 0] / c.vs[c.table[0, 4], h // group, 0]) - rng.uniform(1, 6)
+            q[i, h] = pair.T @ np.linalg.solve(pair @ pair.T, np.array([logit, other]) * np.log(2) * dim ** 0.5)
+    q = O.round_to(q, "fp16")
+    got = O.from_bits(run_attention(dev, c, q, start, kv, rows, kv_len, heads * group, "fp16"), "fp16")
+    want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5)
+    assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "fp16", kv_len, dim, 127 * c.vs.max())).all()
+    c.free()
