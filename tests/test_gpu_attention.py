@@ -614,3 +614,54 @@ def test_weights_on_a_block_of_small_scale_are_counted_as_rounded(dev, dim, head
     want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5)
     assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "fp16", kv_len, dim, 127 * c.vs.max())).all()
     c.free()
+
+
+@pytest.mark.parametrize("dim,heads,group,page,rows,lens,window,kind", [
+    # 64 sequences of 8 heads: undivided, and the longest have 272 blocks for four waves, more than 64 each
+    (64, 8, 1, 32, [1] * 64, [8700, 8300] + [3 + i for i in range(62)], 0, "bf16"),
+    (128, 8, 1, 64, [1] * 64, [40] * 63 + [8500], 0, "fp16"),
+    (256, 4, 2, 64, [1] * 128, [17] * 127 + [8400], 8300, "bf16"),
+    # prompts of more than 64 rows a KV head, undivided: workgroups that walk over 72 to 150 blocks
+    (64, 8, 8, 32, [9] * 32, [2300] + [9 + 5 * i for i in range(30)] + [4800], 0, "fp16"),
+    (128, 8, 8, 64, [9] * 32, [2300] + [9] * 31, 0, "bf16"),
+    (128, 8, 8, 64, [9] * 32, [3000] + [9] * 31, 2200, "bf16"),
+    (256, 4, 8, 64, [20] * 63 + [9], [20] * 62 + [2300, 9], 0, "bf16"),              # eight waves
+])
+def test_attention_over_more_blocks_than_one_list_holds(dev, dim, heads, group, page, rows, lens, window, kind):
+    """A wave keeps the numbers and scales of 64 blocks at a time: sequences that need two and three such lists in one
+    workgroup, every block with scales of its own, some pages missing around the lists' ends."""
+    rng = np.random.default_rng(dim + group)
+    c = Cache(dev, rng, lens, page, heads, dim)
+    c.ks *= 2.0 ** rng.uniform(-1.5, 0.5, c.ks.shape)
+    c.vs *= 2.0 ** rng.uniform(-3, 3, c.vs.shape)
+    c.ks, c.vs = (x.astype(np.float32).astype(np.float64) for x in (c.ks, c.vs))
+    longest = int(np.argmax(lens))
+    for block in (63, 64, 255, 257, 260):                 # (of 32 tokens: the page that it lies on)
+        if block * 32 // page < c.table.shape[1]:
+            c.table[longest, block * 32 // page] = -1
+    dev.free(*c.bufs)
+    c.upload()
+    t, hq, start, kv = sum(rows), heads * group, _ragged(rows), np.array(lens, np.int32)
+    q = O.round_to(rng.standard_normal((t, hq, dim)) * 2.0, kind)
+    assert A.paged_attention_q8_workspace_bytes(t, len(lens), max(rows), max(lens), hq, heads, dim) == 0        # undivided
+    got = O.from_bits(run_attention(dev, c, q, start, kv, max(rows), max(lens), hq, kind, window=window), kind)
+    want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5, window=window)
+    tol = attention_tolerance(want, dv, mag, arg, kind, max(lens), dim, 127 * c.vs.max())
+    worst = np.abs(got - want) - tol
+    assert (worst <= 0).all(), (worst.max(), np.unravel_index(worst.argmax(), worst.shape))
+    c.free()
+
+
+@pytest.mark.parametrize("window", [300, 700, 1])
+def test_shares_of_eight_waves_within_a_window(dev, window):
+    """Prompts of D 256 that share the workgroups, each cut into parts of its own, seeing a window only."""
+    rng = np.random.default_rng(96)
+    rows, lens, dim, heads, group = [200, 64, 0, 331], [200, 1100, 0, 1331], 256, 2, 8
+    c = Cache(dev, rng, lens, 128, heads, dim)
+    start, kv = _ragged(rows), np.array(lens, np.int32)
+    q = O.round_to(rng.standard_normal((sum(rows), heads * group, dim)), "fp16")
+    want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5, window=window)
+    for max_q, max_kv in ((331, 1331), (400, 1 << 20)):
+        got = O.from_bits(run_attention(dev, c, q, start, kv, max_q, max_kv, heads * group, "fp16", window=window), "fp16")
+        assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "fp16", 1331, dim, 127 * c.vs.max())).all()
+    c.free()
