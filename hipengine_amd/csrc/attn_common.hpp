@@ -17,7 +17,7 @@
 namespace hipengine_gfx950 {
 
 constexpr int KV_BLOCK = 32;
-constexpr float KV_SCALE_FLOOR = 5.421010862427522e-20f;   // 2^-64: no block has a smaller scale
+constexpr float KV_SCALE_FLOOR = 5.421010862427522e-20f;   // 2^-64: what is less counts as this
 
 struct KvCacheQ8 {
   uint8_t* k;          // [pages, heads, page_size / 32, D * 32]
@@ -30,6 +30,9 @@ struct KvCacheQ8 {
   int heads;
   int page_log2;       // log2(page_size)
 };
+
+// A block's scale as it counts; a NaN stays one.
+__device__ __forceinline__ float kv_scale(float s) { return s < KV_SCALE_FLOOR ? KV_SCALE_FLOOR : s; }
 
 __device__ __forceinline__ int v_place(int t) { return (t & 3) | ((t >> 3 & 3) << 2) | ((t >> 2 & 1) << 4); }
 __device__ __forceinline__ int v_token(int p) { return (p & 3) | ((p >> 2 & 3) << 3) | ((p >> 4 & 1) << 2); }

@@ -159,7 +159,7 @@ __device__ __forceinline__ void append_piece(const AppendArgs& a, AppendLds<D>& 
   uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + block * (D * KV_BLOCK);
   float* scale_at = (is_v ? a.cache.v_scale : a.cache.k_scale) + block;
   float old = 0.0f;
-  if (threadIdx.x == 0 && p.first > 0) old = *scale_at;      // by the thread that will write it
+  if (threadIdx.x == 0 && p.first > 0) old = kv_scale(*scale_at);      // by the thread that will write it
   uint4 kept[ITEMS];
   if (is_v && !whole) {
 #pragma unroll
@@ -292,7 +292,7 @@ __device__ __forceinline__ void read_piece(const ReadArgs& a, uint8_t* lds) {
   Piece p;
   if (!find_piece(a.start, a.kv_lens, a.tokens, a.batch, a.per_seq, blockIdx.x, p)) return;
   const int64_t block = kv_block_index(a.cache, p.seq, p.block, head);
-  const float scale = block < 0 ? 0.0f : (is_v ? a.cache.v_scale : a.cache.k_scale)[block];
+  const float scale = block < 0 ? 0.0f : kv_scale((is_v ? a.cache.v_scale : a.cache.k_scale)[block]);
   const uint8_t* bytes = (is_v ? a.cache.v : a.cache.k) + max(block, int64_t{0}) * (D * KV_BLOCK);
   const int slot = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   uint2 direct[PASSES];

@@ -251,7 +251,7 @@ struct Blocks {
   __device__ __forceinline__ void scales(const KvCacheQ8& c) {
     const float v = c.v_scale[number], k = c.k_scale[number];
     const float v_clean = fmaxf(v, KV_SCALE_FLOOR);          // of a NaN: the floor
-    ks = !found ? 0.0f : fmaxf(k, k != k ? k : KV_SCALE_FLOOR);
+    ks = !found ? 0.0f : kv_scale(k);
     lv = !found ? -__builtin_inff() : v == v ? __builtin_amdgcn_logf(v_clean) : v;
     iv = !found ? 0.0f : 1.0f / v_clean;
   }

@@ -101,7 +101,7 @@ def append(k, v, k_int, v_int, k_scale, v_scale, table, q_start, kv_lens):
                 off = base % page_size
                 for h in range(ints.shape[1]):
                     new = x[row + first - at: row + last - at, h]
-                    old = scales[page, h, off // BLOCK] if first > base else 0.0
+                    old = float(counts_as(scales[page, h, off // BLOCK])) if first > base else 0.0
                     with np.errstate(invalid="ignore"):
                         bad = not np.isfinite(new).all() or np.isnan(old)
                         scale = np.nan if bad else max(old, np.abs(new).max() / 127.0, FLOOR)
@@ -117,6 +117,11 @@ def append(k, v, k_int, v_int, k_scale, v_scale, table, q_start, kv_lens):
     return touched
 
 
+def counts_as(scale):
+    """A block's scale as it counts: at least FLOOR; a NaN stays one."""
+    return np.where(scale < FLOOR, FLOOR, scale)
+
+
 def gather(ints, scales, table_row, length):
     """The cached values of a sequence [heads, length, dim] and which of its tokens are there."""
     pages, heads, size, dim = ints.shape
@@ -125,7 +130,7 @@ def gather(ints, scales, table_row, length):
         page = int(table_row[slot]) if slot < len(table_row) else -1
         a, b = slot * size, min(length, (slot + 1) * size)
         if 0 <= page < pages:
-            out[:, a:b] = (ints[page] * np.repeat(scales[page], BLOCK, axis=1)[..., None])[:, : b - a]
+            out[:, a:b] = (ints[page] * np.repeat(counts_as(scales[page]), BLOCK, axis=1)[..., None])[:, : b - a]
             there[a:b] = True
     return out, there
 

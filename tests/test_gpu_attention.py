@@ -665,3 +665,45 @@ def test_shares_of_eight_waves_within_a_window(dev, window):
         got = O.from_bits(run_attention(dev, c, q, start, kv, max_q, max_kv, heads * group, "fp16", window=window), "fp16")
         assert (np.abs(got - want) <= attention_tolerance(want, dv, mag, arg, "fp16", 1331, dim, 127 * c.vs.max())).all()
     c.free()
+
+
+def test_scales_under_the_least_count_as_the_least(dev):
+    """A scale below 2^-64 (0, negative, subnormal) stands for 2^-64 wherever the cache is looked at: reading back, the
+    earlier tokens of a block that is appended to, and attention. A NaN stays one."""
+    rng = np.random.default_rng(21)
+    dim, heads, page, lens = 64, 2, 32, [40, 20, 5]
+    c = Cache(dev, rng, lens, page, heads, dim)
+    for s in (c.ks, c.vs):
+        s[...] = np.array([0.0, 2.0 ** -70, -1.0, 2.0 ** -140])[rng.integers(0, 4, s.shape)]
+        s[c.table[2, 0], 1] = np.nan
+    dev.free(*c.bufs)
+    c.upload()
+    least = np.float32(O.FLOOR)
+    start, kv = _ragged(lens), np.array(lens, np.int32)
+    out = [dev.empty(sum(lens) * heads * dim * 4) for _ in range(2)]
+    ints = [dev.put(start), dev.put(kv)]
+    C.kv_read_q8(c.handle, out[0].ptr, out[1].ptr, *c.where, ints[0].ptr, ints[1].ptr, sum(lens), 3, out_kind="f32")
+    for buf, held, scales in ((out[0], c.k, c.ks), (out[1], c.v, c.vs)):
+        got = dev.get(buf, np.float32, (sum(lens), heads, dim))
+        for b, n in enumerate(lens):
+            for t in range(n):
+                pg, off = c.table[b, t // page], t % page
+                want = held[pg, :, off].astype(np.float32) * np.where(np.isnan(scales[pg, :, 0]), np.nan, least)[:, None].astype(np.float32)
+                assert np.array_equal(got[start[b] + t], want, equal_nan=True)
+    # one more token each: zeros to sequence 0, values of two steps of 2^-64 at most to sequence 1, anything to sequence 2
+    new = np.zeros((3, heads, dim), np.float32)
+    new[1] = np.float32(2.0 ** -63) * rng.integers(-127, 128, (heads, dim))
+    new[1, :, 0] = np.float32(127 * 2.0 ** -63)
+    new[2] = rng.standard_normal((heads, dim))
+    more = [dev.put(new), dev.put(_ragged([1, 1, 1])), dev.put(kv + 1)]
+    C.kv_append_q8(c.handle, more[0].ptr, more[0].ptr, *c.where, more[1].ptr, more[2].ptr, 3, 3, 1, in_kind="f32")
+    gk, gv, gks, gvs = c.download()
+    for got, gs, held in ((gk, gks, c.k), (gv, gvs, c.v)):
+        at = c.table[0, 1]
+        assert (gs[at] == least).all() and np.array_equal(got[at, :, :8], held[at, :, :8]) and (got[at, :, 8] == 0).all()
+        at = c.table[1, 0]
+        assert (gs[at] == 2 * least).all() and np.array_equal(got[at, :, :20], np.rint(held[at, :, :20] * 0.5))
+        assert np.array_equal(got[at, :, 20], np.rint(new[1] / np.float32(2.0 ** -63)))
+        assert np.isnan(gs[c.table[2, 0], 1]).all() and not np.isnan(gs[c.table[2, 0], 0]).any()
+    dev.free(*out, *ints, *more)
+    c.free()
