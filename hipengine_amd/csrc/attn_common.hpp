@@ -110,14 +110,25 @@ __device__ __forceinline__ void store8_f32(void* base, int64_t idx, const float 
 // ---- position rotation ---------------------------------------------------------------------------------------
 
 // cos and sin of position * inv_freq, times `scale`.  The product and its reduction to a fraction of a turn are in 64
-// bits: at position 10^6 a 32-bit product is off by a tenth of a radian.  The fraction goes to the sine and cosine
-// instructions, which take turns and are good to 1.25e-7 (measured over 2^22 fractions; sincospif is good to 5.1e-8 and takes
-// 40 instructions more).
+// bits: at position 10^6 a 32-bit product is off by a tenth of a radian.  For what is rounded to 16 or 8 bits behind it the
+// fraction goes in float32 (off by up to 2^-26 turns, 9.4e-8) to the sine and cosine instructions, which take turns and are
+// good to 1.25e-7 (measured over 2^22 fractions; sincospif is good to 5.1e-8 and takes 40 instructions more).  For float32
+// outputs (EXACT), whose half step is 6e-8, both are summed in 64 bits and rounded once: Taylor's series within an eighth of a
+// turn of the nearest quarter, good to 1e-11 (sincospi makes a launch of 8191 tokens 72 to 84 us, this one 58 to 60).
 __device__ __forceinline__ double turns_of(float inv_freq) { return static_cast<double>(inv_freq) * 0.15915494309189535; }
+template <bool EXACT = false>
 __device__ __forceinline__ float2 rotation(int64_t position, double turns, float scale) {
-  const double whole = static_cast<double>(position) * turns;
-  const float part = static_cast<float>(whole - rint(whole));   // -0.5 .. 0.5
-  return make_float2(__builtin_amdgcn_cosf(part) * scale, __builtin_amdgcn_sinf(part) * scale);
+  const double whole = static_cast<double>(position) * turns, part = whole - rint(whole);   // -0.5 .. 0.5
+  if constexpr (EXACT) {
+    const double quarter = rint(4.0 * part), x = (part - 0.25 * quarter) * 6.283185307179586, z = x * x;
+    const double s = x + x * z * (-1.0 / 6 + z * (1.0 / 120 + z * (-1.0 / 5040 + z * (1.0 / 362880 + z * (-1.0 / 39916800)))));
+    const double c = 1.0 + z * (-0.5 + z * (1.0 / 24 + z * (-1.0 / 720 + z * (1.0 / 40320 + z * (-1.0 / 3628800 + z * (1.0 / 479001600))))));
+    const int n = static_cast<int>(quarter);       // -2 .. 2
+    const double cosine = n & 1 ? s : c, sine = n & 1 ? c : s;
+    return make_float2(static_cast<float>(((n + 1) & 2 ? -cosine : cosine) * scale), static_cast<float>((n & 2 ? -sine : sine) * scale));
+  }
+  const float turn = static_cast<float>(part);
+  return make_float2(__builtin_amdgcn_cosf(turn) * scale, __builtin_amdgcn_sinf(turn) * scale);
 }
 
 // Sum over an aligned group of 8, 16 or 32 lanes, in all of them; no LDS.

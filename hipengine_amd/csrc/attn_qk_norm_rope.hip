@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_kernel(QkArgs a) {
     const int64_t next = t + gridDim.x;
     if (pairs > 0) {
       if (turns) {
-        turn[buffer][threadIdx.x] = rotation(position, freq, a.rope_scale);
+        turn[buffer][threadIdx.x] = rotation<OUT == KIND_F32>(position, freq, a.rope_scale);
         position = next < a.tokens ? a.positions[next] : 0;
       }
       __syncthreads();        // (two buffers: who is a token ahead writes the other one, and nobody gets further ahead)

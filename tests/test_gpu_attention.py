@@ -707,3 +707,25 @@ def test_scales_under_the_least_count_as_the_least(dev):
         assert np.isnan(gs[c.table[2, 0], 1]).all() and not np.isnan(gs[c.table[2, 0], 0]).any()
     dev.free(*out, *ints, *more)
     c.free()
+
+
+@pytest.mark.parametrize("dim,interleaved", [(128, False), (256, True), (64, False)])
+def test_rotation_into_float32_is_rounded_once(dev, dim, interleaved):
+    """Pairs (1, 0): the outputs are cos and sin of position * inv_freq as they are. A value of at most 1 rounded once is off
+    by half a step, 2^-25; the angle, up to 2^20 radians in float64 with three roundings of 2^-53 here and on the device each,
+    by 2^20 * 6 * 2^-53 < 2^-30."""
+    rng = np.random.default_rng(dim)
+    t = 700
+    freq = inv_freq(dim)
+    pos = np.sort(rng.integers(0, 1 << 20, t)).astype(np.int64)
+    x = np.zeros((t, dim), np.float32)
+    first = np.arange(0, dim, 2) if interleaved else np.arange(dim // 2)
+    x[:, first] = 1
+    bufs = [dev.put(x), dev.put(pos), dev.put(freq), dev.empty(x.nbytes)]
+    R.qk_norm_rope(bufs[0].ptr, None, bufs[3].ptr, None, t, 1, 0, dim, positions_ptr=bufs[1].ptr, inv_freq_ptr=bufs[2].ptr,
+                   rotary_dim=dim, interleaved=interleaved, in_kind="f32", out_kind="f32")
+    got = dev.get(bufs[3], np.float32, (t, dim)).astype(np.float64)
+    angle = pos[:, None].astype(np.float64) * freq.astype(np.float64)
+    for cols, want in ((first, np.cos(angle)), (first + (1 if interleaved else dim // 2), np.sin(angle))):
+        assert np.abs(got[:, cols] - want).max() <= 2.0 ** -25 + 2.0 ** -30
+    dev.free(*bufs)
