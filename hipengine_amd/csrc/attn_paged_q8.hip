@@ -677,17 +677,34 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
         sum = weigh(s, c, lv - m + OFFSET, p);
       }
       lv_top = fmaxf(lv_top, b.lv);
-      l = fmaf(sum, b.iv, l);
-      if (b.lv < lv_top - 2.0f && b.lv > -__builtin_inff() && (D == 256 || __any(least_of(p) < FULL))) {
-        // V's scale is less than a quarter of the largest so far, and some w may be lost in fp16 although p counts in the sum,
-        // which then takes p itself in their place, at the price of 16 more exponentials (8192 tokens whose scales lie up to
-        // 2^6 apart: 696 us against 671; looking first for such w costs D 256 more registers than there are).
-        const float shift = none ? -__builtin_inff() : OFFSET - m;
+      // Where V's scale is less than a quarter of the largest so far, some w may be lost in fp16 although p counts in the sum,
+      // which then takes p itself in their place, at the price of 16 more exponentials (8192 tokens whose scales lie up to 2^6
+      // apart: 703 us against 671).  Of D 256 there are no registers to look for such w first, nor to take them off the sum
+      // afterwards (512 tokens 39.4 us against 38.3, whatever the scales).
+      const bool far = b.lv < lv_top - 2.0f && b.lv > -__builtin_inff();
+      const float p_shift = none ? -__builtin_inff() : OFFSET - m;
+      if constexpr (D == 256) {
+        if (far) {
+          float add = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const _Float16 w = p[i >> 3][i & 7];
-          const float more = fmaf(-static_cast<float>(w), b.iv, __builtin_amdgcn_exp2f(fmaf(s[i], c, shift)));
-          l += w < FULL ? more : 0.0f;
+          for (int i = 0; i < 16; ++i) {
+            const _Float16 w = p[i >> 3][i & 7];
+            const float p_i = __builtin_amdgcn_exp2f(fmaf(s[i], c, p_shift));
+            add += w < FULL ? p_i : static_cast<float>(w) * b.iv;
+          }
+          l += add;
+        } else {
+          l = fmaf(sum, b.iv, l);
+        }
+      } else {
+        l = fmaf(sum, b.iv, l);
+        if (far && __any(least_of(p) < FULL)) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const _Float16 w = p[i >> 3][i & 7];
+            const float more = fmaf(-static_cast<float>(w), b.iv, __builtin_amdgcn_exp2f(fmaf(s[i], c, p_shift)));
+            l += w < FULL ? more : 0.0f;
+          }
         }
       }
 #pragma unroll
