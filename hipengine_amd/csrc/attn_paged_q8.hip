@@ -43,6 +43,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr int WAVES = 4;               // of a workgroup (of attention_rows_kernel also twice as many)
 constexpr int MAX_KV = 1 << 30;
+constexpr int least_rows(int dim) { return 2048 / dim; }   // fewest blocks in a part of a prompt's keys
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEVER = -3e38f;        // a maximum before any key: finite, so that differences to it are no NaN
 constexpr float HEADROOM = 8.0f;       // attention_keys_kernel: log2 by which a row's maximum may pass its reference
@@ -63,7 +64,7 @@ struct AttnArgs {
   int q_heads;
   int window;
   int splits;             // most chunks of keys
-  int chunk;              // fewest blocks of 32 keys in a chunk
+  int chunk;              // fewest blocks of 32 keys in a chunk; 0: of a prompt by itself, see chunk_of
   // Of several prompts in parts:
   int32_t* parts;         // [batch] chunks of each sequence; else null
   int items, tiles;       // workgroups for a KV head, and for a sequence's rows at most
@@ -104,6 +105,13 @@ __device__ __forceinline__ float read_lane_f(float v, int lane) {
   return bits_to_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(float_to_bits(v)), lane)));
 }
 
+// Blocks that some tile of a sequence can see, at most.
+template <typename T>
+__host__ __device__ __forceinline__ T blocks_of(T kv_len, T q_len, T window) {
+  const T all = (kv_len + 31) / 32, near = (window + q_len + 62) / 32 + 1;      // (a window may begin anywhere in a block)
+  return window > 0 && near < all ? near : all;
+}
+
 // The keys that a query sees: places [lower, limit).
 struct Sight {
   int kv_len, q_len, window;
@@ -111,9 +119,19 @@ struct Sight {
   __device__ __forceinline__ int lower(int query) const { return window > 0 ? max(kv_len - q_len + query + 1 - window, 0) : 0; }
 };
 
-// Blocks in each of a tile's chunks, from the blocks that it sees: the announced lengths only say how many chunks there may
-// be, so that a call captured for the longest cache cuts a short one as finely.
-__device__ __forceinline__ int chunk_of(const AttnArgs& a, int parts, int blocks) { return max((blocks + parts - 1) / parts, a.chunk); }
+// Blocks in each of a tile's chunks, at most `parts` of them, from the keys that there are: the announced lengths only say how
+// many chunks there may be, so that a call captured for the longest cache cuts a short one as finely.  All tiles of a prompt by
+// itself have the same chunks, so that they read a block at the same time, and no more of them than have least_rows() blocks each
+// (512 tokens behind 8000, D 128, announced for 131072: 129 us, as announced for 8512; with chunks of the announced length 231).
+// (Made uniform by hand: the quotient comes from vector registers, of which D 256 has none to spare.)
+template <int D, bool KEYS = false>
+__device__ __forceinline__ int chunk_of(const AttnArgs& a, const Sight& sight, int parts, int blocks) {
+  if (!KEYS && a.chunk == 0) {
+    blocks = blocks_of(sight.kv_len, sight.q_len, a.window);
+    parts = max(min(parts, (blocks + least_rows(D) - 1) / least_rows(D)), 1);
+  }
+  return __builtin_amdgcn_readfirstlane(max((blocks + parts - 1) / parts, KEYS ? a.chunk : max(a.chunk, 1)));
+}
 
 // Which part of which tile a workgroup works on.
 struct Share {
@@ -412,7 +430,7 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
   const int lim_first = sight.limit(first_q), lo_last = sight.lower(last_q);
   int blk = sight.lower(first_q) >> 5, blk_end = (sight.limit(last_q) + 31) >> 5;
   if (a.splits > 1) {
-    const int chunk = chunk_of(a, a.splits, blk_end - blk);
+    const int chunk = chunk_of<D, true>(a, sight, a.splits, blk_end - blk);
     blk += split * chunk;
     blk_end = min(blk_end, blk + chunk);
   }
@@ -559,7 +577,7 @@ __global__ void __launch_bounds__(W * 64, D <= 128 ? 3 : 2) attention_rows_kerne
   int blk = sight.lower(tile0 / a.group) >> 5;
   int blk_end = (sight.limit((min(tile0 + TILE, n_rows) - 1) / a.group) + 31) >> 5;
   if (share.parts > 1) {
-    const int chunk = chunk_of(a, share.parts, blk_end - blk);
+    const int chunk = chunk_of<D>(a, sight, share.parts, blk_end - blk);
     blk += share.split * chunk;
     blk_end = min(blk_end, blk + chunk);
   }
@@ -740,7 +758,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttnArgs a, int tile_rows) {
   const Sight sight{min(max(a.kv_lens[seq], 0), MAX_KV), static_cast<int>(rows.count), a.window};
   const int row = query * a.group + q_head % a.group;
   const int tile0 = row / tile_rows * tile_rows, last_q = (min(tile0 + tile_rows, static_cast<int>(rows.count) * a.group) - 1) / a.group;
-  const int first = sight.lower(tile0 / a.group) >> 5, chunk = chunk_of(a, parts, ((sight.limit(last_q) + 31) >> 5) - first);
+  const int first = sight.lower(tile0 / a.group) >> 5, chunk = chunk_of<D>(a, sight, parts, ((sight.limit(last_q) + 31) >> 5) - first);
   const int blocks = max(((sight.limit(query) + 31) >> 5) - first, 0), splits = (blocks + chunk - 1) / chunk;
   const int64_t at = (rows.first + query) * a.q_heads + q_head, pitch = a.tokens * a.q_heads;
   float m = NEVER;
@@ -805,7 +823,7 @@ struct Plan {
   int splits;         // most parts of a tile's keys
   int most_splits;    // what the workspace is sized for: no fewer for fewer keys
   int typical;        // parts where all sequences are as long as announced
-  int chunk, least;   // fewest blocks in a part of a sequence by itself, and where sequences share workgroups
+  int chunk, least;   // as in AttnArgs
   bool shares;        // several prompts in parts
   int64_t items;      // their workgroups a KV head
 };
@@ -823,7 +841,7 @@ void cut(Plan& p, int64_t rows, int64_t blocks, int64_t batch, int64_t kv_heads,
   p.splits = p.most_splits = static_cast<int>(up_to < most ? up_to : most);
   p.shares = !p.keys && batch > 1 && p.splits > 1;
   p.least = static_cast<int>(least);
-  p.chunk = p.shares ? 1 : p.keys ? p.least : static_cast<int>((blocks + p.splits - 1) / p.splits);
+  p.chunk = p.keys ? p.least : p.shares ? 1 : 0;
   p.items = slots / kv_heads > batch * p.tiles ? slots / kv_heads : batch * p.tiles;
 }
 
@@ -831,17 +849,13 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
   Plan p;
   const int64_t rows = max_q * (q_heads / kv_heads);
   p.keys = rows <= 64;
-  // Keys that a tile can see.
-  int64_t span = max_kv;
-  if (window > 0 && window + max_q + 31 < span) span = window + max_q + 31;
-  int64_t blocks = (span + 31) / 32;
-  if (blocks < (max_kv + 31) / 32) ++blocks;      // (a window may begin anywhere in a block)
+  const int64_t blocks = blocks_of(max_kv, max_q, window);
   // Two workgroups a CU.  With a workgroup a CU from the rows alone, prompts are not split (they would be joined for less
   // than they gain: 2048 tokens, 640 tiles, 72 us as they are and 97 us in two parts).  A part of a prompt has at least
   // LEAST_ROWS and one of few rows, whose keys four waves share, at least LEAST_KEYS: a single token behind 600 others (19
   // blocks of 128) takes 14.4 us undivided and 17.3 us in two parts and the joining of them, behind 32768 others 22 us in
   // 32 parts and 26 us in 64; 512 tokens of D 128 (16 blocks) 23 us undivided and 35 us in two, of D 256 40 and 38 us.
-  const int64_t LEAST_KEYS = 4096 / dim, LEAST_ROWS = 2048 / dim;
+  const int64_t LEAST_KEYS = 4096 / dim, LEAST_ROWS = least_rows(static_cast<int>(dim));
   p.waves = WAVES;
   p.tile_rows = p.keys ? 32 : 32 * WAVES;
   cut(p, rows, blocks, batch, kv_heads, 2 * CUS, p.keys ? LEAST_KEYS : LEAST_ROWS);

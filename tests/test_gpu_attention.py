@@ -729,3 +729,27 @@ def test_rotation_into_float32_is_rounded_once(dev, dim, interleaved):
     for cols, want in ((first, np.cos(angle)), (first + (1 if interleaved else dim // 2), np.sin(angle))):
         assert np.abs(got[:, cols] - want).max() <= 2.0 ** -25 + 2.0 ** -30
     dev.free(*bufs)
+
+
+@pytest.mark.parametrize("dim,heads,group,rows,kv_len,window,longer", [
+    (128, 2, 8, 100, 4000, 0, (9000, 1 << 17, 1 << 30)),
+    (64, 8, 4, 64, 3000, 0, (1 << 15, 1 << 20)),
+    (256, 2, 8, 60, 2500, 0, (5000, 10000)),
+    (128, 2, 8, 100, 300, 0, (4000, 1 << 17)),            # fewer blocks than two parts have
+    (128, 2, 8, 100, 6000, 2500, (1 << 17,)),
+    (128, 2, 8, 100, 60, 0, (1 << 17,)),                  # rows that see nothing
+])
+def test_one_prompt_is_cut_by_the_keys_that_there_are(dev, dim, heads, group, rows, kv_len, window, longer):
+    """The parts that a prompt's keys are cut into follow the length at run time: announced for a longer cache the call gives
+    the same bits, being joined from the same parts."""
+    rng = np.random.default_rng(95)
+    c = Cache(dev, rng, [kv_len], 64, heads, dim)
+    start, kv = np.array([0, rows], np.int32), np.array([kv_len], np.int32)
+    q = O.round_to(rng.standard_normal((rows, heads * group, dim)), "bf16")
+    exact = run_attention(dev, c, q, start, kv, rows, kv_len, heads * group, "bf16", window=window)
+    want, dv, mag, arg = O.attention(q, c.k, c.v, c.ks, c.vs, c.table, start, kv, scale=dim ** -0.5, window=window)
+    tol = attention_tolerance(want, dv, mag, arg, "bf16", kv_len, dim, 127 * c.vs.max())
+    assert (np.abs(O.from_bits(exact, "bf16") - want) <= tol).all()
+    for max_kv in longer:
+        assert np.array_equal(run_attention(dev, c, q, start, kv, rows, max_kv, heads * group, "bf16", window=window), exact)
+    c.free()
