@@ -875,13 +875,15 @@ Plan plan_of(int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int6
 }
 
 constexpr int BAD = static_cast<int>(hipErrorInvalidValue);
+constexpr int64_t MAX_TILES = 65535;   // of a sequence: the grid's second dimension
 
+// The rows of D 256 that are more than MAX_TILES tiles of four waves are tiles of eight (they fill the chip).
 bool shape_ok(int64_t tokens, int64_t batch, int64_t max_q, int64_t max_kv, int64_t q_heads, int64_t kv_heads, int64_t dim,
               int64_t window) {
   return tokens > 0 && batch > 0 && batch <= 65535 && max_q > 0 && max_kv >= 0 && max_kv <= MAX_KV && kv_heads > 0 &&
          kv_heads <= 65535 && q_heads > 0 && q_heads % kv_heads == 0 && q_heads <= 4096 &&
          (dim == 64 || dim == 128 || dim == 256) && window >= 0 && window <= (1 << 30) && tokens <= (1 << 26) &&
-         max_q * (q_heads / kv_heads) <= (1 << 30);
+         (max_q < tokens ? max_q : tokens) * (q_heads / kv_heads) <= MAX_TILES * 32 * (dim == 256 ? 2 * WAVES : WAVES);
 }
 
 int64_t workspace_of(bool keys, int splits, int64_t tokens, int64_t batch, int64_t q_heads, int64_t dim) {
@@ -945,7 +947,6 @@ extern "C" int hipengine_gfx950_paged_attention_q8(const void* q, void* out, int
   const Plan p = plan_of(batch, longest, max_kv_len, q_heads, kv_heads, head_dim, window);
   const int64_t need = workspace_of(p.keys, p.splits, tokens, batch, q_heads, head_dim);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return BAD;
-  if (p.tiles > 65535 || batch * p.splits > 65535) return BAD;
   const KvCacheQ8 cache{const_cast<uint8_t*>(k_cache), const_cast<uint8_t*>(v_cache), const_cast<float*>(k_scale),
                         const_cast<float*>(v_scale), page_table, table_stride, pages, static_cast<int>(kv_heads),
                         63 - __builtin_clzll(static_cast<unsigned long long>(page_size))};

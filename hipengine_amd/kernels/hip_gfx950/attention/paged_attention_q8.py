@@ -30,6 +30,12 @@ from hipengine_amd.kernels.registry import KernelKey, register
 _ARGS = [VOID, VOID, I32, I64, I64] + [VOID] * 5 + [I64] + [VOID] * 2 + [I64] * 9 + [F32, I64, VOID, I64, VOID]
 _WORKSPACE_ARGS = [I64] * 7 + [ctypes.POINTER(I64)]
 
+_MOST_ROWS = 65535 * 128            # of a sequence and KV head; twice as many of head_dim 256
+
+
+def _rows_fit(tokens: int, max_q_len: int, q_heads: int, kv_heads: int, head_dim: int) -> bool:
+    return min(max_q_len, tokens) * (q_heads // kv_heads) <= (2 * _MOST_ROWS if head_dim == 256 else _MOST_ROWS)
+
 
 def _check_shape(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int, kv_heads: int, head_dim: int) -> None:
     check_positive(tokens=tokens, batch=batch, max_q_len=max_q_len, q_heads=q_heads, kv_heads=kv_heads)
@@ -41,6 +47,9 @@ def _check_shape(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_hea
     if q_heads % kv_heads != 0 or q_heads > 4096:
         raise ValueError("q_heads must be a multiple of kv_heads, at most 4096")
     check_head_dim(head_dim)
+    if not _rows_fit(tokens, max_q_len, q_heads, kv_heads, head_dim):
+        raise ValueError("a sequence may have at most 65535 * 128 rows (tokens * query heads) for each KV head, "
+                         "65535 * 256 of head_dim 256: attend to a longer prompt in chunks")
 
 
 def paged_attention_q8_workspace_bytes(tokens: int, batch: int, max_q_len: int, max_kv_len: int, q_heads: int,
@@ -82,6 +91,7 @@ def paged_attention_q8(cache: KVCacheQ8, q_ptr: int, out_ptr: int, page_table_pt
             and 0 < q_heads <= 4096 and q_heads % kv_heads == 0 and table_stride > 0 and (kind == "bf16" or kind == "fp16")
             and (scale is None or 0.0 < scale < math.inf) and 0 <= window <= 1 << 30
             and (q_stride == 0 or q_stride >= width) and (out_stride == 0 or out_stride >= width) and q_ptr != out_ptr
+            and (tokens * q_heads <= _MOST_ROWS or _rows_fit(tokens, max_q_len, q_heads, kv_heads, head_dim))
             and are_pointers(q_ptr, out_ptr, page_table_ptr, q_start_ptr, kv_lens_ptr)):
         _check_shape(tokens, batch, max_q_len, max_kv_len, q_heads, kv_heads, head_dim)
         check_positive(table_stride=table_stride)

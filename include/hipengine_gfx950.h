@@ -901,7 +901,8 @@ int hipengine_gfx950_moe_tile_map(const int64_t* expert_start_compact, int64_t* 
  *   batch           at most 65535
  *   kv_lens         int32 [batch]: tokens in sequence b's cache, its rows of this call (the last ones) included.
  *                   A sequence may have no rows, and no tokens.
- *   max_q_len, max_kv_len  at least the longest sequence's rows / cached tokens (any larger value is right, too)
+ *   max_q_len, max_kv_len  at least the longest sequence's rows / cached tokens; larger values are right, too (max_q_len
+ *                   counts as `tokens` at most; max_kv_len is at most 2^30)
  * ------------------------------------------------------------------------ */
 
 /* RMS norm of every head (weight float32 [head_dim]; null: none) and rotation of q [tokens, q_heads, head_dim] and
@@ -919,7 +920,8 @@ int hipengine_gfx950_qk_norm_rope(const void* q, const void* k, const float* q_w
  * the new tokens and its earlier tokens are rescaled then; a block whose first token is appended starts anew; bytes behind
  * the new tokens stay as they were.  Rows at negative places (more rows than kv_lens[b]) are left out.  A NaN or infinity
  * makes its block's scale NaN until the block starts anew.  Within one call no block may be appended to under two
- * names (two sequences, or a page twice in one table): whose tokens it then holds is not defined. */
+ * names (two sequences, or a page twice in one table): whose tokens it then holds is not defined.  Here and in the read,
+ * tokens / 32 + 2 * batch is at most 8388607. */
 int hipengine_gfx950_kv_append_q8(const void* k, const void* v, int32_t in_kind, int64_t k_stride, int64_t v_stride,
                                   const float* k_weight, const int64_t* positions, const float* inv_freq,
                                   int64_t rotary_dim, int32_t interleaved, float eps, float rope_scale, uint8_t* k_cache,
@@ -940,7 +942,10 @@ int hipengine_gfx950_kv_read_q8(const uint8_t* k_cache, const uint8_t* v_cache, 
 /* out = softmax(softmax_scale * q K^T) V for q, out [tokens, q_heads, head_dim], bf16 or fp16 (`kind`, of both).  The query
  * in row i of n of sequence b is at place kv_lens[b] - n + i and sees the places up to its own (window > 0: the last
  * `window` of them); q head h reads KV head h / (q_heads / kv_heads).  A query that sees nothing gives zeros; rows of no
- * sequence are left as they were.  `workspace` (16-byte aligned, the size that the function below gives for the same
+ * sequence are left as they were.  K, V and bf16 or fp16 q go into the products as they are, the softmax's weights rounded
+ * to fp16 (and counted so in their sum), products, sums and statistics in float32.  At most 2^26 tokens, 4096 query heads, a
+ * window of 2^30, and 65535 * 128 rows (65535 * 256 of head_dim 256) of a sequence for a KV head: min(max_q_len, tokens) *
+ * (q_heads / kv_heads).  `workspace` (16-byte aligned, the size that the function below gives for the same
  * sizes; null if 0) is scratch: calls that overlap in time need one each.  Results do not depend on timing. */
 int hipengine_gfx950_paged_attention_q8(const void* q, void* out, int32_t kind, int64_t q_stride, int64_t out_stride,
                                         const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale,

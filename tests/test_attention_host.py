@@ -281,3 +281,34 @@ def test_statement_of_sampling():
     assert one(row, 0.99, temperature=0) == 1 and one(np.full(3, -np.inf), 0.5) == -1
     assert np.isclose(O.sample(row, 0.0)[0][0], math.log(1 / 12))
     assert set(O.sample(row, 1 / 12 + 1e-9, accuracy=1e-6)) == {0, 1}    # on the border between the first two tokens
+
+
+# ---- limits of attention's sizes ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("tokens,max_q,q_heads,kv_heads,dim,fits", [
+    (1 << 20, 1 << 20, 7, 1, 128, True),
+    (1048560, 1048560, 8, 1, 128, True), (1048561, 1048561, 8, 1, 128, False),     # 65535 * 128 rows, and a token more
+    (1 << 20, 1 << 20, 8, 1, 64, False), (1 << 26, 1 << 26, 16, 16, 64, False),
+    (1 << 20, 1 << 20, 8, 1, 256, True), (2097120, 2097120, 8, 1, 256, True), (2097121, 2097121, 8, 1, 256, False),
+    (1 << 20, 1000, 8, 1, 64, True),                                               # many short sequences
+    (5, 1 << 40, 40, 8, 128, True), (1, 2**62, 4096, 1, 64, True),                 # announced for more rows than there are
+])
+def test_rows_of_a_sequence_that_fit(tokens, max_q, q_heads, kv_heads, dim, fits):
+    """The workspace function, the launch and both wrappers agree on what they take."""
+    fn = load_library().hipengine_gfx950_paged_attention_q8_workspace_bytes
+    fn.argtypes = A._WORKSPACE_ARGS
+    sizes = (tokens, 1, max_q, 4096, q_heads, kv_heads, dim)
+    assert fn(*sizes, ctypes.byref(ctypes.c_int64())) == (0 if fits else 1)
+    call = dict(ATTEND, tokens=tokens, batch=1, max_q_len=max_q, max_kv_len=4096, q_heads=q_heads)
+    small = cache(kv_heads=kv_heads, head_dim=dim)
+    if fits:
+        assert A.paged_attention_q8_workspace_bytes(*sizes) >= 0
+        with pytest.raises(AssertionError, match="was reached"):
+            A.paged_attention_q8(small, **call, library=Never())
+    else:
+        assert _attend(tokens=tokens, batch=1, maxq=max_q, maxkv=4096, hq=q_heads, hk=kv_heads, dim=dim, ws=4096, wsb=1 << 62) == 1
+        with pytest.raises(ValueError, match="65535"):
+            A.paged_attention_q8_workspace_bytes(*sizes)
+        with pytest.raises(ValueError, match="65535"):
+            A.paged_attention_q8(small, **call, library=Never())

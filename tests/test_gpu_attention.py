@@ -753,3 +753,16 @@ def test_one_prompt_is_cut_by_the_keys_that_there_are(dev, dim, heads, group, ro
     for max_kv in longer:
         assert np.array_equal(run_attention(dev, c, q, start, kv, rows, max_kv, heads * group, "bf16", window=window), exact)
     c.free()
+
+
+def test_attention_announced_for_more_rows_than_there_are(dev):
+    """max_q_len counts as the batch's tokens at most."""
+    rng = np.random.default_rng(98)
+    rows, lens, dim, heads, group = [1, 30], [300, 70], 128, 2, 40
+    c = Cache(dev, rng, lens, 64, heads, dim)
+    start, kv = _ragged(rows), np.array(lens, np.int32)
+    q = O.round_to(rng.standard_normal((31, heads * group, dim)), "bf16")
+    want = run_attention(dev, c, q, start, kv, 31, 300, heads * group, "bf16")
+    for max_q in (1 << 20, 1 << 30, 1 << 40):
+        assert np.array_equal(run_attention(dev, c, q, start, kv, max_q, 300, heads * group, "bf16"), want)
+    c.free()
