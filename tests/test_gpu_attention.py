@@ -766,3 +766,42 @@ def test_attention_announced_for_more_rows_than_there_are(dev):
     for max_q in (1 << 20, 1 << 30, 1 << 40):
         assert np.array_equal(run_attention(dev, c, q, start, kv, max_q, 300, heads * group, "bf16"), want)
     c.free()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_poisoned_block_stays_so_until_it_starts_anew(dev, which, bad):
+    """A NaN or infinity in one token of K or V: finite tokens behind it leave the scale NaN, whatever their size, and reading
+    gives NaN; once its first token is appended again the block is as good as any."""
+    rng = np.random.default_rng(23)
+    dim, heads, page = 64, 2, 32
+    c = Cache(dev, rng, [70], page, heads, dim)
+    start, one = dev.put(np.array([0, 2], np.int32)), dev.put(np.array([0, 1], np.int32))
+
+    def append(x, end, rows):
+        bufs = [dev.put(y.astype(np.float32)) for y in x] + [dev.put(np.array([end], np.int32))]
+        C.kv_append_q8(c.handle, bufs[0].ptr, bufs[1].ptr, *c.where, (start if rows == 2 else one).ptr, bufs[2].ptr, rows, 1, rows, in_kind="f32")
+        dev.sync()
+        dev.free(*bufs)
+        return c.download()
+
+    x = rng.standard_normal((2, 2, heads, dim))
+    x[which, 1, 1, 7] = bad
+    append(x, 34, 2)                                       # places 32, 33
+    pg = c.table[0, 1]
+    for end, size in ((35, 1.0), (36, 0.0), (37, 1e30)):
+        got = append(rng.standard_normal((2, 1, heads, dim)) * size, end, 1)
+        scales, other = got[2 + which], got[3 - which]
+        assert np.isnan(scales[pg, 1, 0]) and np.isfinite(scales[pg, 0, 0]) and np.isfinite(other[pg]).all()
+    out, lens, full = dev.empty(37 * heads * dim * 4), dev.put(np.array([37], np.int32)), dev.put(np.array([0, 37], np.int32))
+    C.kv_read_q8(c.handle, *((out.ptr, None) if which == 0 else (None, out.ptr)), *c.where, full.ptr, lens.ptr, 37, 1, out_kind="f32")
+    nan = np.isnan(dev.get(out, np.float32, (37, heads, dim)))
+    assert nan[32:, 1].all() and not nan[:32].any() and not nan[:, 0].any()
+    x = rng.standard_normal((2, 1, heads, dim))
+    gk, gv, gks, gvs = append(x, 33, 1)
+    for g, gs, y in ((gk, gks, x[0, 0]), (gv, gvs, x[1, 0])):
+        scale = np.abs(y.astype(np.float32)).max(-1) / np.float32(127)
+        assert np.array_equal(gs[pg, :, 0], scale)
+        assert np.array_equal(g[pg, :, 0], np.rint(y.astype(np.float32) / scale[:, None]))
+    dev.free(start, one, out, lens, full)
+    c.free()

@@ -183,3 +183,28 @@ def test_small_workspace_is_refused(dev):
             S.sample_f32_rows_i32(bufs[0].ptr, bufs[1].ptr, bufs[2].ptr, 2, 1000, workspace_ptr=ptr, workspace_bytes=size)
     assert (dev.get(bufs[2], np.uint8, (8,)) == 0xA5).all()
     dev.free(*bufs)
+
+
+@pytest.mark.parametrize("vocab", [262145, 400003, 1 << 20, 1 << 22])
+@pytest.mark.parametrize("settings", [dict(), dict(top_p=0.9, temperature=0.8), dict(top_k=50, top_p=0.95), dict(top_k=3000, min_p=0.001)],
+                         ids=lambda s: ",".join(f"{k}={v}" for k, v in s.items()) or "none")
+def test_vocabularies_of_many_chunks(dev, vocab, settings):
+    """More chunks than a wave has lanes, and than the borders' kernel adds up at once, up to the 1024 that there can be."""
+    rng = np.random.default_rng(vocab + len(settings))
+    rows = 2 if vocab < 1 << 20 else 1
+    logits = (rng.standard_normal((rows, vocab)) * 2.5).astype(np.float32)
+    for u in (0.02, 0.985):
+        check(dev, logits, [u] * rows, borders=rows, **settings)
+
+
+@pytest.mark.parametrize("vocab", [400003, 1 << 22])
+def test_flat_rows_of_many_chunks(dev, vocab):
+    """The largest sums that there are: every weight is the largest, 2^40, and the answer is known."""
+    logits = np.full((1, vocab), -3.5, np.float32)
+    for u in (0.0, 0.25, 0.7501, 0.99999):
+        u = float(np.float32(u))
+        ids, logprobs = run(dev, logits, [u])
+        assert ids[0] == int(u * vocab) and abs(logprobs[0] + np.log(vocab)) <= 2.0 ** -20
+        kept = int(np.ceil(0.5 * vocab))                   # by top-p, then by top-k: the first so many by index
+        assert run(dev, logits, [u], top_p=0.5)[0][0] == int(u * kept)
+        assert run(dev, logits, [u], top_k=300000)[0][0] == int(u * 300000)
