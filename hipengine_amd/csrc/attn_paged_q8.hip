@@ -413,9 +413,11 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const SeqRows& r
 // ---- few rows: the four waves of a workgroup share 32 rows and take blocks of keys in turn --------------------------
 // grid (KV heads, row tiles, batch * splits).  Nothing passes through LDS but the waves' join at the end.  With work for
 // every CU it is bound by the cache's bytes, K's and V's next blocks being on their way while one is worked on: 8
-// sequences of about 30000 tokens, 8 heads of 128, 276 MB in 63 us, 4.4 TB/s (a large copy: 4.8); 64 of about 7500 of
-// D 64, 278 MB in 59 us.  A short call is bound by its chain of loads (lengths, page, block) and two launches: 600 tokens
-// 10.4 us.
+// sequences of 900 to 32767 tokens (16800 on average), 8 heads of 128, 276 MB in 59 us, 4.7 TB/s (a large copy: 4.8), and 5
+// for the join; 64 of 300 to 8192 of D 64, 278 MB in 64 us.  A short call is bound by its chain of loads (lengths, page,
+// block) and the steps behind it, one after the other: 600 tokens, 19 blocks in five steps of the waves, 10.3 us.
+// All sequences get as many parts, whatever their lengths, and one each where sequences times KV heads are 512 or more: 64 of 8
+// heads of 128, one of 32768 tokens and 63 of 200 to 296, take 201 us, ten times what their bytes do.
 template <int D, int KIND>
 __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_kernel(AttnArgs a) {
   constexpr int KC = D / 32;           // 16-byte loads of K a lane, and tiles of 32 dims of V
@@ -542,9 +544,9 @@ __global__ void __launch_bounds__(WAVES * 64, D <= 128 ? 2 : 1) attention_keys_k
 // There is no running maximum: P is taken against the reference as it is, and only where a column's sum says that P has
 // grown out of its range is the maximum looked for, the reference moved and P taken again.
 //
-// What bounds it: 8192 tokens, 40 / 8 heads of 128, 695 us (0.99 PFLOP/s; a large bf16 product: 1.37): vector instructions
-// 63 % and matrix instructions 51 % of the cycles, at 2.05 GHz.  Of D 256 it is the occupancy, two waves a SIMD, which wait
-// for each other at the barrier: 0.6 PFLOP/s.
+// What bounds it: 8192 tokens, 40 / 8 heads of 128, 674 to 720 us (0.95 to 1.02 PFLOP/s; a large bf16 product: 1.37): vector
+// instructions 66 % and matrix instructions 53 % of the cycles, at 2.05 GHz.  Of D 256 it is the occupancy, two waves a SIMD,
+// which wait for each other at the barrier (45 % of a wave's time; matrix instructions 44 % of the cycles): 0.6 PFLOP/s.
 // Four waves, three such workgroups a CU, let one wave's softmax run in another's products.  Measured and not taken: eight
 // waves (half the conversions a wave, but two waves a SIMD) 717 to 735 us, with half of them half a step behind the others
 // 786 to 802; products of the next block behind the softmax of this one (250 registers, two waves a SIMD) 765 to 780; 64

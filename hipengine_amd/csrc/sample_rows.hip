@@ -14,9 +14,11 @@
 // over the bins, from which one workgroup a row then finds the bin B that holds the border; 3. the tokens of B in a list
 // (with top-k, all tokens down to B).  4. One workgroup a row finds the exact border inside the list, then the chunk that
 // holds the token by the chunks' weights up to B, and the token in it.
-// A list that would not fit (a row so flat that one bin holds over 16384 tokens) is replaced by the row itself.
+// A list that would not fit (a row so flat that one bin holds over 16384 tokens) is replaced by the row itself, which one
+// workgroup then reads once for every digit: one such row of 151936 takes 740 us, 64 of them 1010.
 //
 // What bounds it.  One row of 151936 with top-k 50: four launches of 4 to 8 us, each a few steps that wait for each other.
+// Nothing but a temperature: one row 22 us by the clock, 64 rows 38.
 // 64 rows with top-p 0.9 (39 MB): 11 + 16 + 5 + 15 + 16 us; the passes over the logits stand at what such a launch takes to
 // read them (11) plus 4 us for 10^7 weights in the second, and pass 4 at its barriers.  Sums of bins through global
 // atomics, and a counter beside the neighbouring rows', cost 15 us more: additions to one line wait for each other.
@@ -318,7 +320,9 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
   uint64_t best = 0, sum[2] = {0, 0};
   const int pair = 2 * (threadIdx.x % (BINS / 2)), part = __builtin_amdgcn_readfirstlane(threadIdx.x / (BINS / 2));
   if (g.t > 0.0f && (g.k > 0 || g.p < 1.0f || g.m > 0.0f)) {   // (what no histogram was written for is not used)
-    constexpr int AHEAD = 20;                          // loads on their way, the last few too: not a loop over the rest
+    // Loads on their way, the last few too: not a loop over the rest. 20 make two rounds of the 38 chunks of 151936 logits, 16
+    // made three (one row: 7.3 us for the pass against 7.8); more take registers and gain nothing.
+    constexpr int AHEAD = 20;
     for (int c0 = part; c0 < a.chunks; c0 += AHEAD * PARTS) {
       uint64_t v[AHEAD][2] = {};
 #pragma unroll

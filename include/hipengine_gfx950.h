@@ -894,6 +894,7 @@ int hipengine_gfx950_moe_tile_map(const int64_t* expert_start_compact, int64_t* 
  *                   -127..127, in blocks of 32 tokens.  K block: [head_dim / 16][32 tokens][16]; V block:
  *                   [head_dim][32], token t at place (t & 3) | (t >> 3 & 3) << 2 | (t >> 2 & 1) << 4.
  *   k_scale, v_scale  float32 [pages, kv_heads, page_size / 32]: value = q * scale.  A scale under 2^-64 counts as 2^-64.
+ *                   Attention holds V's scales of up to 2^100, at most 2^100 apart within a sequence.
  *   page_size       tokens of a page: a power of two, 32 .. 2^20
  *   page_table      int32 [batch, table_stride] page numbers.  A number outside 0 .. pages - 1 is no page: tokens on it are
  *                   not written, read as zeros and not attended to.  Entries behind a sequence's end are not looked at.
