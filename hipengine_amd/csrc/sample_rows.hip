@@ -321,7 +321,7 @@ __device__ __forceinline__ void find_cut(const Args& a, int64_t row, CutLds<N>& 
   const int pair = 2 * (threadIdx.x % (BINS / 2)), part = __builtin_amdgcn_readfirstlane(threadIdx.x / (BINS / 2));
   if (g.t > 0.0f && (g.k > 0 || g.p < 1.0f || g.m > 0.0f)) {   // (what no histogram was written for is not used)
     // Loads on their way, the last few too: not a loop over the rest. 20 make two rounds of the 38 chunks of 151936 logits, 16
-    // made three (one row: 7.3 us for the pass against 7.8); more take registers and gain nothing.
+    // made three (one row: 7.3 us for the pass against 7.8).
     constexpr int AHEAD = 20;
     for (int c0 = part; c0 < a.chunks; c0 += AHEAD * PARTS) {
       uint64_t v[AHEAD][2] = {};

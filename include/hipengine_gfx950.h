@@ -943,11 +943,12 @@ int hipengine_gfx950_kv_read_q8(const uint8_t* k_cache, const uint8_t* v_cache, 
 /* out = softmax(softmax_scale * q K^T) V for q, out [tokens, q_heads, head_dim], bf16 or fp16 (`kind`, of both).  The query
  * in row i of n of sequence b is at place kv_lens[b] - n + i and sees the places up to its own (window > 0: the last
  * `window` of them); q head h reads KV head h / (q_heads / kv_heads).  A query that sees nothing gives zeros; rows of no
- * sequence are left as they were.  K, V and bf16 or fp16 q go into the products as they are, the softmax's weights rounded
- * to fp16 (and counted so in their sum), products, sums and statistics in float32.  At most 2^26 tokens, 4096 query heads, a
- * window of 2^30, and 65535 * 128 rows (65535 * 256 of head_dim 256) of a sequence for a KV head: min(max_q_len, tokens) *
- * (q_heads / kv_heads).  `workspace` (16-byte aligned, the size that the function below gives for the same
- * sizes; null if 0) is scratch: calls that overlap in time need one each.  Results do not depend on timing. */
+ * sequence are left as they were.  K, V and q go into the products as they are (bf16 q down to 2^-24 of a row's largest
+ * value), the softmax's weights rounded to fp16 and counted so in their sum; products, sums and statistics are float32.
+ * At most 2^26 tokens, 4096 query heads, a window of 2^30, and 65535 * 128 rows (65535 * 256 of head_dim 256) of a sequence
+ * for a KV head: min(max_q_len, tokens) * (q_heads / kv_heads).  `workspace` (16-byte aligned, the size that the function
+ * below gives for the same sizes; null if 0) is scratch: calls that overlap in time need one each.  Results do not depend on
+ * timing. */
 int hipengine_gfx950_paged_attention_q8(const void* q, void* out, int32_t kind, int64_t q_stride, int64_t out_stride,
                                         const uint8_t* k_cache, const uint8_t* v_cache, const float* k_scale,
                                         const float* v_scale, const int32_t* page_table, int64_t table_stride,
